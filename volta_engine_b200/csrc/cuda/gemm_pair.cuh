@@ -1,0 +1,234 @@
+// Matrix products on pairs of CTAs (tcgen05 cta_group::2) with 32-bit sums that do not lose bits along K.
+//
+//   D[m, n] = sum over operand pairs (a, b) and over k of A_a[m, k] * B_b[n, k]
+//
+// Tile: 256 x 256 a pair, each CTA holds 128 rows of A, 128 of the 256 rows of B and 128 x 256 of the sums. A step of 64 along K brings
+// 32 KB to each CTA for 512 cycles of its tensor core, half of what a 128 x 256 tile of one CTA asks of L2. Either operand is K-major
+// ([rows, K]) or MN-major ([K, rows]).
+//
+// Sums. The tensor core cuts each addition to its accumulator off instead of rounding it: against 64 bits a sum over K = 5120 of random
+// products is 5.6e-6 too small (4.7e-6 of that is bias), over 16384 it is 1.9e-5, where fp32 FMAs are 7e-7 and 1.5e-6 off; pieces of 256
+// along K are 2.2e-7 off. So a sum stays in tensor memory for `chunk` steps only; two buffers of 256 columns alternate, and eight warps add
+// each finished piece to registers (128 sums a thread) with ordinary rounding while the next one runs.
+//
+// Operands of more than bf16 precision come as slabs: an fp32 value is the exact sum of three bf16 values (8 + 8 + 8 bits), and the product
+// is summed over the pairs of slabs whose orders add up to two at most (what is left out is below 2^-24 of the product).
+//
+// Roles (320 threads a CTA): warp 0 loads by TMA, warp 1 of the pair's first CTA issues the MMAs, warps 2..9 sum and run the epilogue.
+// Every wait is bounded.
+#pragma once
+#include "common.cuh"
+
+namespace ve {
+
+constexpr int kPairStages = 6, kPairHalf = 128 * 128, kPairStage = 2 * kPairHalf;       // bytes: 128 rows x 64 of A and of B
+constexpr int kPairSmem = kPairStages * kPairStage + 1024;
+constexpr int kPairClusters = 74, kPairThreads = 320;
+
+VE_DEVINL uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+VE_DEVINL uint32_t first_cta_addr(const void* p) {          // the same shared-memory object in the pair's first CTA
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+  return a;
+}
+VE_DEVINL void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+VE_DEVINL void mbar_arrive_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// A load into this CTA's shared memory that reports to a barrier of the pair's first CTA.
+VE_DEVINL void tma_load_3d_pair(void* smem_dst, const CUtensorMap* map, uint32_t bar_cluster, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(map), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+VE_DEVINL void tmem_alloc_pair(uint32_t* smem_holder, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_holder)), "r"(ncols) : "memory");
+}
+VE_DEVINL void tmem_relinquish_pair() { asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory"); }
+VE_DEVINL void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// Arrive on the barrier at this address in both CTAs when the MMAs issued so far are complete.
+VE_DEVINL void tc_commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+VE_DEVINL void tc_mma_f16_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// What one tile covers. Rows and columns count from the operands' own origins; steps of 64 along K.
+struct PairTile {
+  int m0, n0;                 // first row / column of the 256 x 256 tile
+  int k0, ksteps;             // first step and number of steps (of each pair of slabs)
+  int split;
+};
+
+struct PairLoop {
+  int pairs;                  // pairs of slabs
+  uint32_t a_slab, b_slab;    // four bits each
+  int chunk;                  // steps that a sum stays in tensor memory
+};
+
+// The pairs (i, j) of `sa` x `sb` slabs with i + j <= order, the small ones first.
+static inline PairLoop pair_loop(int sa, int sb, int order, int chunk) {
+  PairLoop l{0, 0, 0, chunk};
+  for (int o = order; o >= 0; --o)
+    for (int i = 0; i < sa; ++i) {
+      const int j = o - i;
+      if (j < 0 || j >= sb) continue;
+      l.a_slab |= (uint32_t)i << (4 * l.pairs);
+      l.b_slab |= (uint32_t)j << (4 * l.pairs);
+      ++l.pairs;
+    }
+  return l;
+}
+
+// Job: gives the tiles (int tiles(), PairTile tile(int i)) and takes the sums of a thread: finish(tile, row of the tile, first column, sums[128]).
+// A_MN / B_MN: the operand is MN-major.
+template <bool A_MN, bool B_MN, class Job>
+VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap* amap, const CUtensorMap* bmap, int* status) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_holder;
+  __shared__ int s_fail;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_rank(), cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 16); }
+    s_fail = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) { tmem_alloc_pair(&tmem_holder, 512); tmem_relinquish_pair(); }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                       // the pair's barriers stand before either CTA signals them
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_holder;
+  const int ntiles = job.tiles();
+
+  if (warp == 0) {
+    if (elect_one()) {
+      prefetch_tmap(amap);
+      prefetch_tmap(bmap);
+      int it = 0;
+      bool ok = true;
+      for (int t = cluster; t < ntiles && ok; t += clusters) {
+        const PairTile tl = job.tile(t);
+        const int am = tl.m0 + rank * 128, bn = tl.n0 + rank * 128;
+        for (int p = 0; p < loop.pairs && ok; ++p) {
+          const int sa = (loop.a_slab >> (4 * p)) & 15, sb = (loop.b_slab >> (4 * p)) & 15;
+          for (int k = 0; k < tl.ksteps; ++k, ++it) {
+            const int s = it % kPairStages;
+            ok = mbar_wait(&empty[s], ((it / kPairStages) & 1) ^ 1);
+            if (!ok) break;
+            uint8_t* st = smem + s * kPairStage;
+            if (rank == 0) mbar_expect_tx(&full[s], 2 * kPairStage);
+            const uint32_t bar = first_cta_addr(&full[s]);
+            const int kk = (tl.k0 + k) * 64;
+            if (A_MN) {
+              tma_load_3d_pair(st, amap, bar, am, kk, sa);
+              tma_load_3d_pair(st + kPairHalf / 2, amap, bar, am + 64, kk, sa);
+            } else {
+              tma_load_3d_pair(st, amap, bar, kk, am, sa);
+            }
+            if (B_MN) {
+              tma_load_3d_pair(st + kPairHalf, bmap, bar, bn, kk, sb);
+              tma_load_3d_pair(st + kPairHalf + kPairHalf / 2, bmap, bar, bn + 64, kk, sb);
+            } else {
+              tma_load_3d_pair(st + kPairHalf, bmap, bar, kk, bn, sb);
+            }
+          }
+        }
+      }
+      if (!ok) atomicExch(&s_fail, 1);
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = make_idesc_f16(1, 1, 256, 256) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+      int it = 0, piece = 0;
+      bool ok = true;
+      for (int t = cluster; t < ntiles && ok; t += clusters) {
+        const int total = job.tile(t).ksteps * loop.pairs;
+        for (int i = 0; i < total && ok; ++piece) {
+          const int buf = piece & 1;
+          ok = mbar_wait(&acc_empty[buf], ((piece >> 1) & 1) ^ 1);
+          if (!ok) break;
+          tc_fence_after();
+          const int end = min(total, i + loop.chunk);
+          for (bool first = true; i < end; ++i, ++it, first = false) {
+            const int s = it % kPairStages;
+            ok = mbar_wait(&full[s], (it / kPairStages) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t a = smem_u32(smem + s * kPairStage), b = a + kPairHalf;
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb) {
+              const uint64_t ad = A_MN ? make_desc_sw128_mn(a + kb * 2048, kPairHalf / 2, 1024) : make_desc_sw128(a) + kb * 2;
+              const uint64_t bd = B_MN ? make_desc_sw128_mn(b + kb * 2048, kPairHalf / 2, 1024) : make_desc_sw128(b) + kb * 2;
+              tc_mma_f16_pair(tmem_base + buf * 256, ad, bd, idesc, (first && kb == 0) ? 0u : 1u);
+            }
+            tc_commit_pair(&empty[s]);
+          }
+          if (ok) tc_commit_pair(&acc_full[buf]);
+        }
+      }
+      if (!ok) atomicExch(&s_fail, 1);
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
+    int piece = 0;
+    bool ok = true;
+    for (int t = cluster; t < ntiles; t += clusters) {
+      const PairTile tl = job.tile(t);
+      const int total = tl.ksteps * loop.pairs, pieces = (total + loop.chunk - 1) / loop.chunk;
+      float acc[128];
+#pragma unroll
+      for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < pieces; ++c, ++piece) {
+        const int buf = piece & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (piece >> 1) & 1));
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          uint32_t r[32];
+          tmem_ld32(taddr + buf * 256 + g * 32, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[g * 32 + j] += __uint_as_float(r[j]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(first_cta_addr(&acc_empty[buf]));
+      }
+      if (!ok) break;
+      job.finish(tl, rank * 128 + quarter * 32 + lane, half * 128, acc);
+    }
+    if (!ok) atomicExch(&s_fail, 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                       // no CTA leaves while its pair may still signal or read it
+  if (warp == 1) { __syncwarp(); tc_fence_after(); tmem_dealloc_pair(tmem_base, 512); }
+  if (threadIdx.x == 0 && s_fail && status) atomicExch(status, (int)kErrMbarTimeout);
+}
+
+}  // namespace ve

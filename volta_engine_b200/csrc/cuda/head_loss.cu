@@ -1,0 +1,748 @@
+// Losses of a language model head without its logits: softmax cross entropy against labels, and KL(teacher || model) against a teacher's
+// K most likely tokens and the mass of the rest; both with the gradients of the states and of the head.
+//
+//   z_rv = cap(sum_h x_rh W_vh),  cap(z) = c tanh(z / c) or z        s_rv = exp(z_rv - lse_r),  lse_r = log sum_v exp z_rv
+//   cross entropy   nll_r = lse_r - z_ry = log(1 + exp(rest_r - z_ry))                     rest_r = log sum_{v != y} exp z_rv
+//   divergence      kl_r  = sum_k a_k (log a_k - log s_k) + t (log t - log max(rho_r, 1e-12))    rho_r = exp(rest_r - lse_r), rest over v not in K
+//   gradients       dz_rv = g_r s_rv ((A + t) - [v not in K] t / rho_r) - g_r [v in K] a_v,  A = sum_k a_k
+//                   (the label is a teacher of one token: A = 1, t = 0; its own dz is -g exp(rest - lse), which does not cancel)
+//                   dx = (dz cap') W,  dW = (dz cap')^T x
+//
+// The logits exist a 256 x 256 tile at a time, in registers (gemm_pair.cuh). Scoring keeps of each row and 128 columns the maximum and the sum
+// of exponentials without the targets, and the targets' logits; one more pass over these few numbers gives the loss. The targets are left
+// out of the sums so that log(1 + exp(..)) and log(rho) do not come from the difference of two nearly equal numbers. The gradient computes the
+// logits again, a piece of the vocabulary at a time, writes dz of that piece in bf16 slabs (rows x piece: the only array of that kind) and
+// multiplies it with the head's rows and with the states. dz is rounded to the operands' precision: bf16 for bf16 states (half a unit, 2^-9 of its
+// value, as the rounding of the gradient itself), three bf16 slabs (fp32's 24 bits) for fp32 states.
+// Sums run in a fixed order: the same call gives the same bits.
+//
+// Rows that are left out (label below zero, a teacher row of padding) are taken out in front: the states of the others are gathered, so what
+// stands in the rest is never read, and time goes by the rows that count. The number of rows stays on the device.
+#include "common.cuh"
+#include "gemm_pair.cuh"
+#include "tmap.h"
+
+namespace ve {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxTopk = 1024;
+
+VE_DEVINL float neg_inf() { return __int_as_float(0xff800000); }
+
+// ------------------------------------------------------------------------------------------------ rows and operands
+struct HeadRows {
+  const void* labels;         // cross entropy: int32 or int64 [R]
+  int label_bytes;
+  const int* ids;             // divergence: [R, K]
+  const float *logp, *tail;   // [R, K], [R]
+  int K, R, V;
+};
+
+// Divergence: the teacher's tokens of a row in ascending order, with their places: sid / slp [R, K] (padding behind, as INT_MAX), and at
+// off[r, b] the first one at or behind column 128 b. One block a row, counting ranks: K is small.
+__global__ void __launch_bounds__(128) head_targets_kernel(const HeadRows p, int nblk, int* sid, float* slp, uint16_t* off, int* flag) {
+  __shared__ int id[kMaxTopk], srt[kMaxTopk];
+  const int r = blockIdx.x;
+  int any = 0;
+  for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
+    const int v = p.ids[(size_t)r * p.K + k];
+    id[k] = v < 0 ? INT_MAX : v;
+    any |= v >= 0;
+  }
+  any = __syncthreads_or(any);
+  if (threadIdx.x == 0) flag[r] = any;
+  if (!any) return;                                   // (uniform)
+  for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
+    const int v = id[k];
+    int at = 0;
+    for (int j = 0; j < p.K; ++j) at += id[j] < v || (id[j] == v && j < k);
+    srt[at] = v;
+    sid[(size_t)r * p.K + at] = v;
+    slp[(size_t)r * p.K + at] = v == INT_MAX ? neg_inf() : p.logp[(size_t)r * p.K + k];
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b <= nblk; b += blockDim.x) {
+    int lo = 0, hi = p.K;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (srt[mid] < b * 128) lo = mid + 1; else hi = mid;
+    }
+    off[(size_t)r * (nblk + 1) + b] = (uint16_t)lo;
+  }
+}
+
+VE_DEVINL long label_of(const HeadRows& p, int r) {
+  return p.label_bytes == 8 ? (long)reinterpret_cast<const long long*>(p.labels)[r] : (long)reinterpret_cast<const int*>(p.labels)[r];
+}
+
+// The rows that count, in order: live[i] = row, pos[row] = i or -1, *count.
+__global__ void __launch_bounds__(1024) head_rows_kernel(const HeadRows p, const int* flag, int* live, int* pos, int* count) {
+  __shared__ int part[32], base;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) base = 0;
+  __syncthreads();
+  for (int r0 = 0; r0 < p.R; r0 += 1024) {
+    const int r = r0 + threadIdx.x;
+    const bool on = r < p.R && (p.labels ? label_of(p, r) >= 0 : flag[r] != 0);
+    const unsigned mask = __ballot_sync(0xffffffffu, on);
+    if (lane == 0) part[warp] = __popc(mask);
+    __syncthreads();
+    int before = base;
+    for (int w = 0; w < warp; ++w) before += part[w];
+    const int at = before + __popc(mask & ((1u << lane) - 1));
+    if (r < p.R) pos[r] = on ? at : -1;
+    if (on) live[at] = r;
+    __syncthreads();
+    if (threadIdx.x == 1023) base = at + (on ? 1 : 0);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *count = base;
+}
+
+VE_DEVINL float split_bf16(float v, __nv_bfloat16& out) {     // rounds v, returns what is left of it
+  out = f2bf(v);
+  return v - bf2f(out);
+}
+
+// Four values into the slabs of a row (an infinity or a NaN leaves NaN in the slabs behind the first).
+VE_DEVINL void store_slabs4(__nv_bfloat16* dst, size_t slab, int slabs, float4 v) {
+  for (int s = 0; s < slabs; ++s) {
+    __nv_bfloat16 b[4];
+    v.x = split_bf16(v.x, b[0]); v.y = split_bf16(v.y, b[1]); v.z = split_bf16(v.z, b[2]); v.w = split_bf16(v.w, b[3]);
+    *reinterpret_cast<uint2*>(dst + s * slab) = *reinterpret_cast<const uint2*>(b);
+  }
+}
+
+template <typename T>
+VE_DEVINL float4 load4(const T* row, int c, int H, bool vec) {
+  if (vec && c + 4 <= H) {
+    if (sizeof(T) == 4) return *reinterpret_cast<const float4*>(row + c);
+    const uint2 w = *reinterpret_cast<const uint2*>(row + c);
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+  }
+  float f[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = c + e < H ? (float)row[c + e] : 0.f;
+  return make_float4(f[0], f[1], f[2], f[3]);
+}
+
+// Rows of a matrix as bf16 slabs [slabs][rows of a slab][Hp], zeros behind column H. With `live`: the gathered rows, and zeros behind the last
+// one to the end of its tile of 256 (the products along rows read them).
+template <typename T>
+__global__ void __launch_bounds__(256) head_pack_kernel(const T* src, long ld, const int* live, const int* count, int rows, int H, int Hp, int slabs,
+                                                        size_t slab, __nv_bfloat16* dst) {
+  const bool vec = !((uintptr_t)src & (4 * sizeof(T) - 1)) && ld % 4 == 0;
+  const int n = live ? *count : rows, all = live ? (n + 255) / 256 * 256 : rows;
+  const int per = Hp / 4;
+  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < (size_t)all * per; i += (size_t)gridDim.x * blockDim.x) {
+    const int r = (int)(i / per), c = (int)(i - (size_t)r * per) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < n) v = load4(src + (live ? live[r] : r) * ld, c, H, vec);
+    store_slabs4(dst + (size_t)r * Hp + c, slab, slabs, v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ jobs of the paired GEMM
+struct Targets {              // by row of the caller
+  const void* labels;
+  int label_bytes;
+  const int* sid;             // [R, K]
+  const float* slp;
+  const uint16_t* off;        // [R, nblk + 1]
+  int K, nblk;
+  VE_DEVINL void range(int row, int blk, long col0, int cols, int& begin, int& end) const {      // targets of a row among 128 columns
+    if (labels) {
+      const long y = label_bytes == 8 ? (long)reinterpret_cast<const long long*>(labels)[row] : (long)reinterpret_cast<const int*>(labels)[row];
+      begin = 0;
+      end = y >= col0 && y < col0 + cols;
+    } else {
+      const uint16_t* o = off + (size_t)row * (nblk + 1) + blk;
+      begin = o[0];
+      end = o[1];
+    }
+  }
+  VE_DEVINL int id(int row, int p) const {
+    if (labels) return label_bytes == 8 ? (int)reinterpret_cast<const long long*>(labels)[row] : reinterpret_cast<const int*>(labels)[row];
+    return sid[(size_t)row * K + p];
+  }
+};
+
+struct LogitTiles {           // rows x a piece of the vocabulary: tiles of up to 16 row tiles share the head's rows while L2 holds them
+  const int* count;
+  int v0, nv, ksteps;
+  VE_DEVINL int row_tiles() const { return (*count + 255) >> 8; }
+  VE_DEVINL int tiles() const { return row_tiles() * ((nv + 255) >> 8); }
+  VE_DEVINL PairTile tile(int i) const {
+    const int nm = row_tiles(), nn = (nv + 255) >> 8, per = 16 * nn;
+    const int g = i / per, m_first = g * 16, gm = min(16, nm - m_first), j = i - g * per;
+    return PairTile{(m_first + j % gm) * 256, (j / gm) * 256, 0, ksteps, 0};
+  }
+};
+
+template <bool CAP>
+VE_DEVINL void cap_logits(float* z, float cap, float inv_cap) {
+  if (CAP) {
+#pragma unroll
+    for (int j = 0; j < 128; ++j) z[j] = cap * tanhf(z[j] * inv_cap);
+  }
+}
+
+template <bool CAP>
+struct ScoreJob : LogitTiles {
+  Targets tg;
+  const int* live;
+  int rows_cap;               // pitch of part
+  float2* part;               // [128-column block][row]: maximum and sum of exp(z - maximum) without the targets
+  float* zt;                  // [R, K] logits of the targets, in the targets' ascending order
+  float cap, inv_cap;
+
+  VE_DEVINL void finish(const PairTile& t, int r, int c0, float* z) const {
+    const int i = t.m0 + r, n = *count;
+    if (t.m0 + (r & ~31) >= n || t.n0 + c0 >= nv) return;
+    const bool on = i < n;
+    const int row = on ? live[i] : 0;
+    const int col0 = t.n0 + c0, cols = min(128, nv - col0), blk = (v0 + col0) >> 7;
+    int p = 0, end = 0;
+    if (on) tg.range(row, blk, (long)v0 + col0, cols, p, end);
+    cap_logits<CAP>(z, cap, inv_cap);
+    if (cols < 128) {
+#pragma unroll
+      for (int j = 0; j < 128; ++j)
+        if (j >= cols) z[j] = neg_inf();
+    }
+    if (__any_sync(0xffffffffu, p < end)) {
+      int next = p < end ? tg.id(row, p) - v0 - col0 : 128;
+#pragma unroll
+      for (int j = 0; j < 128; ++j)
+        if (j == next) {
+          do {                                      // (a token listed twice is one token)
+            zt[(size_t)row * tg.K + p] = z[j];
+            next = ++p < end ? tg.id(row, p) - v0 - col0 : 128;
+          } while (j == next);
+          z[j] = neg_inf();
+        }
+    }
+    float m = z[0];
+#pragma unroll
+    for (int j = 1; j < 128; ++j) m = fmaxf(m, z[j]);
+    const float m2 = m == neg_inf() ? 0.f : -(m * kLog2e);
+    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 128; j += 4) {
+      s0 += ex2_approx(fmaf(z[j], kLog2e, m2));
+      s1 += ex2_approx(fmaf(z[j + 1], kLog2e, m2));
+      s2 += ex2_approx(fmaf(z[j + 2], kLog2e, m2));
+      s3 += ex2_approx(fmaf(z[j + 3], kLog2e, m2));
+    }
+    if (on) part[(size_t)blk * rows_cap + i] = make_float2(m, (s0 + s1) + (s2 + s3));
+  }
+};
+
+// Constants of a row's dz: at any token dense * s, at a target `at` * s - g * (teacher's mass); a label's is `at` itself.
+struct RowGrad {
+  float lse2, dense, at, g;
+};
+
+template <bool CAP>
+struct GradJob : LogitTiles {
+  Targets tg;
+  const int* live;
+  const RowGrad* rg;          // by gathered row
+  __nv_bfloat16* G;           // [slabs][rows_cap][pitch]
+  size_t slab;
+  int slabs, pitch;
+  float cap, inv_cap;
+
+  VE_DEVINL void finish(const PairTile& t, int r, int c0, float* z) const {
+    const int i = t.m0 + r, n = *count;
+    const bool on = i < n;
+    const int col0 = t.n0 + c0, cols = max(0, min(128, nv - col0));
+    __nv_bfloat16* dst = G + (size_t)i * pitch + col0;
+    const int row = on ? live[i] : 0;
+    int p = 0, end = 0;
+    RowGrad c{0.f, 0.f, 0.f, 0.f};
+    if (on) {
+      c = rg[i];
+      if (cols) tg.range(row, (v0 + col0) >> 7, (long)v0 + col0, cols, p, end);
+    }
+    const bool any = __any_sync(0xffffffffu, p < end);
+    int next = p < end ? tg.id(row, p) - v0 - col0 : 128;
+#pragma unroll
+    for (int j = 0; j < 128; ++j) {
+      float slope = 1.f, v = z[j];
+      if (CAP) {
+        const float th = tanhf(v * inv_cap);
+        v = cap * th;
+        slope = 1.f - th * th;
+      }
+      const float s = ex2_approx(fmaf(v, kLog2e, -c.lse2));
+      float d = c.dense * s;
+      if (any && j == next) {
+        if (tg.labels) {
+          d = c.at;
+          next = 128;
+        } else {
+          float a = 0.f;
+          do {
+            a += expf(tg.slp[(size_t)row * tg.K + p]);
+            next = ++p < end ? tg.id(row, p) - v0 - col0 : 128;
+          } while (j == next);
+          d = fmaf(c.at, s, -c.g * a);
+        }
+      }
+      if (CAP) d *= slope;
+      z[j] = on && j < cols ? d : 0.f;              // (zeros to the ends of the tile: the products along rows and columns read them)
+    }
+    for (int s = 0; s < slabs; ++s) {
+#pragma unroll
+      for (int j = 0; j < 128; j += 8) {
+        __nv_bfloat16 b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[j + e] = split_bf16(z[j + e], b[e]);
+        *reinterpret_cast<uint4*>(dst + s * slab + j) = *reinterpret_cast<const uint4*>(b);
+      }
+    }
+  }
+};
+
+// dx: gathered rows x H, along a piece of the vocabulary, cut into `splits` ranges that keep their own fp32 sums.
+struct DxJob {
+  const int* count;
+  int H, Hp, ksteps, splits, first;
+  size_t slab;
+  float* acc;                 // [splits][rows_cap][Hp]
+  VE_DEVINL int row_tiles() const { return (*count + 255) >> 8; }
+  VE_DEVINL int tiles() const { return row_tiles() * ((H + 255) >> 8) * splits; }
+  VE_DEVINL PairTile tile(int i) const {
+    const int nm = row_tiles(), per = (ksteps + splits - 1) / splits;
+    const int m = i % nm, j = i / nm, s = j % splits;
+    return PairTile{m * 256, (j / splits) * 256, s * per, max(0, min(per, ksteps - s * per)), s};
+  }
+  VE_DEVINL void finish(const PairTile& t, int r, int c0, float* z) const {
+    const int i = t.m0 + r;
+    if (i >= *count) return;
+    float* dst = acc + t.split * slab + (size_t)i * Hp + t.n0 + c0;
+    const int cols = Hp - t.n0 - c0;
+#pragma unroll
+    for (int j = 0; j < 128; j += 4) {
+      if (j >= cols) continue;
+      float4 v = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
+      if (!first) {
+        const float4 o = *reinterpret_cast<const float4*>(dst + j);
+        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+      }
+      *reinterpret_cast<float4*>(dst + j) = v;
+    }
+  }
+};
+
+// dW: a piece of the vocabulary x H, along the gathered rows.
+template <typename T>
+struct DheadJob {
+  const int* count;
+  int nv, H;
+  T* out;                     // [nv, H], contiguous rows
+  VE_DEVINL int tiles() const { return ((nv + 255) >> 8) * ((H + 255) >> 8); }
+  VE_DEVINL PairTile tile(int i) const {
+    const int nn = (H + 255) >> 8;
+    return PairTile{i / nn * 256, i % nn * 256, 0, (*count + 63) >> 6, 0};
+  }
+  VE_DEVINL void finish(const PairTile& t, int r, int c0, float* z) const {
+    const int v = t.m0 + r;
+    if (v >= nv) return;
+    T* dst = out + (size_t)v * H + t.n0 + c0;
+    const int cols = H - t.n0 - c0;
+    const bool vec = !((uintptr_t)out & 15) && H % (16 / (int)sizeof(T)) == 0;
+#pragma unroll
+    for (int j = 0; j < 128; j += 8) {
+      if (j >= cols) continue;
+      if (vec && j + 8 <= cols) {
+        if (sizeof(T) == 4) {
+          *reinterpret_cast<float4*>(dst + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
+          *reinterpret_cast<float4*>(dst + j + 4) = make_float4(z[j + 4], z[j + 5], z[j + 6], z[j + 7]);
+        } else {
+          __nv_bfloat16 b[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) b[e] = f2bf(z[j + e]);
+          *reinterpret_cast<uint4*>(dst + j) = *reinterpret_cast<const uint4*>(b);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (j + e < cols) dst[j + e] = (T)z[j + e];
+      }
+    }
+  }
+};
+
+template <bool A_MN, bool B_MN, class Job>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+head_gemm_kernel(const Job job, const PairLoop loop, const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, int* status) {
+  pair_gemm<A_MN, B_MN>(job, loop, &amap, &bmap, status);
+}
+
+// ------------------------------------------------------------------------------------------------ the rows' sums
+// Joins a row's blocks and computes its loss, 32 rows a block of 1024 threads: the warps share the blocks of columns, lanes are rows; then a
+// warp takes a row's targets. The few numbers behind the sums are in 64 bits: losses near zero, and divergences of near models, are differences.
+__global__ void __launch_bounds__(1024) head_merge_kernel(const HeadRows p, const int* live, const int* count, int rows_cap, int nblk, const float2* part,
+                                                          const float* zt, const int* sid, const float* slp, float* loss, float* stats) {
+  __shared__ float sm[32][33], ss[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = *count;
+  if (blockIdx.x * 32 >= n) return;
+  const int i = blockIdx.x * 32 + lane;
+  float m = neg_inf(), s = 0.f;
+  if (i < n) {
+    for (int b0 = warp; b0 < nblk; b0 += 32 * 8) {
+      float2 v[8];
+      float mx = m;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int b = b0 + 32 * e;
+        v[e] = b < nblk ? part[(size_t)b * rows_cap + i] : make_float2(neg_inf(), 0.f);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, v[e].x);
+      if (mx != neg_inf()) {
+        s *= exp2f((m - mx) * kLog2e);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += v[e].y * exp2f((v[e].x - mx) * kLog2e);
+        m = mx;
+      }
+    }
+  }
+  sm[warp][lane] = m;
+  ss[warp][lane] = s;
+  __syncthreads();
+  const int j = blockIdx.x * 32 + warp;               // this warp's row
+  if (j >= n) return;
+  const float wm = sm[lane][warp];
+  const float top = warp_max(wm);
+  const double sum = [&] {
+    double v = wm == neg_inf() ? 0.0 : (double)ss[lane][warp] * exp2((double)(wm - top) * 1.4426950408889634);
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }();
+  const int row = live[j];
+  const double rest = (double)top + log(sum);          // (no token besides the targets: minus infinity)
+  double lse, out;
+  if (p.labels) {
+    const long y = label_of(p, row);
+    const double z = zt[row], d = rest - z;
+    out = d > 0 ? d + log1p(exp(-d)) : log1p(exp(d));
+    lse = z + out;
+    if (y >= p.V) out = lse = __longlong_as_double(0x7ff8000000000000ll);
+  } else {
+    const int* id = sid + (size_t)row * p.K;
+    const float* z = zt + (size_t)row * p.K;
+    const float* lp = slp + (size_t)row * p.K;
+    // sum over the targets: each token once
+    double mx = rest;
+    bool bad = false;
+    for (int k = lane; k < p.K; k += 32) {
+      bad |= id[k] >= p.V && id[k] != INT_MAX;
+      if (id[k] < p.V) mx = fmax(mx, (double)z[k]);
+    }
+    for (int o = 16; o > 0; o >>= 1) mx = fmax(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    double v = 0.0;
+    for (int k = lane; k < p.K; k += 32)
+      if (id[k] < p.V && (k == 0 || id[k - 1] != id[k])) v += exp((double)z[k] - mx);
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    lse = mx + log(v + (rest == -INFINITY ? 0.0 : exp(rest - mx)));
+    out = 0.0;
+    for (int k = lane; k < p.K; k += 32)
+      if (id[k] < p.V && lp[k] != neg_inf()) out += exp((double)lp[k]) * ((double)lp[k] - ((double)z[k] - lse));
+    for (int o = 16; o > 0; o >>= 1) out += __shfl_xor_sync(0xffffffffu, out, o);
+    const float lt = p.tail[row];
+    if (lt != neg_inf()) out += exp((double)lt) * ((double)lt - fmax(rest - lse, -27.631021115928547));     // log 1e-12
+    if (__any_sync(0xffffffffu, bad)) out = lse = __longlong_as_double(0x7ff8000000000000ll);
+  }
+  if (lane == 0) {
+    loss[row] = (float)out;
+    stats[row] = (float)lse;
+    stats[p.R + row] = (float)rest;
+  }
+}
+
+// Rows that are left out: zeros.
+__global__ void __launch_bounds__(256) head_blank_kernel(const int* pos, int R, float* loss, float* stats) {
+  const int r = blockIdx.x * blockDim.x + threadIdx.x;
+  if (r < R && pos[r] < 0) loss[r] = stats[r] = stats[R + r] = 0.f;
+}
+
+// The rows' constants of dz, a warp a row.
+__global__ void __launch_bounds__(256) head_rowgrad_kernel(const HeadRows p, const int* live, const int* count, const float* stats, const float* slp,
+                                                           const float* dloss, RowGrad* rg) {
+  const int i = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  if (i >= *count) return;
+  const int row = live[i];
+  const float lse = stats[row], rest = stats[p.R + row], g = dloss[row];
+  RowGrad c;
+  c.lse2 = lse * kLog2e;
+  c.g = g;
+  if (p.labels) {
+    c.dense = g;
+    c.at = -g * expf(rest - lse);
+  } else {
+    double a = 0.0;
+    for (int k = lane; k < p.K; k += 32) a += exp((double)slp[(size_t)row * p.K + k]);      // (padding: exp(-inf) = 0)
+    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    const double t = exp((double)p.tail[row]), lr = (double)rest - (double)lse;
+    const bool above = lr >= -27.631021115928547;
+    c.at = (float)(g * (a + (above ? t : 0.0)));
+    c.dense = (float)(g * (a + (above ? t - t * exp(-lr) : 0.0)));
+  }
+  if (lane == 0) rg[i] = c;
+}
+
+// dx of the caller's rows from the ranges' sums; zeros where a row was left out.
+template <typename T>
+__global__ void __launch_bounds__(256) head_dx_kernel(const int* pos, int R, int H, int Hp, int splits, size_t slab, const float* acc, T* dx) {
+  const int per = Hp / 4;
+  const bool vec = !((uintptr_t)dx & 15) && H % 4 == 0;
+  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < (size_t)R * per; i += (size_t)gridDim.x * blockDim.x) {
+    const int r = (int)(i / per), c = (int)(i - (size_t)r * per) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int at = pos[r];
+    if (at >= 0) {
+      const float* a = acc + (size_t)at * Hp + c;
+      for (int s = 0; s < splits; ++s) {
+        const float4 w = *reinterpret_cast<const float4*>(a + s * slab);
+        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+      }
+    }
+    T* dst = dx + (size_t)r * H + c;
+    const T o[4] = {(T)v.x, (T)v.y, (T)v.z, (T)v.w};
+    if (vec) {
+      if (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
+      else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < H) dst[e] = o[e];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+struct HeadPlan {             // sizes and places in the workspace
+  int Hp, sx, sw, sg;         // padded width; slabs of the states, the head, dz
+  int rows_cap, nblk, ksteps;
+  bool pack_head;             // the head's rows go through slabs of their own, a piece at a time
+  int piece;                  // vocabulary rows at a time (0: all at once)
+  int splits;
+  size_t live, pos, count, flag, sid, slp, off, x, part, zt, rg, head, G, acc, bytes;
+};
+
+static inline int blocks_of(size_t n, int per = 256) {
+  const size_t b = (n + per - 1) / per;
+  return (int)(b < 148 * 16 ? (b ? b : 1) : 148 * 16);
+}
+
+// Sizes of pieces: dz of a piece takes 256 MB at most, packed rows of the head 512 MB.
+static HeadPlan head_plan(bool grads, bool want_dx, int x_fp32, int head_fp32, bool pack_head, int R, int H, int V, int K, bool kl) {
+  HeadPlan p;
+  p.Hp = (H + 7) / 8 * 8;
+  p.sx = x_fp32 ? 3 : 1;
+  p.sw = head_fp32 ? 3 : 1;
+  p.sg = x_fp32 || head_fp32 ? 3 : 1;
+  p.rows_cap = (R + 255) / 256 * 256;
+  p.nblk = (V + 127) / 128;
+  p.ksteps = (H + 63) / 64;
+  p.pack_head = pack_head;
+  size_t piece = ((size_t)V + 255) / 256 * 256;
+  if (pack_head) { const size_t most = (512ull << 20) / ((size_t)p.sw * p.Hp * 2) / 256 * 256; piece = piece < most ? piece : (most ? most : 256); }
+  if (grads) { const size_t most = (256ull << 20) / ((size_t)p.sg * p.rows_cap * 2) / 256 * 256; piece = piece < most ? piece : (most ? most : 256); }
+  p.piece = (int)piece;
+  // dx: few tiles share a long vocabulary
+  const int tiles = p.rows_cap / 256 * ((H + 255) / 256);
+  const int steps = p.piece / 64;
+  p.splits = tiles >= kPairClusters ? 1 : kPairClusters / tiles;
+  while (p.splits > 1 && steps / p.splits < 8) --p.splits;
+  size_t at = 0;
+  auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
+  p.live = take(4ull * R); p.pos = take(4ull * R); p.count = take(4);
+  p.flag = p.sid = p.slp = p.off = 0;
+  if (kl) { p.flag = take(4ull * R); p.sid = take(4ull * R * K); p.slp = take(4ull * R * K); p.off = take(2ull * R * (p.nblk + 1)); }
+  p.x = take(2ull * p.sx * p.rows_cap * p.Hp);
+  p.head = pack_head ? take(2ull * p.sw * p.piece * p.Hp) : 0;
+  p.part = p.zt = p.rg = p.G = p.acc = 0;
+  if (!grads) { p.part = take(8ull * p.nblk * p.rows_cap); p.zt = take(4ull * R * (kl ? K : 1)); }
+  else {
+    p.rg = take(sizeof(RowGrad) * (size_t)p.rows_cap);
+    p.G = take(2ull * p.sg * p.rows_cap * p.piece);
+    if (want_dx) p.acc = take(4ull * p.splits * p.rows_cap * p.Hp);
+  }
+  p.bytes = at;
+  return p;
+}
+
+struct HeadCall {
+  const void* x; int x_fp32; long ldx;
+  const void* head; int head_fp32; long ldw;
+  HeadRows rows;
+  int H;
+  float softcap;
+  uint8_t* ws;
+  int* status;
+  cudaStream_t st;
+};
+
+static bool head_packs(const void* head, int head_fp32, long ldw, int H) { return head_fp32 || H % 8 || ldw % 8 || ((uintptr_t)head & 15); }
+
+static int slab_map(CUtensorMap* m, const void* base, int slabs, uint64_t slab_rows, uint64_t rows, uint64_t cols, uint64_t pitch, bool mn) {
+  return make_tmap_3d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, slabs, rows, cols, slab_rows * pitch * 2, pitch * 2, mn ? 64 : 128, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <bool A_MN, bool B_MN, class Job>
+static int launch_pair(const Job& job, const PairLoop& loop, const CUtensorMap& a, const CUtensorMap& b, const HeadCall& c) {
+  cudaError_t e = allow_smem<head_gemm_kernel<A_MN, B_MN, Job>>(kPairSmem);
+  if (e != cudaSuccess) return (int)e;
+  head_gemm_kernel<A_MN, B_MN, Job><<<2 * kPairClusters, kPairThreads, kPairSmem, c.st>>>(job, loop, a, b, c.status);
+  return (int)cudaGetLastError();
+}
+
+template <typename T>
+static void pack_rows(const void* src, long ld, const int* live, const int* count, int rows, const HeadCall& c, const HeadPlan& p, int slabs, size_t slab, void* dst) {
+  head_pack_kernel<T><<<blocks_of((size_t)rows * p.Hp / 4), 256, 0, c.st>>>((const T*)src, ld, live, count, rows, c.H, p.Hp, slabs, slab, (__nv_bfloat16*)dst);
+}
+
+// The rows that count, their targets and their states.
+static void head_front(const HeadCall& c, const HeadPlan& p) {
+  int *live = (int*)(c.ws + p.live), *pos = (int*)(c.ws + p.pos), *count = (int*)(c.ws + p.count), *flag = (int*)(c.ws + p.flag);
+  if (!c.rows.labels)
+    head_targets_kernel<<<c.rows.R, 128, 0, c.st>>>(c.rows, p.nblk, (int*)(c.ws + p.sid), (float*)(c.ws + p.slp), (uint16_t*)(c.ws + p.off), flag);
+  head_rows_kernel<<<1, 1024, 0, c.st>>>(c.rows, flag, live, pos, count);
+  const size_t slab = (size_t)p.rows_cap * p.Hp;
+  if (c.x_fp32) pack_rows<float>(c.x, c.ldx, live, count, p.rows_cap, c, p, p.sx, slab, c.ws + p.x);
+  else pack_rows<__nv_bfloat16>(c.x, c.ldx, live, count, p.rows_cap, c, p, p.sx, slab, c.ws + p.x);
+}
+
+// The head's rows [v0, v0 + nv) as an operand: in place, or packed.
+static int head_rows_map(CUtensorMap* m, const HeadCall& c, const HeadPlan& p, int v0, int nv, bool mn, bool pack) {
+  if (!p.pack_head) return slab_map(m, (const __nv_bfloat16*)c.head + (size_t)v0 * c.ldw, 1, nv, nv, c.H, c.ldw, mn);
+  if (pack) {
+    const size_t slab = (size_t)p.piece * p.Hp;
+    if (c.head_fp32) pack_rows<float>((const float*)c.head + (size_t)v0 * c.ldw, c.ldw, nullptr, nullptr, nv, c, p, p.sw, slab, c.ws + p.head);
+    else pack_rows<__nv_bfloat16>((const __nv_bfloat16*)c.head + (size_t)v0 * c.ldw, c.ldw, nullptr, nullptr, nv, c, p, p.sw, slab, c.ws + p.head);
+  }
+  return slab_map(m, c.ws + p.head, p.sw, p.piece, nv, p.Hp, p.Hp, mn);
+}
+
+static Targets head_targets_of(const HeadCall& c, const HeadPlan& p) {
+  return Targets{c.rows.labels, c.rows.label_bytes, (const int*)(c.ws + p.sid), (const float*)(c.ws + p.slp), (const uint16_t*)(c.ws + p.off),
+                 c.rows.labels ? 1 : c.rows.K, p.nblk};
+}
+
+constexpr int kExactChunk = 4;         // steps of 64 between fp32 additions where 32 bits are asked for
+constexpr int kRoundedChunk = 16;      // where the result is rounded to bf16 (cut-off sums over 1024: 1e-6)
+
+template <bool CAP>
+static int head_score(const HeadCall& c, const HeadPlan& p, float* loss, float* stats) {
+  head_front(c, p);
+  const int *live = (const int*)(c.ws + p.live), *pos = (const int*)(c.ws + p.pos), *count = (const int*)(c.ws + p.count);
+  CUtensorMap xm, wm;
+  int rc = slab_map(&xm, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, false);
+  if (rc) return rc;
+  ScoreJob<CAP> job;
+  job.count = count; job.ksteps = p.ksteps; job.tg = head_targets_of(c, p); job.live = live; job.rows_cap = p.rows_cap;
+  job.part = (float2*)(c.ws + p.part); job.zt = (float*)(c.ws + p.zt); job.cap = c.softcap; job.inv_cap = CAP ? 1.f / c.softcap : 0.f;
+  for (int v0 = 0; v0 < c.rows.V; v0 += p.piece) {
+    job.v0 = v0;
+    job.nv = c.rows.V - v0 < p.piece ? c.rows.V - v0 : p.piece;
+    if ((rc = head_rows_map(&wm, c, p, v0, job.nv, false, true))) return rc;
+    if ((rc = launch_pair<false, false>(job, pair_loop(p.sx, p.sw, 2, kExactChunk), xm, wm, c))) return rc;
+  }
+  head_merge_kernel<<<(c.rows.R + 31) / 32, 1024, 0, c.st>>>(c.rows, live, count, p.rows_cap, p.nblk, job.part, job.zt, job.tg.sid, job.tg.slp, loss, stats);
+  head_blank_kernel<<<(c.rows.R + 255) / 256, 256, 0, c.st>>>(pos, c.rows.R, loss, stats);
+  return (int)cudaGetLastError();
+}
+
+template <bool CAP>
+static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, const float* dloss, void* dx, void* dhead) {
+  head_front(c, p);
+  const int *live = (const int*)(c.ws + p.live), *pos = (const int*)(c.ws + p.pos), *count = (const int*)(c.ws + p.count);
+  const int R = c.rows.R, H = c.H;
+  RowGrad* rg = (RowGrad*)(c.ws + p.rg);
+  head_rowgrad_kernel<<<(R + 7) / 8, 256, 0, c.st>>>(c.rows, live, count, stats, (const float*)(c.ws + p.slp), dloss, rg);
+  CUtensorMap xk, xmn, wk, wmn, gk, gmn;
+  int rc = slab_map(&xk, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, false);
+  if (!rc) rc = slab_map(&xmn, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, true);
+  if (!rc) rc = slab_map(&gk, c.ws + p.G, p.sg, p.rows_cap, p.rows_cap, p.piece, p.piece, false);
+  if (!rc) rc = slab_map(&gmn, c.ws + p.G, p.sg, p.rows_cap, p.rows_cap, p.piece, p.piece, true);
+  if (rc) return rc;
+  GradJob<CAP> gj;
+  gj.count = count; gj.ksteps = p.ksteps; gj.tg = head_targets_of(c, p); gj.live = live; gj.rg = rg; gj.G = (__nv_bfloat16*)(c.ws + p.G);
+  gj.slab = (size_t)p.rows_cap * p.piece; gj.slabs = p.sg; gj.pitch = p.piece; gj.cap = c.softcap; gj.inv_cap = CAP ? 1.f / c.softcap : 0.f;
+  DxJob xj{count, H, p.Hp, 0, p.splits, 1, (size_t)p.rows_cap * p.Hp, (float*)(c.ws + p.acc)};
+  for (int v0 = 0; v0 < c.rows.V; v0 += p.piece) {
+    const int nv = c.rows.V - v0 < p.piece ? c.rows.V - v0 : p.piece;
+    gj.v0 = v0;
+    gj.nv = nv;
+    if ((rc = head_rows_map(&wk, c, p, v0, nv, false, true))) return rc;
+    if ((rc = launch_pair<false, false>(gj, pair_loop(p.sx, p.sw, 2, kExactChunk), xk, wk, c))) return rc;
+    if (dx) {
+      if ((rc = head_rows_map(&wmn, c, p, v0, nv, true, false))) return rc;
+      xj.ksteps = (nv + 63) / 64;
+      xj.first = v0 == 0;
+      const PairLoop loop = c.x_fp32 ? pair_loop(p.sg, p.sw, 2, kExactChunk) : pair_loop(p.sg, p.sw, p.sg > 1 ? 1 : 0, kRoundedChunk);
+      if ((rc = launch_pair<false, true>(xj, loop, gk, wmn, c))) return rc;
+    }
+    if (dhead) {
+      if (c.head_fp32) {
+        const DheadJob<float> job{count, nv, H, (float*)dhead + (size_t)v0 * H};
+        rc = launch_pair<true, true>(job, pair_loop(p.sg, p.sx, 2, kExactChunk), gmn, xmn, c);
+      } else {
+        const DheadJob<__nv_bfloat16> job{count, nv, H, (__nv_bfloat16*)dhead + (size_t)v0 * H};
+        rc = launch_pair<true, true>(job, pair_loop(p.sg, p.sx, p.sg > 1 ? 1 : 0, kRoundedChunk), gmn, xmn, c);
+      }
+      if (rc) return rc;
+    }
+  }
+  if (dx) {
+    const int grid = blocks_of((size_t)R * p.Hp / 4);
+    if (c.x_fp32) head_dx_kernel<float><<<grid, 256, 0, c.st>>>(pos, R, H, p.Hp, p.splits, xj.slab, xj.acc, (float*)dx);
+    else head_dx_kernel<__nv_bfloat16><<<grid, 256, 0, c.st>>>(pos, R, H, p.Hp, p.splits, xj.slab, xj.acc, (__nv_bfloat16*)dx);
+  }
+  return (int)cudaGetLastError();
+}
+
+}  // namespace ve
+
+using namespace ve;
+
+extern "C" {
+
+// Bytes of workspace that a call needs (256-byte aligned).
+long ve_head_loss_workspace(int grads, int want_dx, int x_fp32, const void* head, int head_fp32, long ldw, int R, int H, int V, int K, int kl) {
+  return (long)head_plan(grads, want_dx, x_fp32, head_fp32, head_packs(head, head_fp32, ldw, H), R, H, V, K, kl).bytes;
+}
+
+// x [R, H] (row pitch ldx), head [V, H] (pitch ldw), each bf16 or fp32. labels (int32 / int64 [R]) or ids int32 [R, K] with logp fp32 [R, K] and
+// tail fp32 [R]. loss fp32 [R], stats fp32 [2, R]: log sum exp of all logits, and of all but the targets.
+int ve_head_loss(const void* x, int x_fp32, long ldx, const void* head, int head_fp32, long ldw, const void* labels, int label_bytes, const void* ids,
+                 const void* logp, const void* tail, int K, int R, int H, int V, float softcap, void* loss, void* stats, void* ws, long ws_bytes, void* status,
+                 cudaStream_t st) {
+  if (R <= 0) return 0;
+  if (H <= 0 || V <= 0 || (!labels && (K < 1 || K > kMaxTopk))) return cudaErrorInvalidValue;
+  const HeadPlan p = head_plan(false, false, x_fp32, head_fp32, head_packs(head, head_fp32, ldw, H), R, H, V, K, !labels);
+  if ((size_t)ws_bytes < p.bytes) return cudaErrorInvalidValue;
+  const HeadCall c{x, x_fp32, ldx, head, head_fp32, ldw, {labels, label_bytes, (const int*)ids, (const float*)logp, (const float*)tail, K, R, V}, H, softcap,
+                   (uint8_t*)ws, (int*)status, st};
+  return softcap > 0.f ? head_score<true>(c, p, (float*)loss, (float*)stats) : head_score<false>(c, p, (float*)loss, (float*)stats);
+}
+
+// The gradients for dloss fp32 [R]: dx [R, H] in the states' type and dhead [V, H] in the head's, either may be null.
+int ve_head_loss_grad(const void* x, int x_fp32, long ldx, const void* head, int head_fp32, long ldw, const void* labels, int label_bytes, const void* ids,
+                      const void* logp, const void* tail, int K, int R, int H, int V, float softcap, const void* stats, const void* dloss, void* dx, void* dhead,
+                      void* ws, long ws_bytes, void* status, cudaStream_t st) {
+  if (R <= 0 || (!dx && !dhead)) return 0;
+  if (H <= 0 || V <= 0 || (!labels && (K < 1 || K > kMaxTopk))) return cudaErrorInvalidValue;
+  const HeadPlan p = head_plan(true, dx != nullptr, x_fp32, head_fp32, head_packs(head, head_fp32, ldw, H), R, H, V, K, !labels);
+  if ((size_t)ws_bytes < p.bytes) return cudaErrorInvalidValue;
+  const HeadCall c{x, x_fp32, ldx, head, head_fp32, ldw, {labels, label_bytes, (const int*)ids, (const float*)logp, (const float*)tail, K, R, V}, H, softcap,
+                   (uint8_t*)ws, (int*)status, st};
+  return softcap > 0.f ? head_grad<true>(c, p, (const float*)stats, (const float*)dloss, dx, dhead)
+                       : head_grad<false>(c, p, (const float*)stats, (const float*)dloss, dx, dhead);
+}
+
+}  // extern "C"

@@ -1,0 +1,304 @@
+"""Losses of a language model head that never hold its logits: softmax cross entropy against labels, and KL(teacher || model) against a teacher's
+K most likely tokens and the mass of the rest (what ``volta_ppl --topk-out`` writes); both with the gradients of the states and of the head.
+
+    z = cap(x head^T),  cap(z) = softcap * tanh(z / softcap) (softcap 0: z as it is)        s = softmax(z)
+    cross entropy   nll = log sum_v exp z_v - z_label
+    divergence      kl  = sum_k a_k (log a_k - log s_k) + t (log t - log max(r, 1e-12)),  a = exp(logp), t = exp(tail),
+                    r = the model's mass outside the teacher's tokens
+
+``x`` [rows, hidden] and ``head`` [vocab, hidden] are bf16 or fp32, each by itself; sums are 32 bits wide and the products of fp32 operands exact to
+2^-24. Rows may be strided. Losses and their sums are fp32; dx has the type of x, dhead that of head.
+
+Rows that do not count: a negative label, or a teacher row whose ids are all negative (single negative ids are padding). Their loss, statistics and
+gradients are zero and their states are not read. An id listed twice is one token whose teacher's mass is the sum. A label or id at or behind
+``vocab`` makes the row's loss NaN (and with it the gradients it takes part in): the ids stay on the device, nothing waits to look at them.
+
+GPU tensors use csrc/cuda/head_loss.cu: the explicit forward / backward pairs launch on the current stream of the tensors' device, take their
+workspace from the caching allocator and may be captured into a CUDA graph. CPU tensors run the same arithmetic in PyTorch (fp64 stays fp64).
+``head_cross_entropy_loss`` and ``head_kl_loss`` are the pairs as one differentiable call.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+
+import torch
+
+from .._lib import call, kernels, ptr
+
+MAX_TOPK = 1024
+REST_FLOOR = 1e-12                 # least probability of "any other token" in a divergence
+_DTYPES = (torch.bfloat16, torch.float32)
+
+
+# ------------------------------------------------------------------------------------------------ arguments
+def _check(x, head, softcap, others, dloss=None, stats=None):
+    """Shapes, types and devices of a call; ``others``: (name, tensor, dtypes, shape)."""
+    if x.dim() != 2 or head.dim() != 2 or x.shape[1] != head.shape[1]:
+        raise ValueError(f"states [rows, hidden] and head [vocab, hidden] are wanted: got {tuple(x.shape)} and {tuple(head.shape)}")
+    if head.shape[0] < 1 or head.shape[1] < 1:
+        raise ValueError(f"a head of {tuple(head.shape)} has no logits")
+    if max(x.shape[0], head.shape[0]) >= 1 << 24:
+        raise ValueError("rows and vocabulary have to stay below 2^24")
+    allowed = _DTYPES if x.is_cuda else _DTYPES + (torch.float64,)
+    for name, t in (("states", x), ("head", head)):
+        if t.dtype not in allowed:
+            raise TypeError(f"{name} of type {t.dtype}: bf16 and fp32 are supported")
+    if not (softcap >= 0 and math.isfinite(softcap)):
+        raise ValueError(f"softcap {softcap}: zero (none) or a positive number is wanted")
+    rows = x.shape[0]
+    if dloss is not None:
+        others = others + [("dloss", dloss, (torch.float32,) if x.is_cuda else (torch.float32, torch.float64), (rows,)),
+                           ("stats", stats, (torch.float32,) if x.is_cuda else (torch.float32, torch.float64), (2, rows))]
+    for name, t, dtypes, shape in others:
+        if t.dtype not in dtypes:
+            raise TypeError(f"{name} of type {t.dtype}: {' or '.join(str(d) for d in dtypes)} is wanted")
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{name} of shape {tuple(t.shape)}: {shape} is wanted")
+    for name, t in [("head", head)] + [(n, t) for n, t, _, _ in others]:
+        if t.device != x.device:
+            raise ValueError(f"{name} on {t.device}, states on {x.device}")
+
+
+def _label_args(x, labels):
+    return [("labels", labels, (torch.int64, torch.int32), (x.shape[0],))]
+
+
+def _teacher_args(x, ids, logp, tail):
+    if ids.dim() != 2 or not 1 <= ids.shape[1] <= MAX_TOPK:
+        raise ValueError(f"teacher ids [rows, K] with K of 1 to {MAX_TOPK} are wanted: got {tuple(ids.shape)}")
+    f = (torch.float32,) if x.is_cuda else (torch.float32, torch.float64)
+    rows, k = x.shape[0], ids.shape[1]
+    return [("ids", ids, (torch.int32,), (rows, k)), ("logp", logp, f, (rows, k)), ("tail", tail, f, (rows,))]
+
+
+def _on(device):
+    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def _rows_of(t):
+    """Rows in place where their elements lie side by side."""
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] or t.shape[0] == 0 else t.contiguous()
+
+
+_workspace_bytes = None
+
+
+def _workspace(grads, want_dx, x, head, K, kl):
+    global _workspace_bytes
+    if _workspace_bytes is None:
+        fn = kernels().ve_head_loss_workspace
+        fn.argtypes = [ctypes.c_int] * 3 + [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64] + [ctypes.c_int] * 5
+        fn.restype = ctypes.c_int64
+        _workspace_bytes = fn
+    n = _workspace_bytes(grads, want_dx, x.dtype == torch.float32, ptr(head), head.dtype == torch.float32, head.stride(0), x.shape[0], x.shape[1],
+                         head.shape[0], K, kl)
+    return torch.empty(n, dtype=torch.uint8, device=x.device)
+
+
+def _forward(x, head, labels, teacher, softcap):
+    x, head = _rows_of(x), _rows_of(head)
+    rows = x.shape[0]
+    ids, logp, tail = (t.contiguous() for t in teacher) if teacher else (None, None, None)
+    labels = labels.contiguous() if labels is not None else None
+    with _on(x.device):
+        from ..ops.kernels import status_word
+        loss = torch.empty(rows, dtype=torch.float32, device=x.device)
+        stats = torch.empty(2, rows, dtype=torch.float32, device=x.device)
+        if not rows:
+            return loss, stats
+        K = ids.shape[1] if teacher else 1
+        ws = _workspace(0, 0, x, head, K, teacher is not None)
+        call("head_loss", "pilpilpipppiiiifppplp", ptr(x), int(x.dtype == torch.float32), x.stride(0), ptr(head), int(head.dtype == torch.float32),
+             head.stride(0), ptr(labels), labels.element_size() if labels is not None else 0, ptr(ids), ptr(logp), ptr(tail), K, rows, x.shape[1],
+             head.shape[0], float(softcap), ptr(loss), ptr(stats), ptr(ws), ws.numel(), ptr(status_word(x.device)))
+    return loss, stats
+
+
+def _backward(x, head, labels, teacher, stats, dloss, softcap, want_dx, want_dhead):
+    x, head = _rows_of(x), _rows_of(head)
+    rows = x.shape[0]
+    ids, logp, tail = (t.contiguous() for t in teacher) if teacher else (None, None, None)
+    labels = labels.contiguous() if labels is not None else None
+    stats, dloss = stats.contiguous(), dloss.contiguous()
+    with _on(x.device):
+        from ..ops.kernels import status_word
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
+        dhead = (torch.empty if rows else torch.zeros)(head.shape, dtype=head.dtype, device=x.device) if want_dhead else None
+        if rows:
+            K = ids.shape[1] if teacher else 1
+            ws = _workspace(1, int(want_dx), x, head, K, teacher is not None)
+            call("head_loss_grad", "pilpilpipppiiiifppppplp", ptr(x), int(x.dtype == torch.float32), x.stride(0), ptr(head),
+                 int(head.dtype == torch.float32), head.stride(0), ptr(labels), labels.element_size() if labels is not None else 0, ptr(ids), ptr(logp),
+                 ptr(tail), K, rows, x.shape[1], head.shape[0], float(softcap), ptr(stats), ptr(dloss), ptr(dx), ptr(dhead), ptr(ws), ws.numel(),
+                 ptr(status_word(x.device)))
+    return dx, dhead
+
+
+# ------------------------------------------------------------------------------------------------ the statement in PyTorch (CPU)
+def _wide(t):
+    return t if t.dtype == torch.float64 else t.float()
+
+
+def _capped(x, head, softcap):
+    z = _wide(x) @ _wide(head).t()
+    if softcap > 0:
+        t = torch.tanh(z / softcap)
+        return softcap * t, 1 - t * t
+    return z, None
+
+
+def _gathered(x, live):
+    """The rows that count (what stands in the others is not used)."""
+    return x[live] if not bool(live.all()) else x
+
+
+def _spread(v, live):
+    out = torch.zeros(live.shape[0], *v.shape[1:], dtype=v.dtype)
+    out[live] = v
+    return out
+
+
+def _sums(z, targets):
+    """-> (log sum exp, the same without ``targets``), targets bool [rows, vocab]."""
+    return torch.logsumexp(z, 1), torch.logsumexp(z.masked_fill(targets, -math.inf), 1)
+
+
+def _finish_grads(dz, slope, bad, x, head, live, want_dx, want_dhead):
+    if slope is not None:
+        dz = dz * slope
+    dz = torch.where(bad[:, None], torch.full_like(dz, math.nan), dz)
+    dx = _spread((dz @ _wide(head)).to(x.dtype), live) if want_dx else None
+    dhead = (dz.t() @ _wide(_gathered(x, live))).to(head.dtype) if want_dhead else None
+    return dx, dhead
+
+
+def _cpu_labels(z, labels):
+    bad = labels >= z.shape[1]
+    y = labels.long().clamp(max=z.shape[1] - 1)[:, None]
+    return bad, y, torch.zeros_like(z, dtype=torch.bool).scatter_(1, y, True)
+
+
+def _cpu_ce(x, head, labels, softcap):
+    live = labels >= 0
+    z, _ = _capped(_gathered(x, live), head, softcap)
+    bad, y, hit = _cpu_labels(z, labels[live])
+    lse, rest = _sums(z, hit)
+    nll = torch.nn.functional.softplus(rest - z.gather(1, y)[:, 0], threshold=1e9)
+    nan = torch.full_like(nll, math.nan)
+    return _spread(torch.where(bad, nan, nll), live), torch.stack([_spread(torch.where(bad, nan, lse), live), _spread(rest, live)])
+
+
+def _cpu_ce_grad(x, head, labels, stats, dloss, softcap, want_dx, want_dhead):
+    live = labels >= 0
+    z, slope = _capped(_gathered(x, live), head, softcap)
+    bad, y, _ = _cpu_labels(z, labels[live])
+    lse, rest = stats[0][live].to(z.dtype), stats[1][live].to(z.dtype)
+    dz = torch.exp(z - lse[:, None]).scatter(1, y, -torch.exp(rest - lse)[:, None]) * dloss[live].to(z.dtype)[:, None]
+    return _finish_grads(dz, slope, bad, x, head, live, want_dx, want_dhead)
+
+
+def _cpu_teacher(z, ids, logp, tail):
+    """-> (bad rows, places, the teacher's masses with zeros at padding, log masses, rest mass, targets bool)."""
+    vocab = z.shape[1]
+    known, at = ids >= 0, ids.long().clamp(0, vocab - 1)
+    bad = ((ids >= vocab) & known).any(1)
+    hit = torch.zeros(z.shape[0], vocab + 1, dtype=torch.bool).scatter_(1, torch.where(known & (ids < vocab), ids.long(), vocab), True)[:, :vocab]
+    logp = torch.where(known, logp.to(z.dtype), torch.full((), -math.inf, dtype=z.dtype))
+    return bad, at, torch.exp(logp), logp, tail.to(z.dtype), hit
+
+
+def _cpu_kl(x, head, ids, logp, tail, softcap):
+    live = (ids >= 0).any(1)
+    z, _ = _capped(_gathered(x, live), head, softcap)
+    bad, at, a, logp, tail, hit = _cpu_teacher(z, ids[live], logp[live], tail[live])
+    lse, rest = _sums(z, hit)
+    zero = torch.zeros((), dtype=z.dtype)
+    kl = torch.where(a > 0, a * (logp - (z.gather(1, at) - lse[:, None])), zero).sum(1)
+    kl = kl + torch.where(tail > -math.inf, torch.exp(tail) * (tail - (rest - lse).clamp(min=math.log(REST_FLOOR))), zero)
+    nan = torch.full_like(kl, math.nan)
+    return _spread(torch.where(bad, nan, kl), live), torch.stack([_spread(torch.where(bad, nan, lse), live), _spread(rest, live)])
+
+
+def _cpu_kl_grad(x, head, ids, logp, tail, stats, dloss, softcap, want_dx, want_dhead):
+    live = (ids >= 0).any(1)
+    z, slope = _capped(_gathered(x, live), head, softcap)
+    bad, at, a, _, tail, hit = _cpu_teacher(z, ids[live], logp[live], tail[live])
+    lse, rest = stats[0][live].to(z.dtype), stats[1][live].to(z.dtype)
+    s, t = torch.exp(z - lse[:, None]), torch.exp(tail)
+    t = torch.where(rest - lse >= math.log(REST_FLOOR), t, torch.zeros_like(t))
+    over = torch.where(t > 0, t * torch.exp(lse - rest), t)
+    dz = s * (a.sum(1) + t)[:, None] - s.masked_fill(hit, 0.0) * over[:, None]
+    dz = dz.scatter_add(1, at, -a) * dloss[live].to(z.dtype)[:, None]
+    return _finish_grads(dz, slope, bad, x, head, live, want_dx, want_dhead)
+
+
+# ------------------------------------------------------------------------------------------------ entry points
+def head_cross_entropy(x, head, labels, *, softcap: float = 0.0):
+    """-> (nll [rows], stats [2, rows]): stats are log sum_v exp z_v and the same sum without the label, for the backward pass."""
+    _check(x, head, softcap, _label_args(x, labels))
+    return _forward(x, head, labels, None, softcap) if x.is_cuda else _cpu_ce(x, head, labels, softcap)
+
+
+def head_cross_entropy_backward(x, head, labels, stats, dloss, *, softcap: float = 0.0, want_dx: bool = True, want_dhead: bool = True):
+    """Gradients of ``(nll * dloss).sum()``: -> (dx or None, dhead or None)."""
+    _check(x, head, softcap, _label_args(x, labels), dloss, stats)
+    if not (want_dx or want_dhead):
+        return None, None
+    if x.is_cuda:
+        return _backward(x, head, labels, None, stats, dloss, softcap, want_dx, want_dhead)
+    return _cpu_ce_grad(x, head, labels, stats, dloss, softcap, want_dx, want_dhead)
+
+
+def head_kl(x, head, ids, logp, tail, *, softcap: float = 0.0):
+    """ids int32 [rows, K], logp fp32 [rows, K] and tail fp32 [rows]: the teacher's tokens, their log-probabilities and the log of the mass outside
+    them. -> (kl [rows], stats [2, rows]): stats are log sum_v exp z_v and the same sum without the teacher's tokens."""
+    _check(x, head, softcap, _teacher_args(x, ids, logp, tail))
+    return _forward(x, head, None, (ids, logp, tail), softcap) if x.is_cuda else _cpu_kl(x, head, ids, logp, tail, softcap)
+
+
+def head_kl_backward(x, head, ids, logp, tail, stats, dloss, *, softcap: float = 0.0, want_dx: bool = True, want_dhead: bool = True):
+    """Gradients of ``(kl * dloss).sum()``: -> (dx or None, dhead or None). The teacher is a constant."""
+    _check(x, head, softcap, _teacher_args(x, ids, logp, tail), dloss, stats)
+    if not (want_dx or want_dhead):
+        return None, None
+    if x.is_cuda:
+        return _backward(x, head, None, (ids, logp, tail), stats, dloss, softcap, want_dx, want_dhead)
+    return _cpu_kl_grad(x, head, ids, logp, tail, stats, dloss, softcap, want_dx, want_dhead)
+
+
+def _refuse_capture(x):
+    if x.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("differentiable head losses are not captured into CUDA graphs (autograd may meet leaves of an eager graph on another "
+                           "stream): capture the explicit forward and backward functions")
+
+
+class _HeadLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, head, softcap, *targets):
+        _refuse_capture(x)
+        loss, stats = (head_cross_entropy if len(targets) == 1 else head_kl)(x, head, *targets, softcap=softcap)
+        ctx.save_for_backward(x, head, stats, *targets)
+        ctx.softcap = softcap
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        x, head, stats, *targets = ctx.saved_tensors
+        _refuse_capture(x)
+        fn = head_cross_entropy_backward if len(targets) == 1 else head_kl_backward
+        dx, dhead = fn(x, head, *targets, stats, dloss.to(stats.dtype), softcap=ctx.softcap, want_dx=ctx.needs_input_grad[0],
+                       want_dhead=ctx.needs_input_grad[1])
+        return (dx, dhead, None) + (None,) * len(targets)
+
+
+def head_cross_entropy_loss(x, head, labels, softcap: float = 0.0):
+    """nll [rows], differentiable in ``x`` and ``head``."""
+    return _HeadLoss.apply(x, head, float(softcap), labels)
+
+
+def head_kl_loss(x, head, ids, logp, tail, softcap: float = 0.0):
+    """kl [rows], differentiable in ``x`` and ``head``."""
+    return _HeadLoss.apply(x, head, float(softcap), ids, logp, tail)

@@ -19,13 +19,13 @@ workspace from the caching allocator and may be captured into a CUDA graph. CPU 
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 
 import torch
 
 from .._lib import call, kernels, ptr
+from .launch import on, refuse_capture, rows_of
 
 MAX_TOPK = 1024
 REST_FLOOR = 1e-12                 # least probability of "any other token" in a divergence
@@ -73,15 +73,6 @@ def _teacher_args(x, ids, logp, tail):
     return [("ids", ids, (torch.int32,), (rows, k)), ("logp", logp, f, (rows, k)), ("tail", tail, f, (rows,))]
 
 
-def _on(device):
-    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else contextlib.nullcontext()
-
-
-def _rows_of(t):
-    """Rows in place where their elements lie side by side."""
-    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] or t.shape[0] == 0 else t.contiguous()
-
-
 _workspace_bytes = None
 
 
@@ -98,11 +89,11 @@ def _workspace(grads, want_dx, x, head, K, kl):
 
 
 def _forward(x, head, labels, teacher, softcap):
-    x, head = _rows_of(x), _rows_of(head)
+    x, head = rows_of(x), rows_of(head)
     rows = x.shape[0]
     ids, logp, tail = (t.contiguous() for t in teacher) if teacher else (None, None, None)
     labels = labels.contiguous() if labels is not None else None
-    with _on(x.device):
+    with on(x.device):
         from ..ops.kernels import status_word
         loss = torch.empty(rows, dtype=torch.float32, device=x.device)
         stats = torch.empty(2, rows, dtype=torch.float32, device=x.device)
@@ -117,12 +108,12 @@ def _forward(x, head, labels, teacher, softcap):
 
 
 def _backward(x, head, labels, teacher, stats, dloss, softcap, want_dx, want_dhead):
-    x, head = _rows_of(x), _rows_of(head)
+    x, head = rows_of(x), rows_of(head)
     rows = x.shape[0]
     ids, logp, tail = (t.contiguous() for t in teacher) if teacher else (None, None, None)
     labels = labels.contiguous() if labels is not None else None
     stats, dloss = stats.contiguous(), dloss.contiguous()
-    with _on(x.device):
+    with on(x.device):
         from ..ops.kernels import status_word
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
         dhead = (torch.empty if rows else torch.zeros)(head.shape, dtype=head.dtype, device=x.device) if want_dhead else None
@@ -268,16 +259,10 @@ def head_kl_backward(x, head, ids, logp, tail, stats, dloss, *, softcap: float =
     return _cpu_kl_grad(x, head, ids, logp, tail, stats, dloss, softcap, want_dx, want_dhead)
 
 
-def _refuse_capture(x):
-    if x.is_cuda and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("differentiable head losses are not captured into CUDA graphs (autograd may meet leaves of an eager graph on another "
-                           "stream): capture the explicit forward and backward functions")
-
-
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, head, softcap, *targets):
-        _refuse_capture(x)
+        refuse_capture(x)
         loss, stats = (head_cross_entropy if len(targets) == 1 else head_kl)(x, head, *targets, softcap=softcap)
         ctx.save_for_backward(x, head, stats, *targets)
         ctx.softcap = softcap
@@ -287,7 +272,7 @@ class _HeadLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
         x, head, stats, *targets = ctx.saved_tensors
-        _refuse_capture(x)
+        refuse_capture(x)
         fn = head_cross_entropy_backward if len(targets) == 1 else head_kl_backward
         dx, dhead = fn(x, head, *targets, stats, dloss.to(stats.dtype), softcap=ctx.softcap, want_dx=ctx.needs_input_grad[0],
                        want_dhead=ctx.needs_input_grad[1])

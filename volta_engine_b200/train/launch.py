@@ -1,0 +1,23 @@
+"""What the training operators share when they launch: the tensors' device, rows in place, and the differentiable calls' stand on graph capture."""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+
+def on(device):
+    """Launches of this block go to ``device``, on its current stream."""
+    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def rows_of(t):
+    """A matrix whose rows' elements lie side by side: ``t`` itself where they do."""
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] or t.shape[0] == 0 else t.contiguous()
+
+
+def refuse_capture(t):
+    """Differentiable calls are not captured: a captured backward pass that meets leaves of an eager graph joins streams outside the capture, and the
+    process ends. The explicit forward and backward functions may be captured."""
+    if t.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("differentiable training operators are not captured into CUDA graphs: capture the explicit forward and backward functions")

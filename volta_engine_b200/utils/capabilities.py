@@ -65,6 +65,7 @@ TABLE = {
     "train_exp_scale": ("Training primitives", P), "train_gather_rows": ("Training primitives", P),
     "train_scatter_add_rows": ("Training primitives", P), "train_scale_rows": ("Training primitives", P),
     "train_mul": ("Training primitives", P),
+    "dropout": ("Dropout", P),
     "head_loss": ("Head losses", P), "head_loss_grad": ("Head losses", P), "head_loss_workspace": ("Head losses", D),
     "decode_step": ("Persistent decode step", D), "decode_step_sizes": ("Persistent decode step", D),
     "make_tmap_2d": ("Persistent decode step", D),

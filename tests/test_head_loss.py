@@ -179,3 +179,200 @@ def test_soft_cap(topk, types):
     got, w = run(*a, 20.0), P.wanted(*a, 20.0)
     for k, limit in (("dx", 2.0 ** -8), ("dhead", 2.0 ** -8)) if xt == "bf16" else (("dx", 2.0 ** -16), ("dhead", 2.0 ** -16)):
         assert float((got[k].double() - w[k]).norm() / w[k].norm()) < limit, k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("topk", [0, 6])
+def test_left_out_rows_and_what_stands_in_them(topk):
+    a = make(290, 136, 700, topk, seed=9, left_out=0.6, device="cuda")
+    live = (a[2][0] >= 0) if not topk else (a[2][0] >= 0).any(1)
+    want = run(*a)
+    x = a[0].clone()
+    x[~live] = math.nan
+    targets = a[2]
+    if topk:
+        targets = (targets[0], targets[1].clone(), targets[2].clone())
+        targets[1][~live], targets[2][~live] = math.nan, math.inf
+    dloss = a[3].clone()
+    dloss[~live] = math.inf
+    got = run(x, a[1], targets, dloss)
+    for k in want:
+        assert torch.equal(got[k], want[k]), k
+    assert float(got["dx"][~live].abs().max()) == 0 and float(got["loss"][~live].abs().max()) == 0 and float(got["stats"][:, ~live].abs().max()) == 0
+    # every row left out, and no rows
+    none = tuple(torch.full_like(t, -1) if i == 0 else t for i, t in enumerate(targets))
+    got = run(x, a[1], none, dloss)
+    assert all(float(got[k].abs().max()) == 0 for k in got)
+    got = run(x[:0], a[1], tuple(t[:0] for t in targets), dloss[:0])
+    assert got["loss"].shape == (0,) and got["dx"].shape == (0, 136) and float(got["dhead"].abs().max()) == 0
+
+
+@pytest.mark.gpu
+def test_labels_behind_the_vocabulary_make_nan():
+    for types in ("bf16", "fp32"):
+        x, head, (lab,), dl = make(20, 72, 300, 0, types, types, seed=2, device="cuda")
+        for v in (300, 383, 384, 1 << 20, (1 << 40) + 1):
+            lab2 = lab.clone()
+            lab2[3] = v
+            got = run(x, head, (lab2,), dl)
+            assert torch.isnan(got["loss"][3]) and torch.isnan(got["dx"][3]).all() and torch.isnan(got["dhead"]).all()
+            assert int(torch.isnan(got["loss"]).sum()) == 1 and int(torch.isnan(got["dx"]).any(1).sum()) == 1
+    x, head, t, dl = make(20, 72, 300, 4, seed=2, device="cuda")
+    t[0][5, 2] = 300
+    got = run(x, head, t, dl)
+    assert torch.isnan(got["loss"][5]) and int(torch.isnan(got["loss"]).sum()) == 1 and torch.isnan(got["dx"][5]).all()
+
+
+@pytest.mark.gpu
+def test_teachers_of_odd_forms():
+    x, head, (ids, logp, tail), dl = make(40, 136, 500, 8, seed=12, device="cuda")
+    # a token listed twice is one whose mass is the sum; the order of the tokens does not matter
+    perm = torch.randperm(8, generator=torch.Generator().manual_seed(0)).cuda()
+    p, q = run(x, head, (ids[:, perm].contiguous(), logp[:, perm].contiguous(), tail), dl), run(x, head, (ids, logp, tail), dl)
+    for k in p:
+        assert torch.allclose(p[k], q[k], rtol=2.0 ** -7, atol=1e-6), k
+    half = (torch.cat([ids, ids[:, :1]], 1), torch.cat([logp, logp[:, :1] - math.log(2)], 1), tail)
+    half[1][:, 0] -= math.log(2)
+    two = run(x, head, half, dl)
+    assert torch.equal(two["stats"], q["stats"]) and torch.allclose(two["dx"].float(), q["dx"].float(), rtol=2.0 ** -7, atol=1e-5)
+    # no mass outside, tokens without mass
+    t = (ids, logp.clone(), torch.full_like(tail, -math.inf))
+    t[1][:, 3] = -math.inf
+    got = run(x, head, t, dl)
+    w = P.wanted(x, head, t, dl, 0.0)
+    assert torch.allclose(got["loss"].double(), w["loss"], rtol=1e-4, atol=1e-5) and not torch.isnan(got["dx"]).any()
+    assert float((got["dx"].double() - w["dx"]).norm() / w["dx"].norm()) < 2.0 ** -8
+    # the model gives the rest less than the floor: it is held at the floor and pulls on nothing
+    big = (x * 0 + 60 * head[ids[:, 0].long()]).to(torch.bfloat16)
+    got = run(big, head, (ids, logp, tail), dl)
+    hold(got, big, head, (ids, logp, tail), dl, 0.0, only=("loss", "stats"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", ["bf16 bf16", "fp32 fp32"])
+def test_strides_and_starts(types):
+    xt, ht = types.split()
+    x, head, t, dl = make(70, 128, 333, 0, xt, ht, seed=6, device="cuda")
+    want = run(x, head, t, dl)
+
+    def placed(m, left, right, step=1):
+        big = torch.full((m.shape[0] * step, left + m.shape[1] + right), math.nan, dtype=m.dtype, device="cuda")
+        v = big[::step, left:left + m.shape[1]]
+        v.copy_(m)
+        return v
+    for xs, hs in ((placed(x, 8, 8), placed(head, 8, 16)), (placed(x, 3, 2), placed(head, 1, 0)), (placed(x, 0, 0, 2), placed(head, 0, 8, 3)),
+                   (x.t().contiguous().t(), head.t().contiguous().t())):
+        got = run(xs, hs, t, dl)
+        for k in got:
+            assert torch.equal(got[k], want[k]), k
+    # labels of 32 bits, strided
+    lab = torch.stack([t[0].int(), t[0].int() * 0], 1)[:, 0]
+    got = run(x, head, (lab,), dl)
+    assert all(torch.equal(got[k], want[k]) for k in got)
+
+
+@pytest.mark.gpu
+def test_one_gradient_alone_and_the_same_bits_again():
+    for topk in (0, 5):
+        x, head, t, dl = make(300, 264, 3000, topk, seed=8, left_out=0.1, device="cuda")
+        a, b = run(x, head, t, dl), run(x, head, t, dl)
+        assert all(torch.equal(a[k], b[k]) for k in a)
+        c, d = run(x, head, t, dl, want_dhead=False), run(x, head, t, dl, want_dx=False)
+        assert c["dhead"] is None and d["dx"] is None and torch.equal(c["dx"], a["dx"]) and torch.equal(d["dhead"], a["dhead"])
+        # a row does not depend on the rows beside it
+        e = run(x[40:120], head, tuple(v[40:120] for v in t), dl[40:120])
+        assert torch.equal(e["loss"], a["loss"][40:120]) and torch.equal(e["stats"], a["stats"][:, 40:120])
+
+
+@pytest.mark.gpu
+def test_streams_and_graphs():
+    x, head, t, dl = make(64, 256, 2000, 7, seed=1, device="cuda")
+    want = run(x, head, t, dl)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run(x, head, t, dl)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(got[k], want[k]) for k in got)
+    # two captured calls replayed in turn, and on two streams at once: each has its own workspace
+    x2 = x.roll(1, 0).contiguous()
+    want2 = run(x2, head, t, dl)
+    graphs = []
+    for v in (x, x2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = run(v, head, t, dl)
+        graphs.append((g, out))
+    for _ in range(3):
+        for (g, out), w in zip(graphs, (want, want2)):
+            g.replay()
+            assert all(torch.equal(out[k], w[k]) for k in out)
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            graphs[0][0].replay()
+        with torch.cuda.stream(other):
+            graphs[1][0].replay()
+    torch.cuda.synchronize()
+    for (_, out), w in zip(graphs, (want, want2)):
+        assert all(torch.equal(out[k], w[k]) for k in out)
+    # the differentiable call gives the pair's gradients, and is not captured
+    xs, hs = x.clone().requires_grad_(), head.clone().requires_grad_()
+    L.head_kl_loss(xs, hs, *t).backward(dl)
+    assert torch.equal(xs.grad, want["dx"]) and torch.equal(hs.grad, want["dhead"])
+    with pytest.raises(RuntimeError, match="not captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            L.head_kl_loss(xs, hs, *t)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_gradients_by_differences():
+    """Directional differences of the kernel's own losses in fp32: a step of 2^-6 in a direction of norm one changes the loss by its gradient, up to the
+    cube of the step (third derivatives of these losses are below 30 here) and the losses' rounding (2^-20) over the step."""
+    for topk in (0, 5):
+        x, head, t, dl = make(24, 40, 120, topk, "fp32", "fp32", seed=3, device="cuda", spread=1.0)
+        got = run(x, head, t, dl, 10.0)
+        f = L.head_cross_entropy if not topk else L.head_kl
+        g = torch.Generator(device="cuda").manual_seed(4)
+        for which in (0, 1):
+            d = torch.randn((x, head)[which].shape, generator=g, device="cuda")
+            d /= d.norm()
+            h = 2.0 ** -6
+            up, dn = (f(*((x + s * d, head) if which == 0 else (x, head + s * d)), *t, softcap=10.0)[0] for s in (h, -h))
+            num = float(((up - dn).double() * dl.double()).sum()) / (2 * h)
+            ana = float(((got["dx"], got["dhead"])[which].double() * d.double()).sum())
+            assert abs(num - ana) < 30 * h * h * float(dl.sum()) / 6 + float(dl.sum()) * 2.0 ** -20 * 8 / h, (topk, which, num, ana)
+
+
+@pytest.mark.gpu
+def test_pieces_of_the_vocabulary():
+    """dz of more than one piece (256 MB: 100 000 columns of 1300 rows), and packed fp32 rows of a head of more than one piece (512 MB)."""
+    x, head, t, dl = make(1300, 64, 100500, 0, seed=5, left_out=0.01, device="cuda")
+    w = hold(run(x, head, t, dl), x, head, t, dl, 0.0)
+    del w
+    x, head, t, dl = make(40, 1000, 90000, 5, "fp32", "fp32", seed=5, device="cuda")
+    hold(run(x, head, t, dl), x, head, t, dl, 0.0)
+
+
+@pytest.mark.gpu
+def test_offsets_that_pass_32_bits():
+    """A head of 2.2 G values; the last rows' labels stand at its end."""
+    vocab, hidden = 540000, 4096
+    head = torch.empty(vocab, hidden, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(0)
+    for lo in range(0, vocab, 60000):
+        head[lo:lo + 60000] = (torch.randn(60000, hidden, generator=g, device="cuda") * (2.0 / 64)).to(torch.bfloat16)
+    x = torch.randn(3, hidden, generator=g, device="cuda").to(torch.bfloat16)
+    labels = torch.tensor([vocab - 1, 5, vocab - 70000], device="cuda")
+    dl = torch.ones(3, device="cuda")
+    got = run(x, head, (labels,), dl)
+    z = torch.cat([x.double() @ head[lo:lo + 60000].double().t() for lo in range(0, vocab, 60000)], 1)
+    lse = torch.logsumexp(z, 1)
+    assert torch.allclose(got["loss"].double(), lse - z.gather(1, labels[:, None])[:, 0], atol=1e-3)
+    s = torch.exp(z - lse[:, None]).scatter_add_(1, labels[:, None], torch.full((3, 1), -1.0, dtype=torch.float64, device="cuda"))
+    dx = sum(s[:, lo:lo + 60000] @ head[lo:lo + 60000].double() for lo in range(0, vocab, 60000))
+    assert float((got["dx"].double() - dx).norm() / dx.norm()) < 2.0 ** -8
+    tail = s[:, -100:].t() @ x.double()
+    assert float((got["dhead"][-100:].double() - tail).norm() / tail.norm()) < 2.0 ** -8

@@ -345,6 +345,15 @@ class DenseModel:
                            self.comm.rank * self.vocab_local)
         return logits
 
+    def scoring_head(self):
+        """(head rows [vocab, hidden], soft cap) for losses computed from ``last_hidden`` without logits (train/head_loss.py); None where the head is
+        not one plain bf16 or fp32 matrix on this rank."""
+        w = getattr(self.lm_head, "weight", None)
+        if w is None or w.dtype not in (torch.bfloat16, torch.float32) or getattr(self.lm_head, "bias", None) is not None or self.comm.size != 1:
+            return None
+        capped = self.cfg.residual not in ("gated", "hc")  # (the multi-stream forms take no cap)
+        return w[: self.cfg.vocab, : self.cfg.hidden], float(self.cfg.logit_softcap) if capped else 0.0
+
     # ------------------------------------------------------------------------------------- multi-stream residuals
     def init_stream_weights(self, seed: int = 9, std: float = 0.02):
         """Weights of the multi-stream residual forms (``cfg.residual``): per sublayer a gated-residual mixer

@@ -3,10 +3,14 @@
 Every quantised linear is a frozen core between a per-input-channel and a per-output-channel scale
 (``W = diag(su) T diag(sv)``; for EXL3 the core is the Hadamard-rotated trellis decode). The tool trains log deltas on all
 those scales and additive deltas on the norm weights with Adam on KL(teacher || model) over token sequences; codes and
-every other weight stay frozen. The model runs in an fp32 training form written in PyTorch (autograd), each layer
+every other weight stay frozen. ``--teacher labels``: cross entropy of the sequences' own next tokens instead. The model runs in an fp32 training form written in PyTorch (autograd), each layer
 recomputed from its saved input in the backward (activation checkpointing). Learning rate: linear warm-up, then a cosine
 down to ``lr_min * lr``. ``devices``: the layers are split evenly over the devices as sequential stages with hand-offs
 between them (``--tp 0`` form of the reference tool).
+``--no-logits``: the divergence from a top-K teacher comes straight from the final states and the head, whose logits are never held
+(train/head_loss.py; cross entropy always does). ``--dropout p``: a sub-layer's result loses a share p of its elements on the way into the
+residual stream while training, by masks that are computed from (seed, step, sequence, sub-layer, row, column) (train/dropout.py): a checkpointed layer
+that runs again in the backward pass, and ranks that hold some of the rows, drop the same ones.
 Reference: docs/QUANTIZATION.md:99 (``volta_e2e``), src/tools/volta_e2e.cpp:473-512 (stage split), inc/engine/train/qwen4_exp.h.
 """
 from __future__ import annotations
@@ -19,6 +23,9 @@ from dataclasses import dataclass, field
 import torch
 import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
+
+from ..train.dropout import dropout_residual
+from ..train.head_loss import head_cross_entropy_loss, head_kl_loss
 
 
 class TunedLinear(torch.nn.Module):
@@ -72,7 +79,19 @@ def _rope(x, pos, theta, rot):
     return torch.cat([a * cs - b * sn, b * cs + a * sn, x[..., rot:]], dim=-1)
 
 
-class TunedLayer(torch.nn.Module):
+class _SubLayers(torch.nn.Module):
+    """Residual additions of a layer's two sub-layers; ``drop`` = (p, seed, first row, site) while training with dropout."""
+
+    drop = None
+
+    def add(self, h, y, sub: int):
+        if self.drop is None or not self.training:
+            return h + y
+        p, seed, row0, site = self.drop
+        return dropout_residual(y, p, seed, h, row0, site + sub)
+
+
+class TunedLayer(_SubLayers):
     def __init__(self, cfg, lin: dict, norms: dict):
         super().__init__()
         self.cfg = cfg
@@ -93,11 +112,11 @@ class TunedLayer(torch.nn.Module):
         att = F.scaled_dot_product_attention(q.transpose(0, 1)[None], k.repeat_interleave(g, 1).transpose(0, 1)[None],
                                              v.repeat_interleave(g, 1).transpose(0, 1)[None], is_causal=True,
                                              scale=c.attn_scale or 1.0 / math.sqrt(hd))[0].transpose(0, 1).reshape(T, nq * hd)
-        h = h + self.o(att)
+        h = self.add(h, self.o(att), 0)
         gu = self.gu(self.n2(h))
         inter = gu.shape[-1] // 2
         act = F.silu(gu[:, :inter]) if c.act == "silu" else F.gelu(gu[:, :inter], approximate="tanh")
-        return h + self.dn(act * gu[:, inter:])
+        return self.add(h, self.dn(act * gu[:, inter:]), 1)
 
 
 @dataclass
@@ -110,6 +129,9 @@ class E2EOptions:
     eval_every: int = 16
     norms: bool = True
     devices: list = field(default_factory=lambda: ["cpu"])
+    no_logits: bool = False       # divergence from a top-K teacher without the logits (``head_kl_loss``)
+    dropout: float = 0.0          # share of a sub-layer result's elements dropped while training
+    seed: int = 0                 # of the dropout masks
 
 
 # ---------------------------------------------------------------------------------------------- tensor parallel form
@@ -144,7 +166,7 @@ class ShardedTunedLinear(torch.nn.Module):
         return [self.a_u] if self.split == "col" else [self.a_v]
 
 
-class TunedLayerSP(torch.nn.Module):
+class TunedLayerSP(_SubLayers):
     """``TunedLayer`` in the sequence-parallel form: every rank owns ``T / ranks`` rows of the fp32 stream and the heads /
     hidden units ``rank :: ranks`` of the sub-layers. A sub-layer normalises its rows, all-gathers them, runs its
     column-parallel and row-parallel linears on its slice and reduce-scatters the partial sums back to rows
@@ -191,11 +213,11 @@ class TunedLayerSP(torch.nn.Module):
         att = F.scaled_dot_product_attention(q.transpose(0, 1)[None], k.repeat_interleave(g, 1).transpose(0, 1)[None],
                                              v.repeat_interleave(g, 1).transpose(0, 1)[None], is_causal=True,
                                              scale=c.attn_scale or 1.0 / math.sqrt(hd))[0].transpose(0, 1).reshape(T, nq * hd)
-        h = h + self.o.finish(reduce_scatter_rows(self.o(att), self.group))
+        h = self.add(h, self.o.finish(reduce_scatter_rows(self.o(att), self.group)), 0)
         gu = self.gu(gather_rows(self.n2(h), self.group))
         inter = gu.shape[-1] // 2
         act = F.silu(gu[:, :inter]) if c.act == "silu" else F.gelu(gu[:, :inter], approximate="tanh")
-        return h + self.dn.finish(reduce_scatter_rows(self.dn(act * gu[:, inter:]), self.group))
+        return self.add(h, self.dn.finish(reduce_scatter_rows(self.dn(act * gu[:, inter:]), self.group)), 1)
 
 
 class TunedModelSP(torch.nn.Module):
@@ -218,13 +240,17 @@ class TunedModelSP(torch.nn.Module):
         assert per * self.world == T, "sequence length must be a multiple of the rank count"
         return slice(self.rank * per, (self.rank + 1) * per)
 
-    def forward(self, ids: torch.Tensor) -> torch.Tensor:
-        """-> logits of this rank's rows [T / ranks, vocab]."""
+    def states(self, ids: torch.Tensor) -> torch.Tensor:
+        """-> final states of this rank's rows [T / ranks, hidden]."""
         mine = ids[self.rows(ids.shape[0])]
         h = self.embed[mine.to(self.embed.device).long()] * self.cfg.embed_scale
         for L in self.layers:
             h = checkpoint(L, h, use_reentrant=False) if self.training else L(h)
-        return self.final_norm(h) @ self.head.t()
+        return self.final_norm(h)
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        """-> logits of this rank's rows [T / ranks, vocab]."""
+        return self.states(ids) @ self.head.t()
 
     def sync_grads(self) -> None:
         from ..parallel.sequence_parallel import sum_replicated_grads
@@ -250,12 +276,15 @@ class TunedModel(torch.nn.Module):
         self.final_norm.to(devices[-1])
         self.register_buffer("head", head.float().to(devices[-1]))
 
-    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+    def states(self, ids: torch.Tensor) -> torch.Tensor:
         h = self.embed[ids.to(self.devices[0]).long()] * self.cfg.embed_scale
         for i, L in enumerate(self.layers):
             h = h.to(self.devices[self.stage[i]])                      # stage hand-off
             h = checkpoint(L, h, use_reentrant=False) if self.training else L(h)
-        return self.final_norm(h.to(self.devices[-1])) @ self.head.t()
+        return self.final_norm(h.to(self.devices[-1]))
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        return self.states(ids) @ self.head.t()
 
 
 def build_from_engine_model(model, devices=("cpu",)) -> TunedModel:
@@ -294,7 +323,36 @@ def kl_teacher(student_logits: torch.Tensor, teacher_logits) -> torch.Tensor:
 
 
 def _to(teacher, device):
+    if teacher is None:
+        return None
     return tuple(t.to(device) for t in teacher) if isinstance(teacher, (tuple, list)) else teacher.to(device)
+
+
+def scoring_head(model) -> torch.Tensor:
+    """The head's rows for losses without logits: bf16 where that holds every value (half the memory, and half the products of fp32 rows)."""
+    short = model.head.to(torch.bfloat16)
+    return short if torch.equal(short.float(), model.head) else model.head
+
+
+def objective(model, ids, teacher, head=None) -> torch.Tensor:
+    """What a sequence is tuned on: its mean divergence from ``teacher``, or with ``teacher`` None the mean cross entropy of its next tokens. ``head``
+    (``scoring_head``): without logits, otherwise (a teacher only) through them. A sequence-parallel model's ranks give parts whose mean that is."""
+    if teacher is not None and head is None:
+        return kl_teacher(model(ids), teacher)
+    x = model.states(ids)
+    if teacher is None:
+        labels = torch.cat([ids[1:].long(), torch.full((1,), -100, dtype=torch.int64, device=ids.device)])
+        mine, ranks = (labels[model.rows(ids.shape[0])], model.world) if isinstance(model, TunedModelSP) else (labels, 1)
+        return head_cross_entropy_loss(x, head, mine.to(x.device)).sum() * (ranks / max(1, ids.shape[0] - 1))
+    t_ids, logp, tail = teacher
+    return head_kl_loss(x[: t_ids.shape[0]], head, t_ids.to(torch.int32), logp.float(), tail.float()).mean()
+
+
+def set_dropout(model, p: float, seed: int, rows: int) -> None:
+    """Masks of the next forward (and its backward) over a sequence of ``rows``; p = 0: none."""
+    row0 = model.rows(rows).start if isinstance(model, TunedModelSP) else 0
+    for i, L in enumerate(model.layers):
+        L.drop = (p, seed, row0, 2 * i) if p > 0 else None
 
 
 def lr_at(step: int, o: E2EOptions) -> float:
@@ -305,8 +363,13 @@ def lr_at(step: int, o: E2EOptions) -> float:
 
 
 def tune(model: TunedModel, sequences: list, teachers: list, o: E2EOptions, held_out: int = 1, log=print) -> dict:
-    """sequences: list of id tensors; teachers: matching teacher logits [T, vocab]. The last ``held_out`` sequences only
-    evaluate. Returns {"eval": [(step, kl)], "train": [kl per step]}."""
+    """sequences: list of id tensors; teachers: matching teacher logits [T, vocab], top-K teachers, or Nones (cross entropy). The last
+    ``held_out`` sequences only evaluate. Returns {"eval": [(step, kl)], "train": [kl per step]}."""
+    direct = o.no_logits or any(t is None for t in teachers)
+    if direct and not all(t is None or isinstance(t, (tuple, list)) for t in teachers):
+        raise ValueError("tuning without logits takes top-K teachers: these are logits")
+    head = scoring_head(model) if direct else None
+    what = "cross entropy" if any(t is None for t in teachers) else "KL"
     params = [p for n, p in model.named_parameters() if o.norms or not n.endswith("delta")]
     opt = torch.optim.Adam(params, lr=o.lr)
     train = list(range(len(sequences) - held_out))
@@ -316,7 +379,7 @@ def tune(model: TunedModel, sequences: list, teachers: list, o: E2EOptions, held
 
     def teacher_of(i, T):
         t = _to(teachers[i], model.devices[-1])
-        if not sp:
+        if not sp or t is None:
             return t
         r = model.rows(T)                                   # this rank scores its own rows
         return tuple(x[r] for x in t) if isinstance(t, (tuple, list)) else t[r]
@@ -332,11 +395,11 @@ def tune(model: TunedModel, sequences: list, teachers: list, o: E2EOptions, held
     def evaluate(step):
         model.eval()
         with torch.no_grad():
-            kl = sum(float(kl_teacher(model(sequences[i]), teacher_of(i, sequences[i].shape[0])))
+            kl = sum(float(objective(model, sequences[i], teacher_of(i, sequences[i].shape[0]), head))
                      for i in range(len(sequences) - held_out, len(sequences))) / max(1, held_out)
         kl = over_ranks(kl)
         hist["eval"].append((step, kl))
-        log(f"step {step}: held-out KL {kl:.6f}")
+        log(f"step {step}: held-out {what} {kl:.6f}")
         return kl
     evaluate(0)
     scale = o.batch * (model.world if sp else 1)
@@ -348,7 +411,8 @@ def tune(model: TunedModel, sequences: list, teachers: list, o: E2EOptions, held
         total = 0.0
         for b in range(o.batch):
             i = train[(step * o.batch + b) % len(train)]
-            loss = kl_teacher(model(sequences[i]), teacher_of(i, sequences[i].shape[0])) / scale
+            set_dropout(model, o.dropout, (o.seed << 32) + step * o.batch + b, sequences[i].shape[0])
+            loss = objective(model, sequences[i], teacher_of(i, sequences[i].shape[0]), head) / scale
             loss.backward()
             total += float(loss.detach())
         if sp:
@@ -413,7 +477,8 @@ def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="volta_e2e", description=__doc__.split("\n\n")[0])
     ap.add_argument("--model", required=True, help="quantised model directory (EXL3 linears are tuned)")
     ap.add_argument("--inputs", required=True, help="torch file: list of int token tensors")
-    ap.add_argument("--teacher", required=True, help="torch file: list of teacher logits, or a model directory to run")
+    ap.add_argument("--teacher", required=True, help="torch file: list of teacher logits or a top-K teacher, a model directory to run, or "
+                    "'labels': no teacher, cross entropy of the next tokens")
     ap.add_argument("--out", required=True)
     ap.add_argument("--devices", default="cpu")
     ap.add_argument("--steps", type=int, default=64)
@@ -423,6 +488,9 @@ def main(argv=None) -> int:
     ap.add_argument("--lr-min", type=float, default=0.1)
     ap.add_argument("--eval-every", type=int, default=16)
     ap.add_argument("--norms", type=int, default=1)
+    ap.add_argument("--no-logits", action="store_true", help="divergence from a top-K teacher without holding the logits")
+    ap.add_argument("--dropout", type=float, default=0.0, help="share of a sub-layer result's elements dropped while training")
+    ap.add_argument("--seed", type=int, default=0, help="of the dropout masks, 0 to 2^32 - 1")
     ap.add_argument("--tp", type=int, default=0,
                     help="N > 0: sequence-parallel tensor parallelism over the N ranks this process was started with "
                          "(python -m torch.distributed.run --nproc-per-node N -m volta_engine_b200.tools.e2e ...); "
@@ -435,7 +503,11 @@ def main(argv=None) -> int:
     model, _ = load_model(a.model, "cpu", None)
     tm = build_from_engine_model(model, devices)
     seqs = torch.load(a.inputs, weights_only=True)
-    if Path(a.teacher).is_dir():
+    if not (0 <= a.dropout <= 1 and 0 <= a.seed < 1 << 32):
+        ap.error("--dropout takes 0 to 1, --seed 0 to 2^32 - 1")
+    if a.teacher == "labels":
+        teachers = [None] * len(seqs)
+    elif Path(a.teacher).is_dir():
         tmodel, _ = load_model(a.teacher, "cpu", None)
         teacher = build_from_engine_model(tmodel, devices).eval()
         with torch.no_grad():
@@ -444,7 +516,9 @@ def main(argv=None) -> int:
         teachers = torch.load(a.teacher, weights_only=True)
         if isinstance(teachers, dict):                   # the top-K teacher of volta_ppl
             teachers = list(zip(teachers["ids"], teachers["logp"], teachers["tail"]))
-    o = E2EOptions(a.steps, a.batch, a.lr, a.warmup, a.lr_min, a.eval_every, bool(a.norms), devices)
+    if a.no_logits and not all(t is None or isinstance(t, (tuple, list)) for t in teachers):
+        ap.error("--no-logits takes a top-K teacher (volta_ppl --topk-out)")
+    o = E2EOptions(a.steps, a.batch, a.lr, a.warmup, a.lr_min, a.eval_every, bool(a.norms), devices, a.no_logits, a.dropout, a.seed)
     rank = 0
     if a.tp > 0:
         import os
@@ -458,7 +532,7 @@ def main(argv=None) -> int:
         tm = TunedModelSP(tm, rank, world, dev)
         # sequences are cut to a multiple of the rank count (rows are sharded evenly)
         seqs = [sq[: sq.shape[0] // world * world] for sq in seqs]
-        teachers = [tuple(x[: sq.shape[0]] for x in t) if isinstance(t, (tuple, list)) else t[: sq.shape[0]]
+        teachers = [None if t is None else tuple(x[: sq.shape[0]] for x in t) if isinstance(t, (tuple, list)) else t[: sq.shape[0]]
                     for t, sq in zip(teachers, seqs)]
     hist = tune(tm, seqs, teachers, o, log=print if rank == 0 else (lambda *_: None))
     if a.tp > 0:
@@ -475,7 +549,7 @@ def main(argv=None) -> int:
         tensors[f"layers.{li}.attn_norm.weight"] = (L.n1.w0 + L.n1.delta).detach().half().cpu()
         tensors[f"layers.{li}.ffn_norm.weight"] = (L.n2.w0 + L.n2.delta).detach().half().cpu()
     write_safetensors(out / "e2e_scales.safetensors", tensors)
-    print(f"held-out KL {hist['eval'][0][1]:.6f} -> {hist['eval'][-1][1]:.6f}")
+    print(f"held-out {'cross entropy' if a.teacher == 'labels' else 'KL'} {hist['eval'][0][1]:.6f} -> {hist['eval'][-1][1]:.6f}")
     return 0
 
 

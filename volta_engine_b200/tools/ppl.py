@@ -11,6 +11,9 @@ the same pass.
       log-mass outside them ({"k", "ids": [S, K] per sequence, "logp": [S, K], "tail": [S]})
   --kl-teacher FILE
       KL(teacher || model) of this checkpoint against such a teacher (the K tokens plus one bucket for the rest)
+  --no-logits
+      both scores straight from the final states and a bf16 or fp32 head (train/head_loss.py): the logits of a portion are never
+      held, so a portion may be as long as the rest of the model allows. Not with --topk-out, which reads the logits
 
 Single rank (the vocabulary-parallel head of a tensor-parallel model would need its shards gathered).
 Reference: tests/4_coherence/test_ppl.cpp as documented in docs/QUANTIZATION.md:99,112 (``--calibrate``, ``--prompts``,
@@ -39,6 +42,26 @@ def sequence_logits(engine, tokens: list[int], chunk: int = 512, slot: int = 0):
         ids = tokens[lo:lo + chunk]
         b = BatchRows.make(ids, list(range(lo, lo + len(ids))), [slot] * len(ids), engine.device, LOGITS_ALL, G, prefill=True)
         yield lo, model.forward(b, kv)[:, :vocab].float()
+
+
+def sequence_states(engine, tokens: list[int], chunk: int = 512, slot: int = 0):
+    """Yields (first position, final states [rows, hidden] or None, fp32 logits or None) like ``sequence_logits``: states for portions of more than
+    MAX_GRAPH_ROWS rows; a few rows run through the decode kernels, which end in logits."""
+    from ..runtime.batch import BatchRows, LOGITS_ALL, LOGITS_NONE, MAX_GRAPH_ROWS
+    model, kv = engine.model, engine.kv
+    kv.reserve(slot, len(tokens) + 1)
+    G = model.nq // model.nkv
+    for lo in range(0, len(tokens), chunk):
+        ids = tokens[lo:lo + chunk]
+        few = len(ids) <= MAX_GRAPH_ROWS
+        b = BatchRows.make(ids, list(range(lo, lo + len(ids))), [slot] * len(ids), engine.device, LOGITS_ALL if few else LOGITS_NONE, G, prefill=True)
+        logits = model.forward(b, kv)
+        if few:
+            yield lo, None, logits[:, :model.cfg.vocab].float()
+        else:
+            if model.last_hidden.shape[0] != len(ids):
+                raise RuntimeError(f"{type(model).__name__} kept {model.last_hidden.shape[0]} final states of {len(ids)} rows")
+            yield lo, model.last_hidden, None
 
 
 def topk_teacher(logits: torch.Tensor, k: int):
@@ -80,24 +103,44 @@ def read_sequences(a, tokenizer) -> list[list[int]]:
     return seqs
 
 
-def run(engine, seqs, chunk: int = 512, topk: int = 0, teacher: dict | None = None, log=print) -> dict:
-    """Scores the sequences one after another in slot 0. -> {"nll", "tokens", "ppl", "kl"?, "teacher"?}."""
+def run(engine, seqs, chunk: int = 512, topk: int = 0, teacher: dict | None = None, log=print, no_logits: bool = False) -> dict:
+    """Scores the sequences one after another in slot 0. -> {"nll", "tokens", "ppl", "kl"?, "teacher"?}. ``no_logits``: from the final states and the
+    head (``scoring_head``), without the logits."""
+    if no_logits:
+        from ..train.head_loss import head_cross_entropy, head_kl
+        if topk:
+            raise ValueError("a teacher is read from logits: not without them")
+        scoring = getattr(engine.model, "scoring_head", lambda: None)()
+        if scoring is None:
+            raise ValueError("scores without logits need one plain bf16 or fp32 head")
+        head, cap = scoring
+        portions = sequence_states
+    else:
+        def portions(*a):
+            return ((lo, None, lg) for lo, lg in sequence_logits(*a))
     nll, count, kl_sum, kl_n = 0.0, 0, 0.0, 0
     out_t = {"k": topk, "ids": [], "logp": [], "tail": []} if topk else None
     for si, seq in enumerate(seqs):
         engine.kv.release(0)
         parts = []
         tgt = torch.tensor(seq[1:], dtype=torch.long, device=engine.device)
-        for lo, lg in sequence_logits(engine, seq, chunk):
-            hi = min(lo + lg.shape[0], len(seq) - 1)
+        for lo, x, lg in portions(engine, seq, chunk):
+            rows = (lg if x is None else x).shape[0]
+            hi = min(lo + rows, len(seq) - 1)
             if hi > lo:
-                nll += float(F.cross_entropy(lg[: hi - lo], tgt[lo:hi], reduction="sum"))
+                if x is None:
+                    nll += float(F.cross_entropy(lg[: hi - lo], tgt[lo:hi], reduction="sum"))
+                else:
+                    nll += float(head_cross_entropy(x[: hi - lo], head, tgt[lo:hi], softcap=cap)[0].sum())
                 count += hi - lo
             if teacher is not None:
-                t_ids = teacher["ids"][si][lo:lo + lg.shape[0]].to(engine.device)
-                t_lp = teacher["logp"][si][lo:lo + lg.shape[0]].to(engine.device)
-                t_tail = teacher["tail"][si][lo:lo + lg.shape[0]].to(engine.device)
-                kl = kl_topk(lg[: t_ids.shape[0]], t_ids, t_lp, t_tail)
+                t_ids = teacher["ids"][si][lo:lo + rows].to(engine.device)
+                t_lp = teacher["logp"][si][lo:lo + rows].to(engine.device)
+                t_tail = teacher["tail"][si][lo:lo + rows].to(engine.device)
+                if x is None:
+                    kl = kl_topk(lg[: t_ids.shape[0]], t_ids, t_lp, t_tail)
+                else:
+                    kl = head_kl(x[: t_ids.shape[0]], head, t_ids, t_lp, t_tail, softcap=cap)[0]
                 kl_sum += float(kl.sum())
                 kl_n += kl.numel()
             if out_t is not None:
@@ -135,7 +178,10 @@ def main(argv=None) -> int:
     ap.add_argument("--topk-out", default="")
     ap.add_argument("--topk", type=int, default=64)
     ap.add_argument("--kl-teacher", default="")
+    ap.add_argument("--no-logits", action="store_true", help="score from the final states and the head, without holding logits")
     a = ap.parse_args(argv)
+    if a.no_logits and a.topk_out:
+        ap.error("--topk-out reads the logits: not with --no-logits")
     if sum(bool(x) for x in (a.file, a.tokens_file, a.prompts)) != 1:
         ap.error("give exactly one of --file, --tokens-file, --prompts")
     from ..models.factory import load_model
@@ -144,6 +190,8 @@ def main(argv=None) -> int:
     from ..runtime.kv_cache import PagedKVCache
     from ..runtime.route_dump import RouteRecorder
     model, _ = load_model(a.model, a.device)
+    if a.no_logits and getattr(model, "scoring_head", lambda: None)() is None:
+        ap.error("--no-logits needs one plain bf16 or fp32 head")
     tok = None
     if not a.tokens_file:
         from ..loader.tokenizer import Tokenizer
@@ -168,7 +216,7 @@ def main(argv=None) -> int:
             rec = model.route_recorder = RouteRecorder(layers, a.route_max_rows)
     teacher = torch.load(a.kl_teacher, weights_only=True) if a.kl_teacher else None
     with torch.no_grad():
-        res = run(engine, seqs, a.chunk, a.topk if a.topk_out else 0, teacher)
+        res = run(engine, seqs, a.chunk, a.topk if a.topk_out else 0, teacher, no_logits=a.no_logits)
     if hs is not None:
         files = hs.dump(a.hessian_dir)
         print(f"volta_ppl: {len(files)} capture files written to {a.hessian_dir}")

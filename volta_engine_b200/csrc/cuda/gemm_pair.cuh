@@ -40,7 +40,7 @@ VE_DEVINL void cluster_sync_all() {
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 VE_DEVINL void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // A load into this CTA's shared memory that reports to a barrier of the pair's first CTA.
 VE_DEVINL void tma_load_3d_pair(void* smem_dst, const CUtensorMap* map, uint32_t bar_cluster, int x, int y, int z) {

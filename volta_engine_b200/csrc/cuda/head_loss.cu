@@ -210,17 +210,20 @@ struct ScoreJob : LogitTiles {
       for (int j = 0; j < 128; ++j)
         if (j >= cols) z[j] = neg_inf();
     }
-    if (__any_sync(0xffffffffu, p < end)) {
-      int next = p < end ? tg.id(row, p) - v0 - col0 : 128;
+    // a token of each lane at a time: selects, for branches in the body of 128 columns fetch their code anew for every tile (20 us a tile that a target
+    // falls into)
+    while (__any_sync(0xffffffffu, p < end)) {
+      const int at = p < end ? tg.id(row, p) - v0 - col0 : -1;
+      float v = 0.f;
 #pragma unroll
-      for (int j = 0; j < 128; ++j)
-        if (j == next) {
-          do {                                      // (a token listed twice is one token)
-            zt[(size_t)row * tg.K + p] = z[j];
-            next = ++p < end ? tg.id(row, p) - v0 - col0 : 128;
-          } while (j == next);
-          z[j] = neg_inf();
-        }
+      for (int j = 0; j < 128; ++j) {
+        v = j == at ? z[j] : v;
+        z[j] = j == at ? neg_inf() : z[j];
+      }
+      if (p < end) {
+        do zt[(size_t)row * tg.K + p] = v;          // (a token listed twice is one token)
+        while (++p < end && tg.id(row, p) - v0 - col0 == at);
+      }
     }
     float m = z[0];
 #pragma unroll
@@ -265,33 +268,46 @@ struct GradJob : LogitTiles {
       c = rg[i];
       if (cols) tg.range(row, (v0 + col0) >> 7, (long)v0 + col0, cols, p, end);
     }
-    const bool any = __any_sync(0xffffffffu, p < end);
-    int next = p < end ? tg.id(row, p) - v0 - col0 : 128;
+    // targets first, one of each lane at a time: their dz takes the logit's place, and its bit says that it stands there
+    uint32_t set[4] = {0u, 0u, 0u, 0u};
+    while (__any_sync(0xffffffffu, p < end)) {
+      const int at = p < end ? tg.id(row, p) - v0 - col0 : -1;
+      float v = 0.f, d = c.at;
+#pragma unroll
+      for (int j = 0; j < 128; ++j) v = j == at ? z[j] : v;
+      if (p < end) {
+        float slope = 1.f;
+        if (CAP) {
+          const float th = tanhf(v * inv_cap);
+          v = cap * th;
+          slope = 1.f - th * th;
+        }
+        if (tg.labels) {
+          ++p;
+        } else {
+          float a = 0.f;
+          do a += expf(tg.slp[(size_t)row * tg.K + p]);
+          while (++p < end && tg.id(row, p) - v0 - col0 == at);
+          d = fmaf(c.at, ex2_approx(fmaf(v, kLog2e, -c.lse2)), -c.g * a);
+        }
+        if (CAP) d *= slope;
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) set[w] |= at >> 5 == w ? 1u << (at & 31) : 0u;
+#pragma unroll
+      for (int j = 0; j < 128; ++j) z[j] = j == at ? d : z[j];
+    }
+    const int width = on ? cols : 0;
 #pragma unroll
     for (int j = 0; j < 128; ++j) {
-      float slope = 1.f, v = z[j];
+      float slope = c.dense, v = z[j];
       if (CAP) {
         const float th = tanhf(v * inv_cap);
         v = cap * th;
-        slope = 1.f - th * th;
+        slope *= 1.f - th * th;
       }
-      const float s = ex2_approx(fmaf(v, kLog2e, -c.lse2));
-      float d = c.dense * s;
-      if (any && j == next) {
-        if (tg.labels) {
-          d = c.at;
-          next = 128;
-        } else {
-          float a = 0.f;
-          do {
-            a += expf(tg.slp[(size_t)row * tg.K + p]);
-            next = ++p < end ? tg.id(row, p) - v0 - col0 : 128;
-          } while (j == next);
-          d = fmaf(c.at, s, -c.g * a);
-        }
-      }
-      if (CAP) d *= slope;
-      z[j] = on && j < cols ? d : 0.f;              // (zeros to the ends of the tile: the products along rows and columns read them)
+      const float d = slope * ex2_approx(fmaf(v, kLog2e, -c.lse2));
+      z[j] = j >= width ? 0.f : set[j >> 5] >> (j & 31) & 1u ? z[j] : d;      // (zeros to the ends of the tile: the products along rows and columns read them)
     }
     for (int s = 0; s < slabs; ++s) {
 #pragma unroll

@@ -147,7 +147,7 @@ def test_refusals():
 
 
 # ------------------------------------------------------------------------------------------------ GPU
-SIZES = [(1, 64, 300), (1, 2048, 1000), (5, 72, 1), (3, 8, 127), (130, 136, 513), (257, 320, 1025), (300, 1001, 2050), (64, 515, 4099), (700, 256, 5000)]
+SIZES = [(1, 64, 300), (1, 2048, 1000), (5, 72, 1), (3, 8, 127), (130, 136, 513), (257, 320, 1025), (300, 1001, 2050), (64, 515, 4099), (700, 256, 5000), (12, 196, 2889)]
 
 
 @pytest.mark.gpu
@@ -160,7 +160,7 @@ def test_cross_entropy(rows, hidden, vocab, types):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,hidden,vocab,topk", [(1, 64, 300, 1), (2, 128, 40, 40), (130, 136, 513, 7), (257, 320, 1025, 64), (77, 515, 5003, 17), (9, 256, 3000, 1024)])
+@pytest.mark.parametrize("rows,hidden,vocab,topk", [(1, 64, 300, 1), (2, 128, 40, 40), (130, 136, 513, 7), (257, 320, 1025, 64), (77, 515, 5003, 17), (9, 256, 3000, 1024), (8, 132, 1877, 62)])
 @pytest.mark.parametrize("types", ["bf16 bf16", "fp32 bf16", "fp32 fp32"])
 def test_divergence(rows, hidden, vocab, topk, types):
     xt, ht = types.split()

@@ -14,16 +14,18 @@
 // Operands of more than bf16 precision come as slabs: an fp32 value is the exact sum of three bf16 values (8 + 8 + 8 bits), and the product
 // is summed over the pairs of slabs whose orders add up to two at most (what is left out is below 2^-24 of the product).
 //
-// Roles (320 threads a CTA): warp 0 loads by TMA, warp 1 of the pair's first CTA issues the MMAs, warps 2..9 sum and run the epilogue.
-// Every wait is bounded.
+// Roles (384 threads a CTA): warp 0 loads by TMA, warp 1 of the pair's first CTA issues the MMAs, warps 4..11 sum and run the epilogue. The first
+// warp group gives registers to the others: 128 x 40 + 256 x 232 = 384 x 168. Every wait is bounded.
 #pragma once
 #include "common.cuh"
 
 namespace ve {
 
 constexpr int kPairStages = 6, kPairHalf = 128 * 128, kPairStage = 2 * kPairHalf;       // bytes: 128 rows x 64 of A and of B
-constexpr int kPairSmem = kPairStages * kPairStage + 1024;
-constexpr int kPairClusters = 74, kPairThreads = 320;
+constexpr int kPairStaging = 8 * 4096;                     // behind the ring: 32 rows x 64 bf16 columns for each summing warp's stores
+constexpr int kPairSmem = kPairStages * kPairStage + kPairStaging + 1024;
+static_assert(kPairSmem <= 227 * 1024 - 512, "shared memory (beside the barriers)");
+constexpr int kPairClusters = 74, kPairThreads = 384;
 
 VE_DEVINL uint32_t cluster_rank() {
   uint32_t r;
@@ -49,6 +51,14 @@ VE_DEVINL void tma_load_3d_pair(void* smem_dst, const CUtensorMap* map, uint32_t
       ::"r"(smem_u32(smem_dst)), "l"(map), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
+// A box from shared memory to the tensor (asynchronous: the groups of the thread that asks for it).
+VE_DEVINL void tma_store_3d(const CUtensorMap* map, const void* smem_src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+               ::"l"(map), "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+VE_DEVINL void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }      // the shared memory may be written again
+VE_DEVINL void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }               // written
 VE_DEVINL void tmem_alloc_pair(uint32_t* smem_holder, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_holder)), "r"(ncols) : "memory");
 }
@@ -83,6 +93,21 @@ struct PairLoop {
   int chunk;                  // steps that a sum stays in tensor memory
 };
 
+// Steps that are worth a second look: bit k of a tile's words asks for step k once more, with the second slab of A (what the first one's rounding
+// left) and the first of B.
+VE_DEVINL uint32_t step_bits(const uint32_t* words, int w, int k0, int k1) {        // word w, cut to steps [k0, k1)
+  uint32_t b = words[w];
+  if (w == k0 >> 5) b &= 0xffffffffu << (k0 & 31);
+  if (w == k1 >> 5) b &= (1u << (k1 & 31)) - 1u;
+  return b;
+}
+VE_DEVINL int step_count(const uint32_t* words, int k0, int k1) {
+  int n = 0;
+  if (words)
+    for (int w = k0 >> 5; w * 32 < k1; ++w) n += __popc(step_bits(words, w, k0, k1));
+  return n;
+}
+
 // The pairs (i, j) of `sa` x `sb` slabs with i + j <= order, the small ones first.
 static inline PairLoop pair_loop(int sa, int sb, int order, int chunk) {
   PairLoop l{0, 0, 0, chunk};
@@ -97,10 +122,12 @@ static inline PairLoop pair_loop(int sa, int sb, int order, int chunk) {
   return l;
 }
 
-// Job: gives the tiles (int tiles(), PairTile tile(int i)) and takes the sums of a thread: finish(tile, row of the tile, first column, sums[128]).
+// Job: gives the tiles (int tiles(), PairTile tile(int i)), the words of steps to repeat (const uint32_t* again(tile), or null), what a thread loads
+// in front of its sums (Row begin(tile, row of the tile, first column)) and takes the sums: finish(tile, row of the tile, first column, Row,
+// sums[128], omap, 4 KB of shared memory of the warp); done() when there are no more.
 // A_MN / B_MN: the operand is MN-major.
 template <bool A_MN, bool B_MN, class Job>
-VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap* amap, const CUtensorMap* bmap, int* status) {
+VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap* amap, const CUtensorMap* bmap, const CUtensorMap* omap, int* status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
@@ -122,8 +149,9 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
   const uint32_t tmem_base = tmem_holder;
   const int ntiles = job.tiles();
 
-  if (warp == 0) {
-    if (elect_one()) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0 && elect_one()) {
       prefetch_tmap(amap);
       prefetch_tmap(bmap);
       int it = 0;
@@ -131,40 +159,44 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
       for (int t = cluster; t < ntiles && ok; t += clusters) {
         const PairTile tl = job.tile(t);
         const int am = tl.m0 + rank * 128, bn = tl.n0 + rank * 128;
-        for (int p = 0; p < loop.pairs && ok; ++p) {
-          const int sa = (loop.a_slab >> (4 * p)) & 15, sb = (loop.b_slab >> (4 * p)) & 15;
-          for (int k = 0; k < tl.ksteps; ++k, ++it) {
-            const int s = it % kPairStages;
-            ok = mbar_wait(&empty[s], ((it / kPairStages) & 1) ^ 1);
-            if (!ok) break;
-            uint8_t* st = smem + s * kPairStage;
-            if (rank == 0) mbar_expect_tx(&full[s], 2 * kPairStage);
-            const uint32_t bar = first_cta_addr(&full[s]);
-            const int kk = (tl.k0 + k) * 64;
-            if (A_MN) {
-              tma_load_3d_pair(st, amap, bar, am, kk, sa);
-              tma_load_3d_pair(st + kPairHalf / 2, amap, bar, am + 64, kk, sa);
-            } else {
-              tma_load_3d_pair(st, amap, bar, kk, am, sa);
-            }
-            if (B_MN) {
-              tma_load_3d_pair(st + kPairHalf, bmap, bar, bn, kk, sb);
-              tma_load_3d_pair(st + kPairHalf + kPairHalf / 2, bmap, bar, bn + 64, kk, sb);
-            } else {
-              tma_load_3d_pair(st + kPairHalf, bmap, bar, kk, bn, sb);
-            }
+        auto load = [&](int k, int sa, int sb) {
+          const int s = it % kPairStages;
+          if (!mbar_wait(&empty[s], ((it / kPairStages) & 1) ^ 1)) return false;
+          ++it;
+          uint8_t* st = smem + s * kPairStage;
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * kPairStage);
+          const uint32_t bar = first_cta_addr(&full[s]);
+          const int kk = k * 64;
+          if (A_MN) {
+            tma_load_3d_pair(st, amap, bar, am, kk, sa);
+            tma_load_3d_pair(st + kPairHalf / 2, amap, bar, am + 64, kk, sa);
+          } else {
+            tma_load_3d_pair(st, amap, bar, kk, am, sa);
           }
-        }
+          if (B_MN) {
+            tma_load_3d_pair(st + kPairHalf, bmap, bar, bn, kk, sb);
+            tma_load_3d_pair(st + kPairHalf + kPairHalf / 2, bmap, bar, bn + 64, kk, sb);
+          } else {
+            tma_load_3d_pair(st + kPairHalf, bmap, bar, kk, bn, sb);
+          }
+          return true;
+        };
+        for (int p = 0; p < loop.pairs && ok; ++p)
+          for (int k = 0; k < tl.ksteps && ok; ++k) ok = load(tl.k0 + k, (loop.a_slab >> (4 * p)) & 15, (loop.b_slab >> (4 * p)) & 15);
+        const uint32_t* words = job.again(tl);
+        const int k1 = tl.k0 + tl.ksteps;
+        if (words)
+          for (int w = tl.k0 >> 5; w * 32 < k1 && ok; ++w)
+            for (uint32_t bits = step_bits(words, w, tl.k0, k1); bits && ok; bits &= bits - 1) ok = load(w * 32 + __ffs(bits) - 1, 1, 0);
       }
       if (!ok) atomicExch(&s_fail, 1);
-    }
-  } else if (warp == 1) {
-    if (rank == 0 && elect_one()) {
+    } else if (warp == 1 && rank == 0 && elect_one()) {
       constexpr uint32_t idesc = make_idesc_f16(1, 1, 256, 256) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
       int it = 0, piece = 0;
       bool ok = true;
       for (int t = cluster; t < ntiles && ok; t += clusters) {
-        const int total = job.tile(t).ksteps * loop.pairs;
+        const PairTile tl = job.tile(t);
+        const int total = tl.ksteps * loop.pairs + step_count(job.again(tl), tl.k0, tl.k0 + tl.ksteps);
         for (int i = 0; i < total && ok; ++piece) {
           const int buf = piece & 1;
           ok = mbar_wait(&acc_empty[buf], ((piece >> 1) & 1) ^ 1);
@@ -191,13 +223,15 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
       if (!ok) atomicExch(&s_fail, 1);
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
     int piece = 0;
     bool ok = true;
     for (int t = cluster; t < ntiles; t += clusters) {
       const PairTile tl = job.tile(t);
-      const int total = tl.ksteps * loop.pairs, pieces = (total + loop.chunk - 1) / loop.chunk;
+      const int total = tl.ksteps * loop.pairs + step_count(job.again(tl), tl.k0, tl.k0 + tl.ksteps), pieces = (total + loop.chunk - 1) / loop.chunk;
+      const auto row = job.begin(tl, rank * 128 + quarter * 32 + lane, half * 128);
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.f;
@@ -220,8 +254,9 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
         if (lane == 0) mbar_arrive_cluster(first_cta_addr(&acc_empty[buf]));
       }
       if (!ok) break;
-      job.finish(tl, rank * 128 + quarter * 32 + lane, half * 128, acc);
+      job.finish(tl, rank * 128 + quarter * 32 + lane, half * 128, row, acc, omap, smem + kPairStages * kPairStage + (warp - 4) * 4096);
     }
+    job.done();
     if (!ok) atomicExch(&s_fail, 1);
   }
   tc_fence_before();

@@ -12,8 +12,10 @@
 // of exponentials without the targets, and the targets' logits; one more pass over these few numbers gives the loss. The targets are left
 // out of the sums so that log(1 + exp(..)) and log(rho) do not come from the difference of two nearly equal numbers. The gradient computes the
 // logits again, a piece of the vocabulary at a time, writes dz of that piece in bf16 slabs (rows x piece: the only array of that kind) and
-// multiplies it with the head's rows and with the states. dz is rounded to the operands' precision: bf16 for bf16 states (half a unit, 2^-9 of its
-// value, as the rounding of the gradient itself), three bf16 slabs (fp32's 24 bits) for fp32 states.
+// multiplies it with the head's rows and with the states. dz beside fp32 operands is three bf16 slabs (fp32's 24 bits). Beside bf16 operands it is one
+// slab, and what its rounding left (up to 2^-8 of a value: as much as the rounding of the gradients, whose error it would raise by 1.41, with few
+// rows by up to 2.5) in a second one that is multiplied only where it matters: blocks of 64 x 64 in which an element is above a sixteenth of its
+// row's largest (a label's own dz is at least every other's; for a teacher's tokens, above 2^-10 of the row's weight). Those are few: a label a row.
 // Sums run in a fixed order: the same call gives the same bits.
 //
 // Rows that are left out (label below zero, a teacher row of padding) are taken out in front: the states of the others are gathered, so what
@@ -172,6 +174,15 @@ struct LogitTiles {           // rows x a piece of the vocabulary: tiles of up t
   int v0, nv, ksteps;
   VE_DEVINL int row_tiles() const { return (*count + 255) >> 8; }
   VE_DEVINL int tiles() const { return row_tiles() * ((nv + 255) >> 8); }
+  VE_DEVINL const uint32_t* again(const PairTile&) const { return nullptr; }
+  VE_DEVINL void done() const {}
+  struct Row { int row, begin, end; };        // the caller's row (-1: behind the last one), its targets among the thread's columns
+  VE_DEVINL Row row_at(const PairTile& t, int r, int c0, const int* live, const Targets& tg) const {
+    const int i = t.m0 + r, col0 = t.n0 + c0;
+    Row w{i < *count ? live[i] : -1, 0, 0};
+    if (w.row >= 0 && col0 < nv) tg.range(w.row, (v0 + col0) >> 7, (long)v0 + col0, min(128, nv - col0), w.begin, w.end);
+    return w;
+  }
   VE_DEVINL PairTile tile(int i) const {
     const int nm = row_tiles(), nn = (nv + 255) >> 8, per = 16 * nn;
     const int g = i / per, m_first = g * 16, gm = min(16, nm - m_first), j = i - g * per;
@@ -195,15 +206,15 @@ struct ScoreJob : LogitTiles {
   float2* part;               // [128-column block][row]: maximum and sum of exp(z - maximum) without the targets
   float* zt;                  // [R, K] logits of the targets, in the targets' ascending order
   float cap, inv_cap;
+  using Row = LogitTiles::Row;
+  VE_DEVINL Row begin(const PairTile& t, int r, int c0) const { return row_at(t, r, c0, live, tg); }
 
-  VE_DEVINL void finish(const PairTile& t, int r, int c0, float* z) const {
-    const int i = t.m0 + r, n = *count;
-    if (t.m0 + (r & ~31) >= n || t.n0 + c0 >= nv) return;
-    const bool on = i < n;
-    const int row = on ? live[i] : 0;
-    const int col0 = t.n0 + c0, cols = min(128, nv - col0), blk = (v0 + col0) >> 7;
-    int p = 0, end = 0;
-    if (on) tg.range(row, blk, (long)v0 + col0, cols, p, end);
+  VE_DEVINL void finish(const PairTile& t, int r, int c0, const Row& w, float* z, const CUtensorMap* omap, uint8_t* staging) const {
+    const int i = t.m0 + r, row = w.row, col0 = t.n0 + c0, cols = min(128, nv - col0), blk = (v0 + col0) >> 7;
+    if (!__any_sync(0xffffffffu, row >= 0) || cols <= 0) return;
+    const bool on = row >= 0;
+    int p = w.begin;
+    const int end = w.end;
     cap_logits<CAP>(z, cap, inv_cap);
     if (cols < 128) {
 #pragma unroll
@@ -244,6 +255,14 @@ struct ScoreJob : LogitTiles {
 // Constants of a row's dz: at any token dense * s, at a target `at` * s - g * (teacher's mass); a label's is `at` itself.
 struct RowGrad {
   float lse2, dense, at, g;
+  float large;                // dz above this is multiplied with its rounding error too
+};
+
+// Blocks of 64 x 64 of a piece's dz with large elements: by tiles of 256 rows, bits over the columns' blocks (dx), and by tiles of 256 columns,
+// bits over the rows' blocks (dhead).
+struct LargeBlocks {
+  uint32_t *of_rows, *of_cols;
+  int row_words, col_words;   // words of a tile
 };
 
 template <bool CAP>
@@ -251,23 +270,22 @@ struct GradJob : LogitTiles {
   Targets tg;
   const int* live;
   const RowGrad* rg;          // by gathered row
-  __nv_bfloat16* G;           // [slabs][rows_cap][pitch]
-  size_t slab;
-  int slabs, pitch;
+  int slabs;                  // of dz
+  LargeBlocks big;            // (null: every slab counts everywhere)
   float cap, inv_cap;
 
-  VE_DEVINL void finish(const PairTile& t, int r, int c0, float* z) const {
-    const int i = t.m0 + r, n = *count;
-    const bool on = i < n;
+  struct Row : LogitTiles::Row { RowGrad c; };
+  VE_DEVINL Row begin(const PairTile& t, int r, int c0) const {
+    Row w{row_at(t, r, c0, live, tg), {0.f, 0.f, 0.f, 0.f, 0.f}};
+    if (w.row >= 0) w.c = rg[t.m0 + r];
+    return w;
+  }
+
+  VE_DEVINL void finish(const PairTile& t, int r, int c0, const Row& w, float* z, const CUtensorMap* omap, uint8_t* staging) const {
+    const int i = t.m0 + r, row = w.row, end = w.end;
     const int col0 = t.n0 + c0, cols = max(0, min(128, nv - col0));
-    __nv_bfloat16* dst = G + (size_t)i * pitch + col0;
-    const int row = on ? live[i] : 0;
-    int p = 0, end = 0;
-    RowGrad c{0.f, 0.f, 0.f, 0.f};
-    if (on) {
-      c = rg[i];
-      if (cols) tg.range(row, (v0 + col0) >> 7, (long)v0 + col0, cols, p, end);
-    }
+    const RowGrad c = w.c;
+    int p = w.begin;
     // targets first, one of each lane at a time: their dz takes the logit's place, and its bit says that it stands there
     uint32_t set[4] = {0u, 0u, 0u, 0u};
     while (__any_sync(0xffffffffu, p < end)) {
@@ -297,27 +315,62 @@ struct GradJob : LogitTiles {
 #pragma unroll
       for (int j = 0; j < 128; ++j) z[j] = j == at ? d : z[j];
     }
-    const int width = on ? cols : 0;
 #pragma unroll
     for (int j = 0; j < 128; ++j) {
-      float slope = c.dense, v = z[j];
+      float f = c.dense, v = z[j];
       if (CAP) {
         const float th = tanhf(v * inv_cap);
         v = cap * th;
-        slope *= 1.f - th * th;
+        f *= 1.f - th * th;
       }
-      const float d = slope * ex2_approx(fmaf(v, kLog2e, -c.lse2));
-      z[j] = j >= width ? 0.f : set[j >> 5] >> (j & 31) & 1u ? z[j] : d;      // (zeros to the ends of the tile: the products along rows and columns read them)
+      const float d = f * ex2_approx(fmaf(v, kLog2e, -c.lse2));
+      z[j] = set[j >> 5] >> (j & 31) & 1u ? z[j] : d;
     }
-    for (int s = 0; s < slabs; ++s) {
+    if (__any_sync(0xffffffffu, row < 0 || cols < 128)) {        // zeros to the ends of the tile: the products along rows and columns read them
+      const int width = row >= 0 ? cols : 0;
 #pragma unroll
-      for (int j = 0; j < 128; j += 8) {
-        __nv_bfloat16 b[8];
+      for (int j = 0; j < 128; ++j) z[j] = j < width ? z[j] : 0.f;
+    }
+    if (big.of_rows) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[j + e] = split_bf16(z[j + e], b[e]);
-        *reinterpret_cast<uint4*>(dst + s * slab + j) = *reinterpret_cast<const uint4*>(b);
+      for (int h = 0; h < 2; ++h) {
+        float m = 0.f;
+#pragma unroll
+        for (int j = 64 * h; j < 64 * h + 64; ++j) m = fmaxf(m, fabsf(z[j]));
+        if (__any_sync(0xffffffffu, m > c.large) && (threadIdx.x & 31) == 0) {
+          const int kc = (col0 >> 6) + h, kr = i >> 6;
+          atomicOr(big.of_rows + (t.m0 >> 8) * big.row_words + (kc >> 5), 1u << (kc & 31));
+          atomicOr(big.of_cols + (t.n0 >> 8) * big.col_words + (kr >> 5), 1u << (kr & 31));
+        }
       }
     }
+    // out by TMA, 32 rows x 64 columns at a time: a thread's own stores are 16 bytes of 32 different rows each, 12 000 cycles a tile of three slabs
+    const int lane = threadIdx.x & 31;
+    for (int s = 0; s < slabs; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (lane == 0) tma_store_wait_read();
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 64; j += 8) {
+          uint32_t b[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float &lo = z[64 * h + j + 2 * e], &hi = z[64 * h + j + 2 * e + 1];
+            const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+            b[e] = *reinterpret_cast<const uint32_t*>(&v);
+            lo -= __uint_as_float(b[e] << 16);
+            hi -= __uint_as_float(b[e] & 0xffff0000u);
+          }
+          *reinterpret_cast<uint4*>(staging + lane * 128 + (((j >> 3) ^ (lane & 7)) << 4)) = make_uint4(b[0], b[1], b[2], b[3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) tma_store_3d(omap, staging, col0 + 64 * h, i, s);
+      }
+  }
+  VE_DEVINL void done() const {
+    if ((threadIdx.x & 31) == 0) tma_store_wait();
   }
 };
 
@@ -327,6 +380,11 @@ struct DxJob {
   int H, Hp, ksteps, splits, first;
   size_t slab;
   float* acc;                 // [splits][rows_cap][Hp]
+  LargeBlocks big;
+  struct Row {};
+  VE_DEVINL Row begin(const PairTile&, int, int) const { return {}; }
+  VE_DEVINL void done() const {}
+  VE_DEVINL const uint32_t* again(const PairTile& t) const { return big.of_rows ? big.of_rows + (t.m0 >> 8) * big.row_words : nullptr; }
   VE_DEVINL int row_tiles() const { return (*count + 255) >> 8; }
   VE_DEVINL int tiles() const { return row_tiles() * ((H + 255) >> 8) * splits; }
   VE_DEVINL PairTile tile(int i) const {
@@ -334,7 +392,7 @@ struct DxJob {
     const int m = i % nm, j = i / nm, s = j % splits;
     return PairTile{m * 256, (j / splits) * 256, s * per, max(0, min(per, ksteps - s * per)), s};
   }
-  VE_DEVINL void finish(const PairTile& t, int r, int c0, float* z) const {
+  VE_DEVINL void finish(const PairTile& t, int r, int c0, const Row& w, float* z, const CUtensorMap* omap, uint8_t* staging) const {
     const int i = t.m0 + r;
     if (i >= *count) return;
     float* dst = acc + t.split * slab + (size_t)i * Hp + t.n0 + c0;
@@ -342,12 +400,10 @@ struct DxJob {
 #pragma unroll
     for (int j = 0; j < 128; j += 4) {
       if (j >= cols) continue;
-      float4 v = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
-      if (!first) {
-        const float4 o = *reinterpret_cast<const float4*>(dst + j);
-        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-      }
-      *reinterpret_cast<float4*>(dst + j) = v;
+      if (first)
+        *reinterpret_cast<float4*>(dst + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
+      else                       // (one addition to each sum a piece, the pieces in order: no choice of order; waiting for the old sums took 17 % of a piece)
+        asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst + j), "f"(z[j]), "f"(z[j + 1]), "f"(z[j + 2]), "f"(z[j + 3]) : "memory");
     }
   }
 };
@@ -358,12 +414,17 @@ struct DheadJob {
   const int* count;
   int nv, H;
   T* out;                     // [nv, H], contiguous rows
+  LargeBlocks big;
+  struct Row {};
+  VE_DEVINL Row begin(const PairTile&, int, int) const { return {}; }
+  VE_DEVINL void done() const {}
+  VE_DEVINL const uint32_t* again(const PairTile& t) const { return big.of_cols ? big.of_cols + (t.m0 >> 8) * big.col_words : nullptr; }
   VE_DEVINL int tiles() const { return ((nv + 255) >> 8) * ((H + 255) >> 8); }
   VE_DEVINL PairTile tile(int i) const {
     const int nn = (H + 255) >> 8;
     return PairTile{i / nn * 256, i % nn * 256, 0, (*count + 63) >> 6, 0};
   }
-  VE_DEVINL void finish(const PairTile& t, int r, int c0, float* z) const {
+  VE_DEVINL void finish(const PairTile& t, int r, int c0, const Row& w, float* z, const CUtensorMap* omap, uint8_t* staging) const {
     const int v = t.m0 + r;
     if (v >= nv) return;
     T* dst = out + (size_t)v * H + t.n0 + c0;
@@ -393,8 +454,9 @@ struct DheadJob {
 
 template <bool A_MN, bool B_MN, class Job>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-head_gemm_kernel(const Job job, const PairLoop loop, const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, int* status) {
-  pair_gemm<A_MN, B_MN>(job, loop, &amap, &bmap, status);
+head_gemm_kernel(const Job job, const PairLoop loop, const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
+                 const __grid_constant__ CUtensorMap omap, int* status) {
+  pair_gemm<A_MN, B_MN>(job, loop, &amap, &bmap, &omap, status);
 }
 
 // ------------------------------------------------------------------------------------------------ the rows' sums
@@ -493,19 +555,23 @@ __global__ void __launch_bounds__(256) head_rowgrad_kernel(const HeadRows p, con
   const int row = live[i];
   const float lse = stats[row], rest = stats[p.R + row], g = dloss[row];
   RowGrad c;
+  // exp(z - lse) as 2^(z log2e - lse2): what the product lse log2e loses to rounding goes into the factors
   c.lse2 = lse * kLog2e;
+  const float fix = exp2f(-fmaf(lse, kLog2e, -c.lse2));
   c.g = g;
   if (p.labels) {
-    c.dense = g;
+    c.dense = g * fix;
     c.at = -g * expf(rest - lse);
+    c.large = fabsf(c.at) * (1.f / 16.f);
   } else {
     double a = 0.0;
     for (int k = lane; k < p.K; k += 32) a += exp((double)slp[(size_t)row * p.K + k]);      // (padding: exp(-inf) = 0)
     for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
     const double t = exp((double)p.tail[row]), lr = (double)rest - (double)lse;
     const bool above = lr >= -27.631021115928547;
-    c.at = (float)(g * (a + (above ? t : 0.0)));
-    c.dense = (float)(g * (a + (above ? t - t * exp(-lr) : 0.0)));
+    c.at = (float)(g * (a + (above ? t : 0.0))) * fix;
+    c.dense = (float)(g * (a + (above ? t - t * exp(-lr) : 0.0))) * fix;
+    c.large = fabsf(g) * (1.f / 1024.f);
   }
   if (lane == 0) rg[i] = c;
 }
@@ -513,7 +579,7 @@ __global__ void __launch_bounds__(256) head_rowgrad_kernel(const HeadRows p, con
 // dx of the caller's rows from the ranges' sums; zeros where a row was left out.
 template <typename T>
 __global__ void __launch_bounds__(256) head_dx_kernel(const int* pos, int R, int H, int Hp, int splits, size_t slab, const float* acc, T* dx) {
-  const int per = Hp / 4;
+  const int per = (H + 3) / 4;
   const bool vec = !((uintptr_t)dx & 15) && H % 4 == 0;
   for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < (size_t)R * per; i += (size_t)gridDim.x * blockDim.x) {
     const int r = (int)(i / per), c = (int)(i - (size_t)r * per) * 4;
@@ -544,9 +610,10 @@ struct HeadPlan {             // sizes and places in the workspace
   int Hp, sx, sw, sg;         // padded width; slabs of the states, the head, dz
   int rows_cap, nblk, ksteps;
   bool pack_head;             // the head's rows go through slabs of their own, a piece at a time
-  int piece;                  // vocabulary rows at a time (0: all at once)
-  int splits;
-  size_t live, pos, count, flag, sid, slp, off, x, part, zt, rg, head, G, acc, bytes;
+  int piece;                  // vocabulary rows at a time
+  int splits;                 // ranges of a piece that dx is summed over
+  int row_words, col_words;   // of LargeBlocks
+  size_t live, pos, count, flag, sid, slp, off, x, part, zt, rg, head, G, acc, big, big_bytes, bytes;
 };
 
 static inline int blocks_of(size_t n, int per = 256) {
@@ -560,7 +627,7 @@ static HeadPlan head_plan(bool grads, bool want_dx, int x_fp32, int head_fp32, b
   p.Hp = (H + 7) / 8 * 8;
   p.sx = x_fp32 ? 3 : 1;
   p.sw = head_fp32 ? 3 : 1;
-  p.sg = x_fp32 || head_fp32 ? 3 : 1;
+  p.sg = x_fp32 || head_fp32 ? 3 : 2;
   p.rows_cap = (R + 255) / 256 * 256;
   p.nblk = (V + 127) / 128;
   p.ksteps = (H + 63) / 64;
@@ -569,11 +636,16 @@ static HeadPlan head_plan(bool grads, bool want_dx, int x_fp32, int head_fp32, b
   if (pack_head) { const size_t most = (512ull << 20) / ((size_t)p.sw * p.Hp * 2) / 256 * 256; piece = piece < most ? piece : (most ? most : 256); }
   if (grads) { const size_t most = (256ull << 20) / ((size_t)p.sg * p.rows_cap * 2) / 256 * 256; piece = piece < most ? piece : (most ? most : 256); }
   p.piece = (int)piece;
-  // dx: few tiles share a long vocabulary
-  const int tiles = p.rows_cap / 256 * ((H + 255) / 256);
-  const int steps = p.piece / 64;
-  p.splits = tiles >= kPairClusters ? 1 : kPairClusters / tiles;
-  while (p.splits > 1 && steps / p.splits < 8) --p.splits;
+  // dx: tiles x ranges fill whole waves of the 74 pairs; a range costs about 12 steps beside its products (sums read and written)
+  const long tiles = (long)(p.rows_cap / 256) * ((H + 255) / 256), steps = p.piece / 64;
+  const int pairs = x_fp32 ? (head_fp32 ? 6 : 3) : (head_fp32 ? 3 : 1);
+  long best = 0;
+  p.splits = 1;
+  for (int s = 1; s <= kPairClusters && s * 4 <= steps; ++s) {
+    const long cost = (tiles * s + kPairClusters - 1) / kPairClusters * ((steps + s - 1) / s * pairs + 12);
+    if (s == 1 || cost < best) { best = cost; p.splits = s; }
+    if (tiles * s > 8 * kPairClusters) break;
+  }
   size_t at = 0;
   auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
   p.live = take(4ull * R); p.pos = take(4ull * R); p.count = take(4);
@@ -581,11 +653,16 @@ static HeadPlan head_plan(bool grads, bool want_dx, int x_fp32, int head_fp32, b
   if (kl) { p.flag = take(4ull * R); p.sid = take(4ull * R * K); p.slp = take(4ull * R * K); p.off = take(2ull * R * (p.nblk + 1)); }
   p.x = take(2ull * p.sx * p.rows_cap * p.Hp);
   p.head = pack_head ? take(2ull * p.sw * p.piece * p.Hp) : 0;
-  p.part = p.zt = p.rg = p.G = p.acc = 0;
+  p.part = p.zt = p.rg = p.G = p.acc = p.big = p.big_bytes = 0;
+  p.row_words = p.col_words = 0;
   if (!grads) { p.part = take(8ull * p.nblk * p.rows_cap); p.zt = take(4ull * R * (kl ? K : 1)); }
   else {
     p.rg = take(sizeof(RowGrad) * (size_t)p.rows_cap);
     p.G = take(2ull * p.sg * p.rows_cap * p.piece);
+    p.row_words = (p.piece / 64 + 31) / 32;
+    p.col_words = (p.rows_cap / 64 + 31) / 32;
+    p.big_bytes = p.sg == 2 ? 4ull * (p.rows_cap / 256 * p.row_words + p.piece / 256 * p.col_words) : 0;
+    p.big = take(p.big_bytes);
     if (want_dx) p.acc = take(4ull * p.splits * p.rows_cap * p.Hp);
   }
   p.bytes = at;
@@ -605,15 +682,16 @@ struct HeadCall {
 
 static bool head_packs(const void* head, int head_fp32, long ldw, int H) { return head_fp32 || H % 8 || ldw % 8 || ((uintptr_t)head & 15); }
 
-static int slab_map(CUtensorMap* m, const void* base, int slabs, uint64_t slab_rows, uint64_t rows, uint64_t cols, uint64_t pitch, bool mn) {
-  return make_tmap_3d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, slabs, rows, cols, slab_rows * pitch * 2, pitch * 2, mn ? 64 : 128, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+// Boxes of 64 columns and 128 rows (an operand along its columns), 64 rows (one along its rows) or 32 (a warp's stores).
+static int slab_map(CUtensorMap* m, const void* base, int slabs, uint64_t slab_rows, uint64_t rows, uint64_t cols, uint64_t pitch, int box_rows) {
+  return make_tmap_3d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, slabs, rows, cols, slab_rows * pitch * 2, pitch * 2, box_rows, 64, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <bool A_MN, bool B_MN, class Job>
-static int launch_pair(const Job& job, const PairLoop& loop, const CUtensorMap& a, const CUtensorMap& b, const HeadCall& c) {
+static int launch_pair(const Job& job, const PairLoop& loop, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const HeadCall& c) {
   cudaError_t e = allow_smem<head_gemm_kernel<A_MN, B_MN, Job>>(kPairSmem);
   if (e != cudaSuccess) return (int)e;
-  head_gemm_kernel<A_MN, B_MN, Job><<<2 * kPairClusters, kPairThreads, kPairSmem, c.st>>>(job, loop, a, b, c.status);
+  head_gemm_kernel<A_MN, B_MN, Job><<<2 * kPairClusters, kPairThreads, kPairSmem, c.st>>>(job, loop, a, b, o, c.status);
   return (int)cudaGetLastError();
 }
 
@@ -634,14 +712,14 @@ static void head_front(const HeadCall& c, const HeadPlan& p) {
 }
 
 // The head's rows [v0, v0 + nv) as an operand: in place, or packed.
-static int head_rows_map(CUtensorMap* m, const HeadCall& c, const HeadPlan& p, int v0, int nv, bool mn, bool pack) {
-  if (!p.pack_head) return slab_map(m, (const __nv_bfloat16*)c.head + (size_t)v0 * c.ldw, 1, nv, nv, c.H, c.ldw, mn);
+static int head_rows_map(CUtensorMap* m, const HeadCall& c, const HeadPlan& p, int v0, int nv, int box_rows, bool pack) {
+  if (!p.pack_head) return slab_map(m, (const __nv_bfloat16*)c.head + (size_t)v0 * c.ldw, 1, nv, nv, c.H, c.ldw, box_rows);
   if (pack) {
     const size_t slab = (size_t)p.piece * p.Hp;
     if (c.head_fp32) pack_rows<float>((const float*)c.head + (size_t)v0 * c.ldw, c.ldw, nullptr, nullptr, nv, c, p, p.sw, slab, c.ws + p.head);
     else pack_rows<__nv_bfloat16>((const __nv_bfloat16*)c.head + (size_t)v0 * c.ldw, c.ldw, nullptr, nullptr, nv, c, p, p.sw, slab, c.ws + p.head);
   }
-  return slab_map(m, c.ws + p.head, p.sw, p.piece, nv, p.Hp, p.Hp, mn);
+  return slab_map(m, c.ws + p.head, p.sw, p.piece, nv, p.Hp, p.Hp, box_rows);
 }
 
 static Targets head_targets_of(const HeadCall& c, const HeadPlan& p) {
@@ -650,14 +728,14 @@ static Targets head_targets_of(const HeadCall& c, const HeadPlan& p) {
 }
 
 constexpr int kExactChunk = 4;         // steps of 64 between fp32 additions where 32 bits are asked for
-constexpr int kRoundedChunk = 16;      // where the result is rounded to bf16 (cut-off sums over 1024: 1e-6)
+constexpr int kRoundedChunk = 32;      // where the result is rounded to bf16 (cut-off sums over 2048: 2e-6), or a gradient's logits are (2e-6 of z: 2^-15 of s)
 
 template <bool CAP>
 static int head_score(const HeadCall& c, const HeadPlan& p, float* loss, float* stats) {
   head_front(c, p);
   const int *live = (const int*)(c.ws + p.live), *pos = (const int*)(c.ws + p.pos), *count = (const int*)(c.ws + p.count);
   CUtensorMap xm, wm;
-  int rc = slab_map(&xm, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, false);
+  int rc = slab_map(&xm, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, 128);
   if (rc) return rc;
   ScoreJob<CAP> job;
   job.count = count; job.ksteps = p.ksteps; job.tg = head_targets_of(c, p); job.live = live; job.rows_cap = p.rows_cap;
@@ -665,8 +743,8 @@ static int head_score(const HeadCall& c, const HeadPlan& p, float* loss, float* 
   for (int v0 = 0; v0 < c.rows.V; v0 += p.piece) {
     job.v0 = v0;
     job.nv = c.rows.V - v0 < p.piece ? c.rows.V - v0 : p.piece;
-    if ((rc = head_rows_map(&wm, c, p, v0, job.nv, false, true))) return rc;
-    if ((rc = launch_pair<false, false>(job, pair_loop(p.sx, p.sw, 2, kExactChunk), xm, wm, c))) return rc;
+    if ((rc = head_rows_map(&wm, c, p, v0, job.nv, 128, true))) return rc;
+    if ((rc = launch_pair<false, false>(job, pair_loop(p.sx, p.sw, 2, kExactChunk), xm, wm, xm, c))) return rc;
   }
   head_merge_kernel<<<(c.rows.R + 31) / 32, 1024, 0, c.st>>>(c.rows, live, count, p.rows_cap, p.nblk, job.part, job.zt, job.tg.sid, job.tg.slp, loss, stats);
   head_blank_kernel<<<(c.rows.R + 255) / 256, 256, 0, c.st>>>(pos, c.rows.R, loss, stats);
@@ -680,36 +758,45 @@ static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, c
   const int R = c.rows.R, H = c.H;
   RowGrad* rg = (RowGrad*)(c.ws + p.rg);
   head_rowgrad_kernel<<<(R + 7) / 8, 256, 0, c.st>>>(c.rows, live, count, stats, (const float*)(c.ws + p.slp), dloss, rg);
-  CUtensorMap xk, xmn, wk, wmn, gk, gmn;
-  int rc = slab_map(&xk, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, false);
-  if (!rc) rc = slab_map(&xmn, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, true);
-  if (!rc) rc = slab_map(&gk, c.ws + p.G, p.sg, p.rows_cap, p.rows_cap, p.piece, p.piece, false);
-  if (!rc) rc = slab_map(&gmn, c.ws + p.G, p.sg, p.rows_cap, p.rows_cap, p.piece, p.piece, true);
+  CUtensorMap xk, xmn, wk, wmn, gk, gmn, gout;
+  int rc = slab_map(&xk, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, 128);
+  if (!rc) rc = slab_map(&xmn, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, 64);
+  if (!rc) rc = slab_map(&gk, c.ws + p.G, p.sg, p.rows_cap, p.rows_cap, p.piece, p.piece, 128);
+  if (!rc) rc = slab_map(&gmn, c.ws + p.G, p.sg, p.rows_cap, p.rows_cap, p.piece, p.piece, 64);
+  if (!rc) rc = slab_map(&gout, c.ws + p.G, p.sg, p.rows_cap, p.rows_cap, p.piece, p.piece, 32);
   if (rc) return rc;
   GradJob<CAP> gj;
-  gj.count = count; gj.ksteps = p.ksteps; gj.tg = head_targets_of(c, p); gj.live = live; gj.rg = rg; gj.G = (__nv_bfloat16*)(c.ws + p.G);
-  gj.slab = (size_t)p.rows_cap * p.piece; gj.slabs = p.sg; gj.pitch = p.piece; gj.cap = c.softcap; gj.inv_cap = CAP ? 1.f / c.softcap : 0.f;
-  DxJob xj{count, H, p.Hp, 0, p.splits, 1, (size_t)p.rows_cap * p.Hp, (float*)(c.ws + p.acc)};
+  gj.count = count; gj.ksteps = p.ksteps; gj.tg = head_targets_of(c, p); gj.live = live; gj.rg = rg;
+  gj.slabs = p.sg; gj.cap = c.softcap; gj.inv_cap = CAP ? 1.f / c.softcap : 0.f;
+  uint32_t* const words = (uint32_t*)(c.ws + p.big);
+  const LargeBlocks big{p.big_bytes ? words : nullptr, p.big_bytes ? words + p.rows_cap / 256 * p.row_words : nullptr, p.row_words, p.col_words};
+  gj.big = big;
+  DxJob xj{count, H, p.Hp, 0, p.splits, 1, (size_t)p.rows_cap * p.Hp, (float*)(c.ws + p.acc), big};
+  const bool exact = p.sg == 3;
   for (int v0 = 0; v0 < c.rows.V; v0 += p.piece) {
     const int nv = c.rows.V - v0 < p.piece ? c.rows.V - v0 : p.piece;
     gj.v0 = v0;
     gj.nv = nv;
-    if ((rc = head_rows_map(&wk, c, p, v0, nv, false, true))) return rc;
-    if ((rc = launch_pair<false, false>(gj, pair_loop(p.sx, p.sw, 2, kExactChunk), xk, wk, c))) return rc;
+    if ((rc = head_rows_map(&wk, c, p, v0, nv, 128, true))) return rc;
+    if (p.big_bytes) {
+      const cudaError_t e = cudaMemsetAsync(words, 0, p.big_bytes, c.st);
+      if (e != cudaSuccess) return (int)e;
+    }
+    if ((rc = launch_pair<false, false>(gj, pair_loop(p.sx, p.sw, 2, exact ? kExactChunk : kRoundedChunk), xk, wk, gout, c))) return rc;
     if (dx) {
-      if ((rc = head_rows_map(&wmn, c, p, v0, nv, true, false))) return rc;
+      if ((rc = head_rows_map(&wmn, c, p, v0, nv, 64, false))) return rc;
       xj.ksteps = (nv + 63) / 64;
       xj.first = v0 == 0;
-      const PairLoop loop = c.x_fp32 ? pair_loop(p.sg, p.sw, 2, kExactChunk) : pair_loop(p.sg, p.sw, p.sg > 1 ? 1 : 0, kRoundedChunk);
-      if ((rc = launch_pair<false, true>(xj, loop, gk, wmn, c))) return rc;
+      const PairLoop loop = c.x_fp32 ? pair_loop(p.sg, p.sw, 2, kExactChunk) : pair_loop(p.sg, p.sw, exact ? 1 : 0, kRoundedChunk);
+      if ((rc = launch_pair<false, true>(xj, loop, gk, wmn, gk, c))) return rc;
     }
     if (dhead) {
       if (c.head_fp32) {
-        const DheadJob<float> job{count, nv, H, (float*)dhead + (size_t)v0 * H};
-        rc = launch_pair<true, true>(job, pair_loop(p.sg, p.sx, 2, kExactChunk), gmn, xmn, c);
+        const DheadJob<float> job{count, nv, H, (float*)dhead + (size_t)v0 * H, big};
+        rc = launch_pair<true, true>(job, pair_loop(p.sg, p.sx, 2, kExactChunk), gmn, xmn, gmn, c);
       } else {
-        const DheadJob<__nv_bfloat16> job{count, nv, H, (__nv_bfloat16*)dhead + (size_t)v0 * H};
-        rc = launch_pair<true, true>(job, pair_loop(p.sg, p.sx, p.sg > 1 ? 1 : 0, kRoundedChunk), gmn, xmn, c);
+        const DheadJob<__nv_bfloat16> job{count, nv, H, (__nv_bfloat16*)dhead + (size_t)v0 * H, big};
+        rc = launch_pair<true, true>(job, pair_loop(p.sg, p.sx, exact ? 1 : 0, kRoundedChunk), gmn, xmn, gmn, c);
       }
       if (rc) return rc;
     }

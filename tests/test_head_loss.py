@@ -357,6 +357,14 @@ def test_pieces_of_the_vocabulary():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("topk", [0, 3])
+def test_many_rows(topk):
+    """More rows than one block looks through for those that count."""
+    a = make(9001, 32, 300, topk, seed=5, left_out=0.3, device="cuda")
+    hold(run(*a), *a, 0.0)
+
+
+@pytest.mark.gpu
 def test_offsets_that_pass_32_bits():
     """A head of 2.2 G values; the last rows' labels stand at its end."""
     vocab, hidden = 540000, 4096

@@ -98,12 +98,16 @@ def ptr(t) -> int:
 
 def call(name: str, sig: str, *args) -> None:
     """Launch ``ve_<name>`` on the current CUDA stream; raises on a CUDA error code."""
+    call_on(torch.cuda.current_stream().cuda_stream, name, sig, *args)
+
+
+def call_on(stream: int, name: str, sig: str, *args) -> None:
+    """``call`` on a stream of the current device, given by its handle."""
     global launch_count
     fn = _bound.get(name)
     if fn is None:
         fn = _bind(kernels(), "ve_" + name, sig + "p")
         _bound[name] = fn
-    stream = torch.cuda.current_stream().cuda_stream
     rc = fn(*args, stream)
     launch_count += 1
     if rc != 0:

@@ -19,7 +19,7 @@ struct DropoutParams {
   int rows, cols;
   uint32_t groups, div_mul;     // groups of eight columns of a row; i / groups = i * div_mul >> (31 + div_shift) for i < 2^31
   int div_shift;
-  uint32_t threshold;
+  uint32_t threshold;           // t * 65536 (t = 65536 never gets here)
   float scale;
   unsigned long long seed;
   const unsigned long long* seed_at;       // on the device, in place of seed
@@ -59,40 +59,58 @@ VE_DEVINL void load8(const T* p, int n, float* v) {
 
 template <typename T, bool VEC, bool RES>
 __global__ void __launch_bounds__(256) dropout_kernel(const DropoutParams p) {
+  // Groups of a thread whose loads are under way at once: with a residual one (two took 160 us where one takes 153, 16384 x 5120 forward and gradient),
+  // without two: half the bytes.
+  constexpr int N = RES ? 1 : 2;
+  grid_dep_launch();
+  grid_dep_wait();
   const unsigned long long seed = p.seed_at ? *p.seed_at : p.seed;
   const uint2 key = make_uint2((uint32_t)seed, (uint32_t)(seed >> 32));
-  const uint32_t total = (uint32_t)p.rows * p.groups;
-  for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += gridDim.x * blockDim.x) {
-    const uint32_t r = (uint32_t)((unsigned long long)i * p.div_mul >> (31 + p.div_shift)), g = i - r * p.groups;
-    const int c = (int)(g * 8), n = min(8, p.cols - c);
-    float x[8], y[8];
-    load8<T, VEC>((const T*)p.x + (size_t)r * p.ldx + c, n, x);
-    if (RES) load8<T, VEC>((const T*)p.res + (size_t)r * p.ldr + c, n, y);
-    const unsigned long long row = p.row0 + r;
-    const uint4 w4 = philox10(make_uint4(g, (uint32_t)row, (uint32_t)(row >> 32), p.site), key);
-    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+  const uint32_t total = (uint32_t)p.rows * p.groups, step = gridDim.x * blockDim.x;
+  for (uint32_t i0 = blockIdx.x * blockDim.x + threadIdx.x; i0 < total; i0 += N * step) {
+    float x[N][8], y[8];
+    uint32_t r[N], g[N];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t u = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
-      const bool keep = u >= p.threshold;               // (a choice, not a product: what stands in a dropped place does not matter)
-      if (RES) y[e] = keep ? fmaf(x[e], p.scale, y[e]) : y[e];
-      else y[e] = keep ? x[e] * p.scale : 0.f;
+    for (int u = 0; u < N; ++u) {
+      const uint32_t i = u ? min(i0 + u * step, total - 1) : i0;
+      r[u] = (uint32_t)((unsigned long long)i * p.div_mul >> (31 + p.div_shift));
+      g[u] = i - r[u] * p.groups;
+      load8<T, VEC>((const T*)p.x + (size_t)r[u] * p.ldx + g[u] * 8, min(8, p.cols - (int)(g[u] * 8)), x[u]);
     }
-    T* dst = (T*)p.y + (size_t)r * p.cols + c;
-    if (VEC) {
-      if (sizeof(T) == 4) {
-        *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
-        *(reinterpret_cast<float4*>(dst) + 1) = make_float4(y[4], y[5], y[6], y[7]);
-      } else {
-        __nv_bfloat16 b[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) b[e] = f2bf(y[e]);
-        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(b);
+    for (int u = 0; u < N; ++u) {
+      if (u && i0 + u * step >= total) break;
+      const int c = (int)(g[u] * 8), n = min(8, p.cols - c);
+      if (RES) load8<T, VEC>((const T*)p.res + (size_t)r[u] * p.ldr + c, n, y);
+      const unsigned long long row = p.row0 + r[u];
+      const uint4 w4 = philox10(make_uint4(g[u], (uint32_t)row, (uint32_t)(row >> 32), p.site), key);
+      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // 16 bits against t as 32 against t * 65536: a high half needs no extraction
+        const bool keep = (e & 1 ? w[e >> 1] : w[e >> 1] << 16) >= p.threshold;       // (a choice, not a product: what stands in a dropped place does not matter)
+        if (RES) y[e] = keep ? fmaf(x[u][e], p.scale, y[e]) : y[e];
+        else y[e] = keep ? x[u][e] * p.scale : 0.f;
       }
-    } else {
+      T* dst = (T*)p.y + (size_t)r[u] * p.cols + c;
+      if (VEC) {
+        if (sizeof(T) == 4) {
+          *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
+          *(reinterpret_cast<float4*>(dst) + 1) = make_float4(y[4], y[5], y[6], y[7]);
+        } else {
+          uint32_t b[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < n) dst[e] = (T)y[e];
+          for (int e = 0; e < 4; ++e) {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(y[2 * e], y[2 * e + 1]);
+            b[e] = *reinterpret_cast<const uint32_t*>(&v);
+          }
+          *reinterpret_cast<uint4*>(dst) = make_uint4(b[0], b[1], b[2], b[3]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < n) dst[e] = (T)y[e];
+      }
     }
   }
 }
@@ -101,15 +119,15 @@ template <typename T, bool VEC>
 static void launch_dropout(const DropoutParams& p, cudaStream_t st) {
   const uint32_t total = (uint32_t)p.rows * p.groups;
   const int grid = (int)((total + 255) / 256 < 148 * 8 ? (total + 255) / 256 : 148 * 8);
-  if (p.res) dropout_kernel<T, VEC, true><<<grid, 256, 0, st>>>(p);
-  else dropout_kernel<T, VEC, false><<<grid, 256, 0, st>>>(p);
+  if (p.res) launch_pdl(dropout_kernel<T, VEC, true>, dim3(grid), dim3(256), 0, st, p);
+  else launch_pdl(dropout_kernel<T, VEC, false>, dim3(grid), dim3(256), 0, st, p);
 }
 
 template <typename T>
 static int run_dropout(DropoutParams p, long rows, cudaStream_t st) {
   const bool vec = p.cols % 8 == 0 && !((uintptr_t)p.x & 15) && !((uintptr_t)p.y & 15) && p.ldx * sizeof(T) % 16 == 0 &&
                    (!p.res || (!((uintptr_t)p.res & 15) && p.ldr * sizeof(T) % 16 == 0));
-  const long most = 0x7fffffffl / p.groups - 148 * 8 * 256 / (long)p.groups - 1;       // (a step behind the last group stays below 2^31 too)
+  const long most = (0x7fffffffl - 2 * 148 * 8 * 256) / p.groups;       // (two steps behind the last group stay below 2^31 too)
   for (long r = 0; r < rows; r += most) {
     DropoutParams q = p;
     q.rows = (int)(rows - r < most ? rows - r : most);
@@ -134,7 +152,12 @@ int ve_dropout(const void* x, long ldx, const void* residual, long ldr, void* y,
                const void* seed_at, long row0, int site, cudaStream_t st) {
   if (rows <= 0 || cols <= 0) return 0;
   if (threshold < 0 || threshold > 65536) return cudaErrorInvalidValue;
-  DropoutParams p{x, residual, ldx, ldr, y, 0, cols, (uint32_t)((cols + 7l) / 8), 0, 0, (uint32_t)threshold, scale, (unsigned long long)seed,
+  if (threshold == 65536) {              // nothing is kept
+    const size_t row = (size_t)cols * (fp32 ? 4 : 2);
+    return (int)(residual ? cudaMemcpy2DAsync(y, row, residual, (size_t)ldr * (fp32 ? 4 : 2), row, rows, cudaMemcpyDeviceToDevice, st)
+                          : cudaMemsetAsync(y, 0, row * rows, st));
+  }
+  DropoutParams p{x, residual, ldx, ldr, y, 0, cols, (uint32_t)((cols + 7l) / 8), 0, 0, (uint32_t)threshold << 16, scale, (unsigned long long)seed,
                   (const unsigned long long*)seed_at, (unsigned long long)row0, (uint32_t)site};
   while ((1ul << p.div_shift) < p.groups) ++p.div_shift;
   p.div_mul = (uint32_t)(((1ull << (31 + p.div_shift)) + p.groups - 1) / p.groups);

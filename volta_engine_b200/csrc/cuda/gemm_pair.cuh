@@ -126,8 +126,9 @@ static inline PairLoop pair_loop(int sa, int sb, int order, int chunk) {
 // in front of its sums (Row begin(tile, row of the tile, first column)) and takes the sums: finish(tile, row of the tile, first column, Row,
 // sums[128], omap, 4 KB of shared memory of the warp); done() when there are no more.
 // A_MN / B_MN: the operand is MN-major.
-template <bool A_MN, bool B_MN, class Job>
-VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap* amap, const CUtensorMap* bmap, const CUtensorMap* omap, int* status) {
+// wait(): the point behind which other kernels' results are read.
+template <bool A_MN, bool B_MN, class Job, class Wait>
+VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap* amap, const CUtensorMap* bmap, const CUtensorMap* omap, int* status, Wait wait) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
@@ -147,6 +148,7 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
   cluster_sync_all();                       // the pair's barriers stand before either CTA signals them
   tc_fence_after();
   const uint32_t tmem_base = tmem_holder;
+  wait();
   const int ntiles = job.tiles();
 
   if (warp < 4) {

@@ -27,7 +27,9 @@
 namespace ve {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLogFloor = -27.631021115928547f;       // log 1e-12: the least share of "any other token"
 constexpr int kMaxTopk = 1024;
+constexpr int kFrontRows = 4096;       // rows that every block of head_front_kernel looks through
 
 VE_DEVINL float neg_inf() { return __int_as_float(0xff800000); }
 
@@ -41,18 +43,28 @@ struct HeadRows {
 };
 
 // Divergence: the teacher's tokens of a row in ascending order, with their places: sid / slp [R, K] (padding behind, as INT_MAX), and at
-// off[r, b] the first one at or behind column 128 b. One block a row, counting ranks: K is small.
-__global__ void __launch_bounds__(128) head_targets_kernel(const HeadRows p, int nblk, int* sid, float* slp, uint16_t* off, int* flag) {
+// off[r, b] the first one at or behind column 128 b; flag[r]: the row counts; mass[r] = sum_k a_k. One block a row, counting ranks: K is small.
+__global__ void __launch_bounds__(128) head_targets_kernel(const HeadRows p, int nblk, int* sid, float* slp, uint16_t* off, int* flag, double* mass) {
   __shared__ int id[kMaxTopk], srt[kMaxTopk];
+  __shared__ double part[4];
+  grid_dep_launch();
+  grid_dep_wait();
   const int r = blockIdx.x;
   int any = 0;
+  double sum = 0.0;
   for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
     const int v = p.ids[(size_t)r * p.K + k];
     id[k] = v < 0 ? INT_MAX : v;
     any |= v >= 0;
+    if (v >= 0) sum += exp((double)p.logp[(size_t)r * p.K + k]);
   }
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
   any = __syncthreads_or(any);
-  if (threadIdx.x == 0) flag[r] = any;
+  if (threadIdx.x == 0) {
+    flag[r] = any;
+    mass[r] = part[0] + part[1] + part[2] + part[3];
+  }
   if (!any) return;                                   // (uniform)
   for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
     const int v = id[k];
@@ -80,6 +92,8 @@ VE_DEVINL long label_of(const HeadRows& p, int r) {
 // The rows that count, in order: live[i] = row, pos[row] = i or -1, *count.
 __global__ void __launch_bounds__(1024) head_rows_kernel(const HeadRows p, const int* flag, int* live, int* pos, int* count) {
   __shared__ int part[32], base;
+  grid_dep_launch();
+  grid_dep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) base = 0;
   __syncthreads();
@@ -101,31 +115,70 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(const HeadRows p, const
   if (threadIdx.x == 0) *count = base;
 }
 
-VE_DEVINL float split_bf16(float v, __nv_bfloat16& out) {     // rounds v, returns what is left of it
-  out = f2bf(v);
-  return v - bf2f(out);
-}
-
-// Four values into the slabs of a row (an infinity or a NaN leaves NaN in the slabs behind the first).
-VE_DEVINL void store_slabs4(__nv_bfloat16* dst, size_t slab, int slabs, float4 v) {
-  for (int s = 0; s < slabs; ++s) {
-    __nv_bfloat16 b[4];
-    v.x = split_bf16(v.x, b[0]); v.y = split_bf16(v.y, b[1]); v.z = split_bf16(v.z, b[2]); v.w = split_bf16(v.w, b[3]);
-    *reinterpret_cast<uint2*>(dst + s * slab) = *reinterpret_cast<const uint2*>(b);
-  }
-}
-
+// Eight values of a row from column c; zeros behind column H. `vec`: whole groups may be read as 16-byte words.
 template <typename T>
-VE_DEVINL float4 load4(const T* row, int c, int H, bool vec) {
-  if (vec && c + 4 <= H) {
-    if (sizeof(T) == 4) return *reinterpret_cast<const float4*>(row + c);
-    const uint2 w = *reinterpret_cast<const uint2*>(row + c);
-    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-  }
-  float f[4];
+VE_DEVINL void load8(const T* row, int c, int H, bool vec, float* v) {
+  if (sizeof(T) == 4) {
+    if (vec && c + 8 <= H) {
+      const float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      return;
+    }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) f[e] = c + e < H ? (float)row[c + e] : 0.f;
-  return make_float4(f[0], f[1], f[2], f[3]);
+    for (int e = 0; e < 8; ++e) v[e] = c + e < H ? (float)row[c + e] : 0.f;
+    return;
+  }
+  uint32_t w[4];
+  if (vec && c + 8 <= H) {
+    const uint4 a = *reinterpret_cast<const uint4*>(row + c);
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+  } else if (c + 8 <= H) {
+    // a row that starts between 4-byte words: five words around its first and last value, which are inside the row's ends or beside them in their words
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row + c);
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+    if (at & 2) {
+      uint32_t x[5];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = q[e];
+      x[4] = *reinterpret_cast<const unsigned short*>(q + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = __funnelshift_r(x[e], x[e + 1], 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = q[e];
+    }
+  } else {
+    const unsigned short* s = reinterpret_cast<const unsigned short*>(row);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = (c + 2 * e < H ? s[c + 2 * e] : 0u) | (c + 2 * e + 1 < H ? (uint32_t)s[c + 2 * e + 1] << 16 : 0u);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) { v[2 * e] = __uint_as_float(w[e] << 16); v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+}
+
+// Pairs of values to bf16, the values become what the rounding left (an infinity or a NaN leaves NaN).
+VE_DEVINL uint32_t split_pair(float& lo, float& hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  const uint32_t b = *reinterpret_cast<const uint32_t*>(&v);
+  lo -= __uint_as_float(b << 16);
+  hi -= __uint_as_float(b & 0xffff0000u);
+  return b;
+}
+
+// A row (null: zeros) into its slabs, by a warp.
+template <typename T>
+VE_DEVINL void pack_row(const T* row, int H, int Hp, int slabs, size_t slab, __nv_bfloat16* dst) {
+  const bool vec = !(reinterpret_cast<uintptr_t>(row) & 15);
+  for (int c = (threadIdx.x & 31) * 8; c < Hp; c += 256) {
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (row) load8(row, c, H, vec, v);
+    for (int s = 0; s < slabs; ++s) {
+      uint32_t b[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] = split_pair(v[2 * e], v[2 * e + 1]);
+      *reinterpret_cast<uint4*>(dst + s * slab + c) = make_uint4(b[0], b[1], b[2], b[3]);
+    }
+  }
 }
 
 // Rows of a matrix as bf16 slabs [slabs][rows of a slab][Hp], zeros behind column H. With `live`: the gathered rows, and zeros behind the last
@@ -133,15 +186,48 @@ VE_DEVINL float4 load4(const T* row, int c, int H, bool vec) {
 template <typename T>
 __global__ void __launch_bounds__(256) head_pack_kernel(const T* src, long ld, const int* live, const int* count, int rows, int H, int Hp, int slabs,
                                                         size_t slab, __nv_bfloat16* dst) {
-  const bool vec = !((uintptr_t)src & (4 * sizeof(T) - 1)) && ld % 4 == 0;
+  grid_dep_launch();
+  grid_dep_wait();
   const int n = live ? *count : rows, all = live ? (n + 255) / 256 * 256 : rows;
-  const int per = Hp / 4;
-  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < (size_t)all * per; i += (size_t)gridDim.x * blockDim.x) {
-    const int r = (int)(i / per), c = (int)(i - (size_t)r * per) * 4;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < n) v = load4(src + (live ? live[r] : r) * ld, c, H, vec);
-    store_slabs4(dst + (size_t)r * Hp + c, slab, slabs, v);
+  for (int r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; r < all; r += gridDim.x * blockDim.x >> 5)
+    pack_row(r < n ? src + (live ? live[r] : r) * ld : (const T*)nullptr, H, Hp, slabs, slab, dst + (size_t)r * Hp);
+}
+
+// head_rows_kernel and head_pack_kernel of few rows in one launch: every block finds all the rows that count and packs its share of them; the words of
+// large blocks become zero on the way.
+template <typename T>
+__global__ void __launch_bounds__(256) head_front_kernel(const HeadRows p, const int* flag, int* live, int* pos, int* count, const T* src, long ld, int H, int Hp,
+                                                         int slabs, size_t slab, __nv_bfloat16* dst, uint4* words, size_t nwords) {
+  __shared__ int row_of[kFrontRows], part[8];
+  grid_dep_launch();
+  grid_dep_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const size_t first = blockIdx.x * (size_t)blockDim.x + threadIdx.x, step = (size_t)gridDim.x * blockDim.x;
+  for (size_t i = first; i < nwords; i += step) words[i] = make_uint4(0u, 0u, 0u, 0u);
+  int n = 0;
+  for (int r0 = 0; r0 < p.R; r0 += 256) {
+    const int r = r0 + threadIdx.x;
+    const bool on = r < p.R && (p.labels ? label_of(p, r) >= 0 : flag[r] != 0);
+    const unsigned mask = __ballot_sync(0xffffffffu, on);
+    if (lane == 0) part[warp] = __popc(mask);
+    __syncthreads();
+    int at = n + __popc(mask & ((1u << lane) - 1));
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      if (w < warp) at += part[w];
+      n += part[w];
+    }
+    if (on) row_of[at] = r;
+    if (blockIdx.x == 0) {
+      if (r < p.R) pos[r] = on ? at : -1;
+      if (on) live[at] = r;
+    }
+    __syncthreads();
   }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *count = n;
+  const int all = (n + 255) / 256 * 256;
+  for (int r = (int)(first >> 5); r < all; r += (int)(step >> 5))
+    pack_row(r < n ? src + row_of[r] * ld : (const T*)nullptr, H, Hp, slabs, slab, dst + (size_t)r * Hp);
 }
 
 // ------------------------------------------------------------------------------------------------ jobs of the paired GEMM
@@ -190,11 +276,15 @@ struct LogitTiles {           // rows x a piece of the vocabulary: tiles of up t
   }
 };
 
+VE_DEVINL float over_cap(float z, float cap, float inv_cap) {          // z / cap to rounding: the quotient with the rounded 1 / cap, and its rest
+  const float q = z * inv_cap;
+  return fmaf(fmaf(-q, cap, z), inv_cap, q);
+}
 template <bool CAP>
 VE_DEVINL void cap_logits(float* z, float cap, float inv_cap) {
   if (CAP) {
 #pragma unroll
-    for (int j = 0; j < 128; ++j) z[j] = cap * tanhf(z[j] * inv_cap);
+    for (int j = 0; j < 128; ++j) z[j] = cap * tanhf(over_cap(z[j], cap, inv_cap));
   }
 }
 
@@ -258,6 +348,32 @@ struct RowGrad {
   float large;                // dz above this is multiplied with its rounding error too
 };
 
+struct RowInputs {            // by row of the caller
+  const float *stats, *dloss, *tail;
+  const double* mass;
+  int R;
+  bool labels;
+  VE_DEVINL RowGrad at(int row) const {
+    const float lse = stats[row], rest = stats[R + row], g = dloss[row];
+    RowGrad c;
+    // exp(z - lse) as 2^(z log2e - lse2): what the product lse log2e loses to rounding goes into the factors
+    c.lse2 = lse * kLog2e;
+    const float fix = exp2f(-fmaf(lse, kLog2e, -c.lse2));
+    c.g = g;
+    if (labels) {
+      c.dense = g * fix;
+      c.at = -g * expf(rest - lse);
+      c.large = fabsf(c.at) * (1.f / 16.f);
+    } else {
+      const double a = mass[row], lr = (double)rest - (double)lse, t = lr >= (double)kLogFloor ? exp((double)tail[row]) : 0.0;
+      c.at = (float)((double)g * (a + t)) * fix;
+      c.dense = (float)((double)g * (t > 0.0 ? a + t - t * exp(-lr) : a)) * fix;       // (a difference: in 64 bits)
+      c.large = fabsf(g) * (1.f / 1024.f);
+    }
+    return c;
+  }
+};
+
 // Blocks of 64 x 64 of a piece's dz with large elements: by tiles of 256 rows, bits over the columns' blocks (dx), and by tiles of 256 columns,
 // bits over the rows' blocks (dhead).
 struct LargeBlocks {
@@ -269,7 +385,7 @@ template <bool CAP>
 struct GradJob : LogitTiles {
   Targets tg;
   const int* live;
-  const RowGrad* rg;          // by gathered row
+  RowInputs in;
   int slabs;                  // of dz
   LargeBlocks big;            // (null: every slab counts everywhere)
   float cap, inv_cap;
@@ -277,7 +393,7 @@ struct GradJob : LogitTiles {
   struct Row : LogitTiles::Row { RowGrad c; };
   VE_DEVINL Row begin(const PairTile& t, int r, int c0) const {
     Row w{row_at(t, r, c0, live, tg), {0.f, 0.f, 0.f, 0.f, 0.f}};
-    if (w.row >= 0) w.c = rg[t.m0 + r];
+    if (w.row >= 0) w.c = in.at(w.row);
     return w;
   }
 
@@ -296,7 +412,7 @@ struct GradJob : LogitTiles {
       if (p < end) {
         float slope = 1.f;
         if (CAP) {
-          const float th = tanhf(v * inv_cap);
+          const float th = tanhf(over_cap(v, cap, inv_cap));
           v = cap * th;
           slope = 1.f - th * th;
         }
@@ -319,7 +435,7 @@ struct GradJob : LogitTiles {
     for (int j = 0; j < 128; ++j) {
       float f = c.dense, v = z[j];
       if (CAP) {
-        const float th = tanhf(v * inv_cap);
+        const float th = tanhf(over_cap(v, cap, inv_cap));
         v = cap * th;
         f *= 1.f - th * th;
       }
@@ -355,13 +471,7 @@ struct GradJob : LogitTiles {
         for (int j = 0; j < 64; j += 8) {
           uint32_t b[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float &lo = z[64 * h + j + 2 * e], &hi = z[64 * h + j + 2 * e + 1];
-            const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-            b[e] = *reinterpret_cast<const uint32_t*>(&v);
-            lo -= __uint_as_float(b[e] << 16);
-            hi -= __uint_as_float(b[e] & 0xffff0000u);
-          }
+          for (int e = 0; e < 4; ++e) b[e] = split_pair(z[64 * h + j + 2 * e], z[64 * h + j + 2 * e + 1]);
           *reinterpret_cast<uint4*>(staging + lane * 128 + (((j >> 3) ^ (lane & 7)) << 4)) = make_uint4(b[0], b[1], b[2], b[3]);
         }
         fence_proxy_async_smem();
@@ -425,29 +535,41 @@ struct DheadJob {
     return PairTile{i / nn * 256, i % nn * 256, 0, (*count + 63) >> 6, 0};
   }
   VE_DEVINL void finish(const PairTile& t, int r, int c0, const Row& w, float* z, const CUtensorMap* omap, uint8_t* staging) const {
-    const int v = t.m0 + r;
-    if (v >= nv) return;
-    T* dst = out + (size_t)v * H + t.n0 + c0;
-    const int cols = H - t.n0 - c0;
+    const int v = t.m0 + r, cols = H - t.n0 - c0;
+    if (cols <= 0 || t.m0 + (r & ~31) >= nv) return;
     const bool vec = !((uintptr_t)out & 15) && H % (16 / (int)sizeof(T)) == 0;
+    if (vec) {
+      if (v >= nv) return;
+      T* dst = out + (size_t)v * H + t.n0 + c0;
 #pragma unroll
-    for (int j = 0; j < 128; j += 8) {
-      if (j >= cols) continue;
-      if (vec && j + 8 <= cols) {
+      for (int j = 0; j < 128; j += 8) {
+        if (j >= cols) continue;                    // (whole groups: the width is a multiple of them, of fp32 values of four)
         if (sizeof(T) == 4) {
           *reinterpret_cast<float4*>(dst + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
-          *reinterpret_cast<float4*>(dst + j + 4) = make_float4(z[j + 4], z[j + 5], z[j + 6], z[j + 7]);
+          if (j + 4 < cols) *reinterpret_cast<float4*>(dst + j + 4) = make_float4(z[j + 4], z[j + 5], z[j + 6], z[j + 7]);
         } else {
-          __nv_bfloat16 b[8];
+          uint32_t b[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) b[e] = f2bf(z[j + e]);
-          *reinterpret_cast<uint4*>(dst + j) = *reinterpret_cast<const uint4*>(b);
+          for (int e = 0; e < 4; ++e) b[e] = split_pair(z[j + 2 * e], z[j + 2 * e + 1]);
+          *reinterpret_cast<uint4*>(dst + j) = make_uint4(b[0], b[1], b[2], b[3]);
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (j + e < cols) dst[j + e] = (T)z[j + e];
       }
+      return;
+    }
+    // rows off 16-byte boundaries: 32 x 32 values at a time through shared memory, so that a warp writes along a row (a thread along its own: 45 us
+    // where this takes 14, 5003 x 515)
+    const int lane = threadIdx.x & 31;
+    float* st = reinterpret_cast<float*>(staging);
+    const int v0 = t.m0 + (r & ~31);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) st[lane * 32 + (j ^ lane)] = z[32 * g + j];
+      __syncwarp();
+      const int c = 32 * g + lane;
+      if (c < cols)
+        for (int k = 0; k < 32 && v0 + k < nv; ++k) out[(size_t)(v0 + k) * H + t.n0 + c0 + c] = (T)st[k * 32 + (lane ^ k)];
+      __syncwarp();
     }
   }
 };
@@ -456,16 +578,21 @@ template <bool A_MN, bool B_MN, class Job>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 head_gemm_kernel(const Job job, const PairLoop loop, const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                  const __grid_constant__ CUtensorMap omap, int* status) {
-  pair_gemm<A_MN, B_MN>(job, loop, &amap, &bmap, &omap, status);
+  grid_dep_launch();
+  pair_gemm<A_MN, B_MN>(job, loop, &amap, &bmap, &omap, status, [] { grid_dep_wait(); });
 }
 
 // ------------------------------------------------------------------------------------------------ the rows' sums
 // Joins a row's blocks and computes its loss, 32 rows a block of 1024 threads: the warps share the blocks of columns, lanes are rows; then a
 // warp takes a row's targets. The few numbers behind the sums are in 64 bits: losses near zero, and divergences of near models, are differences.
-__global__ void __launch_bounds__(1024) head_merge_kernel(const HeadRows p, const int* live, const int* count, int rows_cap, int nblk, const float2* part,
-                                                          const float* zt, const int* sid, const float* slp, float* loss, float* stats) {
+__global__ void __launch_bounds__(1024) head_merge_kernel(const HeadRows p, const int* live, const int* pos, const int* count, int rows_cap, int nblk,
+                                                          const float2* part, const float* zt, const int* sid, const float* slp, float* loss, float* stats) {
   __shared__ float sm[32][33], ss[32][33];
+  grid_dep_launch();
+  grid_dep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = *count;
+  const int r = blockIdx.x * 32 + lane;
+  if (warp == 0 && r < p.R && pos[r] < 0) loss[r] = stats[r] = stats[p.R + r] = 0.f;          // left out
   if (blockIdx.x * 32 >= n) return;
   const int i = blockIdx.x * 32 + lane;
   float m = neg_inf(), s = 0.f;
@@ -531,7 +658,7 @@ __global__ void __launch_bounds__(1024) head_merge_kernel(const HeadRows p, cons
       if (id[k] < p.V && lp[k] != neg_inf()) out += exp((double)lp[k]) * ((double)lp[k] - ((double)z[k] - lse));
     for (int o = 16; o > 0; o >>= 1) out += __shfl_xor_sync(0xffffffffu, out, o);
     const float lt = p.tail[row];
-    if (lt != neg_inf()) out += exp((double)lt) * ((double)lt - fmax(rest - lse, -27.631021115928547));     // log 1e-12
+    if (lt != neg_inf()) out += exp((double)lt) * ((double)lt - fmax(rest - lse, (double)kLogFloor));
     if (__any_sync(0xffffffffu, bad)) out = lse = __longlong_as_double(0x7ff8000000000000ll);
   }
   if (lane == 0) {
@@ -541,44 +668,11 @@ __global__ void __launch_bounds__(1024) head_merge_kernel(const HeadRows p, cons
   }
 }
 
-// Rows that are left out: zeros.
-__global__ void __launch_bounds__(256) head_blank_kernel(const int* pos, int R, float* loss, float* stats) {
-  const int r = blockIdx.x * blockDim.x + threadIdx.x;
-  if (r < R && pos[r] < 0) loss[r] = stats[r] = stats[R + r] = 0.f;
-}
-
-// The rows' constants of dz, a warp a row.
-__global__ void __launch_bounds__(256) head_rowgrad_kernel(const HeadRows p, const int* live, const int* count, const float* stats, const float* slp,
-                                                           const float* dloss, RowGrad* rg) {
-  const int i = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
-  if (i >= *count) return;
-  const int row = live[i];
-  const float lse = stats[row], rest = stats[p.R + row], g = dloss[row];
-  RowGrad c;
-  // exp(z - lse) as 2^(z log2e - lse2): what the product lse log2e loses to rounding goes into the factors
-  c.lse2 = lse * kLog2e;
-  const float fix = exp2f(-fmaf(lse, kLog2e, -c.lse2));
-  c.g = g;
-  if (p.labels) {
-    c.dense = g * fix;
-    c.at = -g * expf(rest - lse);
-    c.large = fabsf(c.at) * (1.f / 16.f);
-  } else {
-    double a = 0.0;
-    for (int k = lane; k < p.K; k += 32) a += exp((double)slp[(size_t)row * p.K + k]);      // (padding: exp(-inf) = 0)
-    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-    const double t = exp((double)p.tail[row]), lr = (double)rest - (double)lse;
-    const bool above = lr >= -27.631021115928547;
-    c.at = (float)(g * (a + (above ? t : 0.0))) * fix;
-    c.dense = (float)(g * (a + (above ? t - t * exp(-lr) : 0.0))) * fix;
-    c.large = fabsf(g) * (1.f / 1024.f);
-  }
-  if (lane == 0) rg[i] = c;
-}
-
 // dx of the caller's rows from the ranges' sums; zeros where a row was left out.
 template <typename T>
 __global__ void __launch_bounds__(256) head_dx_kernel(const int* pos, int R, int H, int Hp, int splits, size_t slab, const float* acc, T* dx) {
+  grid_dep_launch();
+  grid_dep_wait();
   const int per = (H + 3) / 4;
   const bool vec = !((uintptr_t)dx & 15) && H % 4 == 0;
   for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < (size_t)R * per; i += (size_t)gridDim.x * blockDim.x) {
@@ -613,7 +707,7 @@ struct HeadPlan {             // sizes and places in the workspace
   int piece;                  // vocabulary rows at a time
   int splits;                 // ranges of a piece that dx is summed over
   int row_words, col_words;   // of LargeBlocks
-  size_t live, pos, count, flag, sid, slp, off, x, part, zt, rg, head, G, acc, big, big_bytes, bytes;
+  size_t live, pos, count, flag, mass, sid, slp, off, x, part, zt, head, G, acc, big, big_bytes, bytes;      // (big_bytes: of a piece)
 };
 
 static inline int blocks_of(size_t n, int per = 256) {
@@ -649,20 +743,19 @@ static HeadPlan head_plan(bool grads, bool want_dx, int x_fp32, int head_fp32, b
   size_t at = 0;
   auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
   p.live = take(4ull * R); p.pos = take(4ull * R); p.count = take(4);
-  p.flag = p.sid = p.slp = p.off = 0;
-  if (kl) { p.flag = take(4ull * R); p.sid = take(4ull * R * K); p.slp = take(4ull * R * K); p.off = take(2ull * R * (p.nblk + 1)); }
+  p.flag = p.mass = p.sid = p.slp = p.off = 0;
+  if (kl) { p.flag = take(4ull * R); p.mass = take(8ull * R); p.sid = take(4ull * R * K); p.slp = take(4ull * R * K); p.off = take(2ull * R * (p.nblk + 1)); }
   p.x = take(2ull * p.sx * p.rows_cap * p.Hp);
   p.head = pack_head ? take(2ull * p.sw * p.piece * p.Hp) : 0;
-  p.part = p.zt = p.rg = p.G = p.acc = p.big = p.big_bytes = 0;
+  p.part = p.zt = p.G = p.acc = p.big = p.big_bytes = 0;
   p.row_words = p.col_words = 0;
   if (!grads) { p.part = take(8ull * p.nblk * p.rows_cap); p.zt = take(4ull * R * (kl ? K : 1)); }
   else {
-    p.rg = take(sizeof(RowGrad) * (size_t)p.rows_cap);
     p.G = take(2ull * p.sg * p.rows_cap * p.piece);
     p.row_words = (p.piece / 64 + 31) / 32;
     p.col_words = (p.rows_cap / 64 + 31) / 32;
-    p.big_bytes = p.sg == 2 ? 4ull * (p.rows_cap / 256 * p.row_words + p.piece / 256 * p.col_words) : 0;
-    p.big = take(p.big_bytes);
+    p.big_bytes = p.sg == 2 ? (4ull * (p.rows_cap / 256 * p.row_words + p.piece / 256 * p.col_words) + 15) / 16 * 16 : 0;
+    p.big = take(p.big_bytes * (((size_t)V + p.piece - 1) / p.piece));
     if (want_dx) p.acc = take(4ull * p.splits * p.rows_cap * p.Hp);
   }
   p.bytes = at;
@@ -691,24 +784,41 @@ template <bool A_MN, bool B_MN, class Job>
 static int launch_pair(const Job& job, const PairLoop& loop, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const HeadCall& c) {
   cudaError_t e = allow_smem<head_gemm_kernel<A_MN, B_MN, Job>>(kPairSmem);
   if (e != cudaSuccess) return (int)e;
-  head_gemm_kernel<A_MN, B_MN, Job><<<2 * kPairClusters, kPairThreads, kPairSmem, c.st>>>(job, loop, a, b, o, c.status);
+  launch_pdl(head_gemm_kernel<A_MN, B_MN, Job>, dim3(2 * kPairClusters), dim3(kPairThreads), kPairSmem, c.st, job, loop, a, b, o, c.status);
   return (int)cudaGetLastError();
 }
 
 template <typename T>
 static void pack_rows(const void* src, long ld, const int* live, const int* count, int rows, const HeadCall& c, const HeadPlan& p, int slabs, size_t slab, void* dst) {
-  head_pack_kernel<T><<<blocks_of((size_t)rows * p.Hp / 4), 256, 0, c.st>>>((const T*)src, ld, live, count, rows, c.H, p.Hp, slabs, slab, (__nv_bfloat16*)dst);
+  launch_pdl(head_pack_kernel<T>, dim3(blocks_of((size_t)rows, 8)), dim3(256), 0, c.st, (const T*)src, ld, live, count, rows, c.H, p.Hp, slabs, slab,
+             (__nv_bfloat16*)dst);
 }
 
-// The rows that count, their targets and their states.
-static void head_front(const HeadCall& c, const HeadPlan& p) {
+template <typename T>
+static int front_rows(const HeadCall& c, const HeadPlan& p, size_t word_bytes) {
   int *live = (int*)(c.ws + p.live), *pos = (int*)(c.ws + p.pos), *count = (int*)(c.ws + p.count), *flag = (int*)(c.ws + p.flag);
-  if (!c.rows.labels)
-    head_targets_kernel<<<c.rows.R, 128, 0, c.st>>>(c.rows, p.nblk, (int*)(c.ws + p.sid), (float*)(c.ws + p.slp), (uint16_t*)(c.ws + p.off), flag);
-  head_rows_kernel<<<1, 1024, 0, c.st>>>(c.rows, flag, live, pos, count);
   const size_t slab = (size_t)p.rows_cap * p.Hp;
-  if (c.x_fp32) pack_rows<float>(c.x, c.ldx, live, count, p.rows_cap, c, p, p.sx, slab, c.ws + p.x);
-  else pack_rows<__nv_bfloat16>(c.x, c.ldx, live, count, p.rows_cap, c, p, p.sx, slab, c.ws + p.x);
+  if (c.rows.R <= kFrontRows) {
+    launch_pdl(head_front_kernel<T>, dim3(blocks_of((size_t)p.rows_cap, 8)), dim3(256), 0, c.st, c.rows, (const int*)flag, live, pos, count,
+               (const T*)c.x, c.ldx, c.H, p.Hp, p.sx, slab, (__nv_bfloat16*)(c.ws + p.x), (uint4*)(c.ws + p.big), word_bytes / 16);
+    return 0;
+  }
+  if (word_bytes) {
+    const cudaError_t e = cudaMemsetAsync(c.ws + p.big, 0, word_bytes, c.st);
+    if (e != cudaSuccess) return (int)e;
+  }
+  launch_pdl(head_rows_kernel, dim3(1), dim3(1024), 0, c.st, c.rows, (const int*)flag, live, pos, count);
+  pack_rows<T>(c.x, c.ldx, live, count, p.rows_cap, c, p, p.sx, slab, c.ws + p.x);
+  return 0;
+}
+
+// The rows that count, their targets and their states; zeros in the words of large blocks.
+static int head_front(const HeadCall& c, const HeadPlan& p) {
+  const size_t word_bytes = p.big_bytes * (((size_t)c.rows.V + p.piece - 1) / p.piece);
+  if (!c.rows.labels)
+    launch_pdl(head_targets_kernel, dim3(c.rows.R), dim3(128), 0, c.st, c.rows, p.nblk, (int*)(c.ws + p.sid), (float*)(c.ws + p.slp), (uint16_t*)(c.ws + p.off),
+               (int*)(c.ws + p.flag), (double*)(c.ws + p.mass));
+  return c.x_fp32 ? front_rows<float>(c, p, word_bytes) : front_rows<__nv_bfloat16>(c, p, word_bytes);
 }
 
 // The head's rows [v0, v0 + nv) as an operand: in place, or packed.
@@ -727,15 +837,19 @@ static Targets head_targets_of(const HeadCall& c, const HeadPlan& p) {
                  c.rows.labels ? 1 : c.rows.K, p.nblk};
 }
 
-constexpr int kExactChunk = 4;         // steps of 64 between fp32 additions where 32 bits are asked for
+// Steps of 64 between fp32 additions where 32 bits are asked for. Cut-off sums over a step are 5e-8 too small; this keeps that below what fp32 additions
+// along H round by (H = 128 7e-8, 1024 2.5e-7, 5120 7e-7). Shorter pieces wait for their additions: of one step 15 to 50 %, of two up to 6 %.
+static inline int exact_chunk(int H) { return H <= 256 ? 1 : H <= 1280 ? 2 : 4; }
+constexpr int kExactChunk = 4;         // along rows or the vocabulary: gradients in fp32
 constexpr int kRoundedChunk = 32;      // where the result is rounded to bf16 (cut-off sums over 2048: 2e-6), or a gradient's logits are (2e-6 of z: 2^-15 of s)
 
 template <bool CAP>
 static int head_score(const HeadCall& c, const HeadPlan& p, float* loss, float* stats) {
-  head_front(c, p);
+  int rc = head_front(c, p);
+  if (rc) return rc;
   const int *live = (const int*)(c.ws + p.live), *pos = (const int*)(c.ws + p.pos), *count = (const int*)(c.ws + p.count);
   CUtensorMap xm, wm;
-  int rc = slab_map(&xm, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, 128);
+  rc = slab_map(&xm, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, 128);
   if (rc) return rc;
   ScoreJob<CAP> job;
   job.count = count; job.ksteps = p.ksteps; job.tg = head_targets_of(c, p); job.live = live; job.rows_cap = p.rows_cap;
@@ -744,45 +858,44 @@ static int head_score(const HeadCall& c, const HeadPlan& p, float* loss, float* 
     job.v0 = v0;
     job.nv = c.rows.V - v0 < p.piece ? c.rows.V - v0 : p.piece;
     if ((rc = head_rows_map(&wm, c, p, v0, job.nv, 128, true))) return rc;
-    if ((rc = launch_pair<false, false>(job, pair_loop(p.sx, p.sw, 2, kExactChunk), xm, wm, xm, c))) return rc;
+    if ((rc = launch_pair<false, false>(job, pair_loop(p.sx, p.sw, 2, exact_chunk(c.H)), xm, wm, xm, c))) return rc;
   }
-  head_merge_kernel<<<(c.rows.R + 31) / 32, 1024, 0, c.st>>>(c.rows, live, count, p.rows_cap, p.nblk, job.part, job.zt, job.tg.sid, job.tg.slp, loss, stats);
-  head_blank_kernel<<<(c.rows.R + 255) / 256, 256, 0, c.st>>>(pos, c.rows.R, loss, stats);
+  launch_pdl(head_merge_kernel, dim3((c.rows.R + 31) / 32), dim3(1024), 0, c.st, c.rows, live, pos, count, p.rows_cap, p.nblk, (const float2*)job.part,
+             (const float*)job.zt, job.tg.sid, job.tg.slp, loss, stats);
   return (int)cudaGetLastError();
 }
 
 template <bool CAP>
 static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, const float* dloss, void* dx, void* dhead) {
-  head_front(c, p);
+  int rc = head_front(c, p);
+  if (rc) return rc;
   const int *live = (const int*)(c.ws + p.live), *pos = (const int*)(c.ws + p.pos), *count = (const int*)(c.ws + p.count);
   const int R = c.rows.R, H = c.H;
-  RowGrad* rg = (RowGrad*)(c.ws + p.rg);
-  head_rowgrad_kernel<<<(R + 7) / 8, 256, 0, c.st>>>(c.rows, live, count, stats, (const float*)(c.ws + p.slp), dloss, rg);
   CUtensorMap xk, xmn, wk, wmn, gk, gmn, gout;
-  int rc = slab_map(&xk, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, 128);
+  rc = slab_map(&xk, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, 128);
   if (!rc) rc = slab_map(&xmn, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, 64);
   if (!rc) rc = slab_map(&gk, c.ws + p.G, p.sg, p.rows_cap, p.rows_cap, p.piece, p.piece, 128);
   if (!rc) rc = slab_map(&gmn, c.ws + p.G, p.sg, p.rows_cap, p.rows_cap, p.piece, p.piece, 64);
   if (!rc) rc = slab_map(&gout, c.ws + p.G, p.sg, p.rows_cap, p.rows_cap, p.piece, p.piece, 32);
   if (rc) return rc;
   GradJob<CAP> gj;
-  gj.count = count; gj.ksteps = p.ksteps; gj.tg = head_targets_of(c, p); gj.live = live; gj.rg = rg;
+  gj.count = count; gj.ksteps = p.ksteps; gj.tg = head_targets_of(c, p); gj.live = live; 
   gj.slabs = p.sg; gj.cap = c.softcap; gj.inv_cap = CAP ? 1.f / c.softcap : 0.f;
-  uint32_t* const words = (uint32_t*)(c.ws + p.big);
-  const LargeBlocks big{p.big_bytes ? words : nullptr, p.big_bytes ? words + p.rows_cap / 256 * p.row_words : nullptr, p.row_words, p.col_words};
-  gj.big = big;
-  DxJob xj{count, H, p.Hp, 0, p.splits, 1, (size_t)p.rows_cap * p.Hp, (float*)(c.ws + p.acc), big};
+  gj.in = RowInputs{stats, dloss, c.rows.tail, (const double*)(c.ws + p.mass), R, c.rows.labels != nullptr};
+  DxJob xj{count, H, p.Hp, 0, p.splits, 1, (size_t)p.rows_cap * p.Hp, (float*)(c.ws + p.acc), {}};
   const bool exact = p.sg == 3;
   for (int v0 = 0; v0 < c.rows.V; v0 += p.piece) {
     const int nv = c.rows.V - v0 < p.piece ? c.rows.V - v0 : p.piece;
     gj.v0 = v0;
     gj.nv = nv;
     if ((rc = head_rows_map(&wk, c, p, v0, nv, 128, true))) return rc;
+    LargeBlocks big{nullptr, nullptr, p.row_words, p.col_words};
     if (p.big_bytes) {
-      const cudaError_t e = cudaMemsetAsync(words, 0, p.big_bytes, c.st);
-      if (e != cudaSuccess) return (int)e;
+      big.of_rows = (uint32_t*)(c.ws + p.big + p.big_bytes * (v0 / p.piece));
+      big.of_cols = big.of_rows + p.rows_cap / 256 * p.row_words;
     }
-    if ((rc = launch_pair<false, false>(gj, pair_loop(p.sx, p.sw, 2, exact ? kExactChunk : kRoundedChunk), xk, wk, gout, c))) return rc;
+    gj.big = xj.big = big;
+    if ((rc = launch_pair<false, false>(gj, pair_loop(p.sx, p.sw, 2, exact ? exact_chunk(c.H) : kRoundedChunk), xk, wk, gout, c))) return rc;
     if (dx) {
       if ((rc = head_rows_map(&wmn, c, p, v0, nv, 64, false))) return rc;
       xj.ksteps = (nv + 63) / 64;
@@ -803,8 +916,8 @@ static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, c
   }
   if (dx) {
     const int grid = blocks_of((size_t)R * p.Hp / 4);
-    if (c.x_fp32) head_dx_kernel<float><<<grid, 256, 0, c.st>>>(pos, R, H, p.Hp, p.splits, xj.slab, xj.acc, (float*)dx);
-    else head_dx_kernel<__nv_bfloat16><<<grid, 256, 0, c.st>>>(pos, R, H, p.Hp, p.splits, xj.slab, xj.acc, (__nv_bfloat16*)dx);
+    if (c.x_fp32) launch_pdl(head_dx_kernel<float>, dim3(grid), dim3(256), 0, c.st, pos, R, H, p.Hp, p.splits, xj.slab, (const float*)xj.acc, (float*)dx);
+    else launch_pdl(head_dx_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, c.st, pos, R, H, p.Hp, p.splits, xj.slab, (const float*)xj.acc, (__nv_bfloat16*)dx);
   }
   return (int)cudaGetLastError();
 }
@@ -815,9 +928,9 @@ using namespace ve;
 
 extern "C" {
 
-// Bytes of workspace that a call needs (256-byte aligned).
-long ve_head_loss_workspace(int grads, int want_dx, int x_fp32, const void* head, int head_fp32, long ldw, int R, int H, int V, int K, int kl) {
-  return (long)head_plan(grads, want_dx, x_fp32, head_fp32, head_packs(head, head_fp32, ldw, H), R, H, V, K, kl).bytes;
+// Bytes of workspace that a call needs (256-byte aligned). packs: the head is fp32, or its width, pitch or start keep its rows off 16-byte boundaries.
+long ve_head_loss_workspace(int grads, int want_dx, int x_fp32, int head_fp32, int packs, int R, int H, int V, int K, int kl) {
+  return (long)head_plan(grads, want_dx, x_fp32, head_fp32, packs, R, H, V, K, kl).bytes;
 }
 
 // x [R, H] (row pitch ldx), head [V, H] (pitch ldw), each bf16 or fp32. labels (int32 / int64 [R]) or ids int32 [R, K] with logp fp32 [R, K] and

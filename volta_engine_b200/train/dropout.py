@@ -13,8 +13,8 @@ from __future__ import annotations
 
 import torch
 
-from .._lib import call, ptr
-from .launch import on, refuse_capture, rows_of
+from .._lib import ptr
+from .launch import launch, refuse_capture, rows_of
 
 _DTYPES = (torch.bfloat16, torch.float32)
 
@@ -77,9 +77,8 @@ def _launch(x, residual, t, seed, row0, site):
     residual = rows_of(residual) if residual is not None else None
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     on_device = isinstance(seed, torch.Tensor)
-    with on(x.device):
-        call("dropout", "plplpiliiflpli", ptr(x), x.stride(0), ptr(residual), residual.stride(0) if residual is not None else 0, ptr(y),
-             int(x.dtype == torch.float32), x.shape[0], x.shape[1], t, _scale_of(t), 0 if on_device else seed, ptr(seed) if on_device else 0, row0, site)
+    launch(x.device, "dropout", "plplpiliiflpli", x.data_ptr(), x.stride(0), ptr(residual), residual.stride(0) if residual is not None else 0, y.data_ptr(),
+           x.dtype == torch.float32, x.shape[0], x.shape[1], t, _scale_of(t), 0 if on_device else seed, seed.data_ptr() if on_device else 0, row0, site)
     return y
 
 

@@ -20,12 +20,14 @@ workspace from the caching allocator and may be captured into a CUDA graph. CPU 
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
 
-from .._lib import call, kernels, ptr
-from .launch import on, refuse_capture, rows_of
+from .._lib import kernels, ptr
+from ..ops.kernels import status_word
+from .launch import launch, refuse_capture, rows_of
 
 MAX_TOPK = 1024
 REST_FLOOR = 1e-12                 # least probability of "any other token" in a divergence
@@ -37,32 +39,34 @@ def _check(x, head, softcap, others, dloss=None, stats=None):
     """Shapes, types and devices of a call; ``others``: (name, tensor, dtypes, shape)."""
     if x.dim() != 2 or head.dim() != 2 or x.shape[1] != head.shape[1]:
         raise ValueError(f"states [rows, hidden] and head [vocab, hidden] are wanted: got {tuple(x.shape)} and {tuple(head.shape)}")
-    if head.shape[0] < 1 or head.shape[1] < 1:
+    rows, vocab, device = x.shape[0], head.shape[0], x.device
+    if vocab < 1 or x.shape[1] < 1:
         raise ValueError(f"a head of {tuple(head.shape)} has no logits")
-    if max(x.shape[0], head.shape[0]) >= 1 << 24:
+    if rows >= 1 << 24 or vocab >= 1 << 24:
         raise ValueError("rows and vocabulary have to stay below 2^24")
     allowed = _DTYPES if x.is_cuda else _DTYPES + (torch.float64,)
-    for name, t in (("states", x), ("head", head)):
-        if t.dtype not in allowed:
-            raise TypeError(f"{name} of type {t.dtype}: bf16 and fp32 are supported")
-    if not (softcap >= 0 and math.isfinite(softcap)):
+    if x.dtype not in allowed:
+        raise TypeError(f"states of type {x.dtype}: bf16 and fp32 are supported")
+    if head.dtype not in allowed:
+        raise TypeError(f"head of type {head.dtype}: bf16 and fp32 are supported")
+    if head.device != device:
+        raise ValueError(f"head on {head.device}, states on {device}")
+    if not 0 <= softcap < math.inf:
         raise ValueError(f"softcap {softcap}: zero (none) or a positive number is wanted")
-    rows = x.shape[0]
     if dloss is not None:
-        others = others + [("dloss", dloss, (torch.float32,) if x.is_cuda else (torch.float32, torch.float64), (rows,)),
-                           ("stats", stats, (torch.float32,) if x.is_cuda else (torch.float32, torch.float64), (2, rows))]
+        f = (torch.float32,) if x.is_cuda else (torch.float32, torch.float64)
+        others += (("dloss", dloss, f, (rows,)), ("stats", stats, f, (2, rows)))
     for name, t, dtypes, shape in others:
         if t.dtype not in dtypes:
             raise TypeError(f"{name} of type {t.dtype}: {' or '.join(str(d) for d in dtypes)} is wanted")
-        if tuple(t.shape) != shape:
+        if t.shape != shape:
             raise ValueError(f"{name} of shape {tuple(t.shape)}: {shape} is wanted")
-    for name, t in [("head", head)] + [(n, t) for n, t, _, _ in others]:
-        if t.device != x.device:
-            raise ValueError(f"{name} on {t.device}, states on {x.device}")
+        if t.device != device:
+            raise ValueError(f"{name} on {t.device}, states on {device}")
 
 
 def _label_args(x, labels):
-    return [("labels", labels, (torch.int64, torch.int32), (x.shape[0],))]
+    return (("labels", labels, (torch.int64, torch.int32), (x.shape[0],)),)
 
 
 def _teacher_args(x, ids, logp, tail):
@@ -70,60 +74,59 @@ def _teacher_args(x, ids, logp, tail):
         raise ValueError(f"teacher ids [rows, K] with K of 1 to {MAX_TOPK} are wanted: got {tuple(ids.shape)}")
     f = (torch.float32,) if x.is_cuda else (torch.float32, torch.float64)
     rows, k = x.shape[0], ids.shape[1]
-    return [("ids", ids, (torch.int32,), (rows, k)), ("logp", logp, f, (rows, k)), ("tail", tail, f, (rows,))]
+    return ("ids", ids, (torch.int32,), (rows, k)), ("logp", logp, f, (rows, k)), ("tail", tail, f, (rows,))
 
 
-_workspace_bytes = None
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*sizes) -> int:
+    fn = kernels().ve_head_loss_workspace
+    fn.argtypes = [ctypes.c_int] * 10
+    fn.restype = ctypes.c_int64
+    return fn(*sizes)
 
 
 def _workspace(grads, want_dx, x, head, K, kl):
-    global _workspace_bytes
-    if _workspace_bytes is None:
-        fn = kernels().ve_head_loss_workspace
-        fn.argtypes = [ctypes.c_int] * 3 + [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64] + [ctypes.c_int] * 5
-        fn.restype = ctypes.c_int64
-        _workspace_bytes = fn
-    n = _workspace_bytes(grads, want_dx, x.dtype == torch.float32, ptr(head), head.dtype == torch.float32, head.stride(0), x.shape[0], x.shape[1],
-                         head.shape[0], K, kl)
+    packs = head.dtype == torch.float32 or head.shape[1] % 8 != 0 or head.stride(0) % 8 != 0 or head.data_ptr() % 16 != 0
+    n = _workspace_bytes(grads, want_dx, x.dtype == torch.float32, head.dtype == torch.float32, packs, x.shape[0], x.shape[1], head.shape[0], K, kl)
     return torch.empty(n, dtype=torch.uint8, device=x.device)
+
+
+_SIG = "pilpilpipppiiiif"
+
+
+def _common(x, head, labels, teacher, softcap):
+    ids, logp, tail = teacher or (None, None, None)
+    return (x.data_ptr(), x.dtype == torch.float32, x.stride(0), head.data_ptr(), head.dtype == torch.float32, head.stride(0), ptr(labels),
+            labels.element_size() if labels is not None else 0, ptr(ids), ptr(logp), ptr(tail), ids.shape[1] if teacher else 1, x.shape[0], x.shape[1],
+            head.shape[0], softcap)
 
 
 def _forward(x, head, labels, teacher, softcap):
     x, head = rows_of(x), rows_of(head)
     rows = x.shape[0]
-    ids, logp, tail = (t.contiguous() for t in teacher) if teacher else (None, None, None)
+    teacher = tuple(t.contiguous() for t in teacher) if teacher else None
     labels = labels.contiguous() if labels is not None else None
-    with on(x.device):
-        from ..ops.kernels import status_word
-        loss = torch.empty(rows, dtype=torch.float32, device=x.device)
-        stats = torch.empty(2, rows, dtype=torch.float32, device=x.device)
-        if not rows:
-            return loss, stats
-        K = ids.shape[1] if teacher else 1
-        ws = _workspace(0, 0, x, head, K, teacher is not None)
-        call("head_loss", "pilpilpipppiiiifppplp", ptr(x), int(x.dtype == torch.float32), x.stride(0), ptr(head), int(head.dtype == torch.float32),
-             head.stride(0), ptr(labels), labels.element_size() if labels is not None else 0, ptr(ids), ptr(logp), ptr(tail), K, rows, x.shape[1],
-             head.shape[0], float(softcap), ptr(loss), ptr(stats), ptr(ws), ws.numel(), ptr(status_word(x.device)))
+    out = torch.empty(3, rows, dtype=torch.float32, device=x.device)
+    loss, stats = out[0], out[1:]
+    if rows:
+        ws = _workspace(False, False, x, head, teacher[0].shape[1] if teacher else 1, teacher is not None)
+        launch(x.device, "head_loss", _SIG + "ppplp", *_common(x, head, labels, teacher, softcap), loss.data_ptr(), stats.data_ptr(), ws.data_ptr(),
+               ws.numel(), status_word(x.device).data_ptr())
     return loss, stats
 
 
 def _backward(x, head, labels, teacher, stats, dloss, softcap, want_dx, want_dhead):
     x, head = rows_of(x), rows_of(head)
     rows = x.shape[0]
-    ids, logp, tail = (t.contiguous() for t in teacher) if teacher else (None, None, None)
+    teacher = tuple(t.contiguous() for t in teacher) if teacher else None
     labels = labels.contiguous() if labels is not None else None
     stats, dloss = stats.contiguous(), dloss.contiguous()
-    with on(x.device):
-        from ..ops.kernels import status_word
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
-        dhead = (torch.empty if rows else torch.zeros)(head.shape, dtype=head.dtype, device=x.device) if want_dhead else None
-        if rows:
-            K = ids.shape[1] if teacher else 1
-            ws = _workspace(1, int(want_dx), x, head, K, teacher is not None)
-            call("head_loss_grad", "pilpilpipppiiiifppppplp", ptr(x), int(x.dtype == torch.float32), x.stride(0), ptr(head),
-                 int(head.dtype == torch.float32), head.stride(0), ptr(labels), labels.element_size() if labels is not None else 0, ptr(ids), ptr(logp),
-                 ptr(tail), K, rows, x.shape[1], head.shape[0], float(softcap), ptr(stats), ptr(dloss), ptr(dx), ptr(dhead), ptr(ws), ws.numel(),
-                 ptr(status_word(x.device)))
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
+    dhead = (torch.empty if rows else torch.zeros)(head.shape, dtype=head.dtype, device=x.device) if want_dhead else None
+    if rows:
+        ws = _workspace(True, want_dx, x, head, teacher[0].shape[1] if teacher else 1, teacher is not None)
+        launch(x.device, "head_loss_grad", _SIG + "ppppplp", *_common(x, head, labels, teacher, softcap), stats.data_ptr(), dloss.data_ptr(), ptr(dx),
+               ptr(dhead), ws.data_ptr(), ws.numel(), status_word(x.device).data_ptr())
     return dx, dhead
 
 

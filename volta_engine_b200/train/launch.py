@@ -1,14 +1,19 @@
 """What the training operators share when they launch: the tensors' device, rows in place, and the differentiable calls' stand on graph capture."""
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
+from .._lib import call_on
 
-def on(device):
-    """Launches of this block go to ``device``, on its current stream."""
-    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+def launch(device, name: str, sig: str, *args) -> None:
+    """``ve_<name>`` on ``device`` and its current stream, whichever device is current."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)           # (the handle alone: a Stream object costs more than a small kernel)
+    if device.index == torch._C._cuda_getDevice():
+        call_on(stream, name, sig, *args)
+    else:
+        with torch.cuda.device(device):
+            call_on(stream, name, sig, *args)
 
 
 def rows_of(t):

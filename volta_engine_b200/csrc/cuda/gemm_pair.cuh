@@ -51,14 +51,32 @@ VE_DEVINL void tma_load_3d_pair(void* smem_dst, const CUtensorMap* map, uint32_t
       ::"r"(smem_u32(smem_dst)), "l"(map), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
-// A box from shared memory to the tensor (asynchronous: the groups of the thread that asks for it).
-VE_DEVINL void tma_store_3d(const CUtensorMap* map, const void* smem_src, int x, int y, int z) {
-  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
-               ::"l"(map), "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z) : "memory");
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+// A warp's box of 32 rows x 128 bytes (64 bf16 or 32 fp32 values, `w`: those of the lane's row) to a tensor, through the warp's 4 KB of shared memory: a
+// thread's own stores would be 16 bytes of 32 different rows each. ADD: added to what stands there (fp32, in L2). Asynchronous.
+template <bool ADD>
+VE_DEVINL void put_box(const CUtensorMap* map, uint8_t* staging, const uint32_t* w, int x, int y, int z) {
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");       // the box in front has been read
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<uint4*>(staging + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    if (ADD)
+      asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.bulk_group [%0, {%2, %3, %4}], [%1];"
+                   ::"l"(map), "r"(smem_u32(staging)), "r"(x), "r"(y), "r"(z) : "memory");
+    else
+      asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+                   ::"l"(map), "r"(smem_u32(staging)), "r"(x), "r"(y), "r"(z) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
 }
-VE_DEVINL void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }      // the shared memory may be written again
-VE_DEVINL void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }               // written
+// The warp's boxes are written (before its CTA ends).
+VE_DEVINL void put_wait() {
+  if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
 VE_DEVINL void tmem_alloc_pair(uint32_t* smem_holder, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_holder)), "r"(ncols) : "memory");
 }
@@ -124,7 +142,7 @@ static inline PairLoop pair_loop(int sa, int sb, int order, int chunk) {
 
 // Job: gives the tiles (int tiles(), PairTile tile(int i)), the words of steps to repeat (const uint32_t* again(tile), or null), what a thread loads
 // in front of its sums (Row begin(tile, row of the tile, first column)) and takes the sums: finish(tile, row of the tile, first column, Row,
-// sums[128], omap, 4 KB of shared memory of the warp); done() when there are no more.
+// sums[128], omap, 4 KB of shared memory of the warp).
 // A_MN / B_MN: the operand is MN-major.
 // wait(): the point behind which other kernels' results are read.
 template <bool A_MN, bool B_MN, class Job, class Wait>
@@ -230,10 +248,12 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
     const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
     int piece = 0;
     bool ok = true;
+    const auto begin = [&](int t) { return job.begin(job.tile(t), rank * 128 + quarter * 32 + lane, half * 128); };
+    decltype(begin(0)) row{};
+    if (cluster < ntiles) row = begin(cluster);
     for (int t = cluster; t < ntiles; t += clusters) {
       const PairTile tl = job.tile(t);
       const int total = tl.ksteps * loop.pairs + step_count(job.again(tl), tl.k0, tl.k0 + tl.ksteps), pieces = (total + loop.chunk - 1) / loop.chunk;
-      const auto row = job.begin(tl, rank * 128 + quarter * 32 + lane, half * 128);
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.f;
@@ -256,9 +276,11 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
         if (lane == 0) mbar_arrive_cluster(first_cta_addr(&acc_empty[buf]));
       }
       if (!ok) break;
-      job.finish(tl, rank * 128 + quarter * 32 + lane, half * 128, row, acc, omap, smem + kPairStages * kPairStage + (warp - 4) * 4096);
+      const auto now = row;
+      if (t + clusters < ntiles) row = begin(t + clusters);  // (what the next tile's rows need is under way while this one's are finished)
+      job.finish(tl, rank * 128 + quarter * 32 + lane, half * 128, now, acc, omap, smem + kPairStages * kPairStage + (warp - 4) * 4096);
     }
-    job.done();
+    put_wait();
     if (!ok) atomicExch(&s_fail, 1);
   }
   tc_fence_before();

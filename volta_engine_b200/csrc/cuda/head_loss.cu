@@ -15,7 +15,7 @@
 // multiplies it with the head's rows and with the states. dz beside fp32 operands is three bf16 slabs (fp32's 24 bits). Beside bf16 operands it is one
 // slab, and what its rounding left (up to 2^-8 of a value: as much as the rounding of the gradients, whose error it would raise by 1.41, with few
 // rows by up to 2.5) in a second one that is multiplied only where it matters: blocks of 64 x 64 in which an element is above a sixteenth of its
-// row's largest (a label's own dz is at least every other's; for a teacher's tokens, above 2^-10 of the row's weight). Those are few: a label a row.
+// row's largest (a label's own dz is at least every other's; beside a teacher, above a 64th of the row's weight). Those are few: a label a row.
 // Sums run in a fixed order: the same call gives the same bits.
 //
 // Rows that are left out (label below zero, a teacher row of padding) are taken out in front: the states of the others are gathered, so what
@@ -89,8 +89,24 @@ VE_DEVINL long label_of(const HeadRows& p, int r) {
   return p.label_bytes == 8 ? (long)reinterpret_cast<const long long*>(p.labels)[r] : (long)reinterpret_cast<const int*>(p.labels)[r];
 }
 
-// The rows that count, in order: live[i] = row, pos[row] = i or -1, *count.
-__global__ void __launch_bounds__(1024) head_rows_kernel(const HeadRows p, const int* flag, int* live, int* pos, int* count) {
+// Ranges of a piece's `steps` that dx is summed over: tiles x ranges fill whole waves of the 74 pairs; a range costs about 12 steps beside its products
+// (its sums are written). Asked for on the device, where the number of rows that count is known: 819 of 2048 left half of the pairs idle.
+struct DxPlan {
+  int col_tiles, steps, pairs, most;
+};
+VE_DEVINL int dx_splits(int rows, const DxPlan& d) {
+  const int tiles = (rows + 255) / 256 * d.col_tiles;
+  int best = 1;
+  float least = 0.f;
+  for (int s = 1; s <= d.most && s * 4 <= d.steps; ++s) {
+    const float cost = (float)((tiles * s + kPairClusters - 1) / kPairClusters) * (float)((d.steps + s - 1) / s * d.pairs + 12);
+    if (s == 1 || cost < least) { least = cost; best = s; }
+  }
+  return best;
+}
+
+// The rows that count, in order: live[i] = row, pos[row] = i or -1, count[0] = their number, count[1] = ranges of dx.
+__global__ void __launch_bounds__(1024) head_rows_kernel(const HeadRows p, const int* flag, int* live, int* pos, int* count, const DxPlan dx) {
   __shared__ int part[32], base;
   grid_dep_launch();
   grid_dep_wait();
@@ -112,7 +128,10 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(const HeadRows p, const
     if (threadIdx.x == 1023) base = at + (on ? 1 : 0);
     __syncthreads();
   }
-  if (threadIdx.x == 0) *count = base;
+  if (threadIdx.x == 0) {
+    count[0] = base;
+    count[1] = dx_splits(base, dx);
+  }
 }
 
 // Eight values of a row from column c; zeros behind column H. `vec`: whole groups may be read as 16-byte words.
@@ -197,7 +216,7 @@ __global__ void __launch_bounds__(256) head_pack_kernel(const T* src, long ld, c
 // large blocks become zero on the way.
 template <typename T>
 __global__ void __launch_bounds__(256) head_front_kernel(const HeadRows p, const int* flag, int* live, int* pos, int* count, const T* src, long ld, int H, int Hp,
-                                                         int slabs, size_t slab, __nv_bfloat16* dst, uint4* words, size_t nwords) {
+                                                         int slabs, size_t slab, __nv_bfloat16* dst, uint4* words, size_t nwords, const DxPlan dx) {
   __shared__ int row_of[kFrontRows], part[8];
   grid_dep_launch();
   grid_dep_wait();
@@ -224,7 +243,10 @@ __global__ void __launch_bounds__(256) head_front_kernel(const HeadRows p, const
     }
     __syncthreads();
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) *count = n;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    count[0] = n;
+    count[1] = dx_splits(n, dx);
+  }
   const int all = (n + 255) / 256 * 256;
   for (int r = (int)(first >> 5); r < all; r += (int)(step >> 5))
     pack_row(r < n ? src + row_of[r] * ld : (const T*)nullptr, H, Hp, slabs, slab, dst + (size_t)r * Hp);
@@ -261,7 +283,6 @@ struct LogitTiles {           // rows x a piece of the vocabulary: tiles of up t
   VE_DEVINL int row_tiles() const { return (*count + 255) >> 8; }
   VE_DEVINL int tiles() const { return row_tiles() * ((nv + 255) >> 8); }
   VE_DEVINL const uint32_t* again(const PairTile&) const { return nullptr; }
-  VE_DEVINL void done() const {}
   struct Row { int row, begin, end; };        // the caller's row (-1: behind the last one), its targets among the thread's columns
   VE_DEVINL Row row_at(const PairTile& t, int r, int c0, const int* live, const Targets& tg) const {
     const int i = t.m0 + r, col0 = t.n0 + c0;
@@ -368,7 +389,7 @@ struct RowInputs {            // by row of the caller
       const double a = mass[row], lr = (double)rest - (double)lse, t = lr >= (double)kLogFloor ? exp((double)tail[row]) : 0.0;
       c.at = (float)((double)g * (a + t)) * fix;
       c.dense = (float)((double)g * (t > 0.0 ? a + t - t * exp(-lr) : a)) * fix;       // (a difference: in 64 bits)
-      c.large = fabsf(g) * (1.f / 1024.f);
+      c.large = fabsf(g) * (1.f / 64.f);
     }
     return c;
   }
@@ -404,6 +425,7 @@ struct GradJob : LogitTiles {
     int p = w.begin;
     // targets first, one of each lane at a time: their dz takes the logit's place, and its bit says that it stands there
     uint32_t set[4] = {0u, 0u, 0u, 0u};
+    const bool any = __any_sync(0xffffffffu, p < end);
     while (__any_sync(0xffffffffu, p < end)) {
       const int at = p < end ? tg.id(row, p) - v0 - col0 : -1;
       float v = 0.f, d = c.at;
@@ -431,16 +453,24 @@ struct GradJob : LogitTiles {
 #pragma unroll
       for (int j = 0; j < 128; ++j) z[j] = j == at ? d : z[j];
     }
-#pragma unroll
-    for (int j = 0; j < 128; ++j) {
-      float f = c.dense, v = z[j];
+    const auto dz = [&](float v) {
+      float f = c.dense;
       if (CAP) {
         const float th = tanhf(over_cap(v, cap, inv_cap));
         v = cap * th;
         f *= 1.f - th * th;
       }
-      const float d = f * ex2_approx(fmaf(v, kLog2e, -c.lse2));
-      z[j] = set[j >> 5] >> (j & 31) & 1u ? z[j] : d;
+      return f * ex2_approx(fmaf(v, kLog2e, -c.lse2));
+    };
+    if (CAP || any) {
+#pragma unroll
+      for (int j = 0; j < 128; ++j) {
+        const float d = dz(z[j]);
+        z[j] = set[j >> 5] >> (j & 31) & 1u ? z[j] : d;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 128; ++j) z[j] = dz(z[j]);
     }
     if (__any_sync(0xffffffffu, row < 0 || cols < 128)) {        // zeros to the ends of the tile: the products along rows and columns read them
       const int width = row >= 0 ? cols : 0;
@@ -460,60 +490,45 @@ struct GradJob : LogitTiles {
         }
       }
     }
-    // out by TMA, 32 rows x 64 columns at a time: a thread's own stores are 16 bytes of 32 different rows each, 12 000 cycles a tile of three slabs
-    const int lane = threadIdx.x & 31;
     for (int s = 0; s < slabs; ++s)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (lane == 0) tma_store_wait_read();
-        __syncwarp();
+        uint32_t b[32];
 #pragma unroll
-        for (int j = 0; j < 64; j += 8) {
-          uint32_t b[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) b[e] = split_pair(z[64 * h + j + 2 * e], z[64 * h + j + 2 * e + 1]);
-          *reinterpret_cast<uint4*>(staging + lane * 128 + (((j >> 3) ^ (lane & 7)) << 4)) = make_uint4(b[0], b[1], b[2], b[3]);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) tma_store_3d(omap, staging, col0 + 64 * h, i, s);
+        for (int j = 0; j < 32; ++j) b[j] = split_pair(z[64 * h + 2 * j], z[64 * h + 2 * j + 1]);
+        put_box<false>(omap, staging, b, col0 + 64 * h, i & ~31, s);
       }
-  }
-  VE_DEVINL void done() const {
-    if ((threadIdx.x & 31) == 0) tma_store_wait();
   }
 };
 
-// dx: gathered rows x H, along a piece of the vocabulary, cut into `splits` ranges that keep their own fp32 sums.
+// dx: gathered rows x H, along a piece of the vocabulary, cut into ranges that keep their own fp32 sums (the same number in every piece).
 struct DxJob {
   const int* count;
-  int H, Hp, ksteps, splits, first;
+  int H, Hp, ksteps, first;
   size_t slab;
-  float* acc;                 // [splits][rows_cap][Hp]
+  float* acc;                 // [ranges][rows_cap][Hp]
   LargeBlocks big;
   struct Row {};
   VE_DEVINL Row begin(const PairTile&, int, int) const { return {}; }
-  VE_DEVINL void done() const {}
   VE_DEVINL const uint32_t* again(const PairTile& t) const { return big.of_rows ? big.of_rows + (t.m0 >> 8) * big.row_words : nullptr; }
   VE_DEVINL int row_tiles() const { return (*count + 255) >> 8; }
-  VE_DEVINL int tiles() const { return row_tiles() * ((H + 255) >> 8) * splits; }
+  VE_DEVINL int splits() const { return count[1]; }
+  VE_DEVINL int tiles() const { return row_tiles() * ((H + 255) >> 8) * splits(); }
   VE_DEVINL PairTile tile(int i) const {
-    const int nm = row_tiles(), per = (ksteps + splits - 1) / splits;
-    const int m = i % nm, j = i / nm, s = j % splits;
-    return PairTile{m * 256, (j / splits) * 256, s * per, max(0, min(per, ksteps - s * per)), s};
+    const int nm = row_tiles(), tiles = nm * ((H + 255) >> 8), s = i / tiles, j = i - s * tiles;
+    const int n = splits(), per = (ksteps + n - 1) / n;
+    return PairTile{j % nm * 256, j / nm * 256, s * per, max(0, min(per, ksteps - s * per)), s};
   }
   VE_DEVINL void finish(const PairTile& t, int r, int c0, const Row& w, float* z, const CUtensorMap* omap, uint8_t* staging) const {
-    const int i = t.m0 + r;
-    if (i >= *count) return;
-    float* dst = acc + t.split * slab + (size_t)i * Hp + t.n0 + c0;
-    const int cols = Hp - t.n0 - c0;
+    const int x = t.n0 + c0, y = t.m0 + (r & ~31);
+    if (y >= *count) return;
 #pragma unroll
-    for (int j = 0; j < 128; j += 4) {
-      if (j >= cols) continue;
-      if (first)
-        *reinterpret_cast<float4*>(dst + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
-      else                       // (one addition to each sum a piece, the pieces in order: no choice of order; waiting for the old sums took 17 % of a piece)
-        asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst + j), "f"(z[j]), "f"(z[j + 1]), "f"(z[j + 2]), "f"(z[j + 3]) : "memory");
+    for (int g = 0; g < 4; ++g) {
+      if (x + 32 * g >= Hp) break;
+      const uint32_t* b = reinterpret_cast<const uint32_t*>(z + 32 * g);
+      // (one addition to each sum a piece, the pieces in order: no choice of order; waiting for the old sums took 17 % of a piece)
+      if (first) put_box<false>(omap, staging, b, x + 32 * g, y, t.split);
+      else put_box<true>(omap, staging, b, x + 32 * g, y, t.split);
     }
   }
 };
@@ -524,10 +539,11 @@ struct DheadJob {
   const int* count;
   int nv, H;
   T* out;                     // [nv, H], contiguous rows
+  bool boxes;                 // rows on 16-byte boundaries: written by TMA (omap)
+  static constexpr int kBox = 128 / sizeof(T);
   LargeBlocks big;
   struct Row {};
   VE_DEVINL Row begin(const PairTile&, int, int) const { return {}; }
-  VE_DEVINL void done() const {}
   VE_DEVINL const uint32_t* again(const PairTile& t) const { return big.of_cols ? big.of_cols + (t.m0 >> 8) * big.col_words : nullptr; }
   VE_DEVINL int tiles() const { return ((nv + 255) >> 8) * ((H + 255) >> 8); }
   VE_DEVINL PairTile tile(int i) const {
@@ -535,24 +551,16 @@ struct DheadJob {
     return PairTile{i / nn * 256, i % nn * 256, 0, (*count + 63) >> 6, 0};
   }
   VE_DEVINL void finish(const PairTile& t, int r, int c0, const Row& w, float* z, const CUtensorMap* omap, uint8_t* staging) const {
-    const int v = t.m0 + r, cols = H - t.n0 - c0;
+    const int cols = H - t.n0 - c0;
     if (cols <= 0 || t.m0 + (r & ~31) >= nv) return;
-    const bool vec = !((uintptr_t)out & 15) && H % (16 / (int)sizeof(T)) == 0;
-    if (vec) {
-      if (v >= nv) return;
-      T* dst = out + (size_t)v * H + t.n0 + c0;
+    if (boxes) {
 #pragma unroll
-      for (int j = 0; j < 128; j += 8) {
-        if (j >= cols) continue;                    // (whole groups: the width is a multiple of them, of fp32 values of four)
-        if (sizeof(T) == 4) {
-          *reinterpret_cast<float4*>(dst + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
-          if (j + 4 < cols) *reinterpret_cast<float4*>(dst + j + 4) = make_float4(z[j + 4], z[j + 5], z[j + 6], z[j + 7]);
-        } else {
-          uint32_t b[4];
+      for (int g = 0; g < 128 / kBox; ++g) {
+        if (g * kBox >= cols) break;
+        uint32_t b[32];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) b[e] = split_pair(z[j + 2 * e], z[j + 2 * e + 1]);
-          *reinterpret_cast<uint4*>(dst + j) = make_uint4(b[0], b[1], b[2], b[3]);
-        }
+        for (int j = 0; j < 32; ++j) b[j] = sizeof(T) == 4 ? __float_as_uint(z[32 * g + j]) : split_pair(z[kBox * g + 2 * j], z[kBox * g + 2 * j + 1]);
+        put_box<false>(omap, staging, b, t.n0 + c0 + kBox * g, t.m0 + (r & ~31), 0);
       }
       return;
     }
@@ -670,9 +678,10 @@ __global__ void __launch_bounds__(1024) head_merge_kernel(const HeadRows p, cons
 
 // dx of the caller's rows from the ranges' sums; zeros where a row was left out.
 template <typename T>
-__global__ void __launch_bounds__(256) head_dx_kernel(const int* pos, int R, int H, int Hp, int splits, size_t slab, const float* acc, T* dx) {
+__global__ void __launch_bounds__(256) head_dx_kernel(const DxJob job, const int* pos, int R, T* dx) {
   grid_dep_launch();
   grid_dep_wait();
+  const int H = job.H, Hp = job.Hp, splits = job.splits();
   const int per = (H + 3) / 4;
   const bool vec = !((uintptr_t)dx & 15) && H % 4 == 0;
   for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < (size_t)R * per; i += (size_t)gridDim.x * blockDim.x) {
@@ -680,9 +689,9 @@ __global__ void __launch_bounds__(256) head_dx_kernel(const int* pos, int R, int
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     const int at = pos[r];
     if (at >= 0) {
-      const float* a = acc + (size_t)at * Hp + c;
+      const float* a = job.acc + (size_t)at * Hp + c;
       for (int s = 0; s < splits; ++s) {
-        const float4 w = *reinterpret_cast<const float4*>(a + s * slab);
+        const float4 w = *reinterpret_cast<const float4*>(a + s * job.slab);
         v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
       }
     }
@@ -705,7 +714,7 @@ struct HeadPlan {             // sizes and places in the workspace
   int rows_cap, nblk, ksteps;
   bool pack_head;             // the head's rows go through slabs of their own, a piece at a time
   int piece;                  // vocabulary rows at a time
-  int splits;                 // ranges of a piece that dx is summed over
+  int splits, pairs;          // most ranges of a piece that dx is summed over; products of slabs
   int row_words, col_words;   // of LargeBlocks
   size_t live, pos, count, flag, mass, sid, slp, off, x, part, zt, head, G, acc, big, big_bytes, bytes;      // (big_bytes: of a piece)
 };
@@ -730,19 +739,12 @@ static HeadPlan head_plan(bool grads, bool want_dx, int x_fp32, int head_fp32, b
   if (pack_head) { const size_t most = (512ull << 20) / ((size_t)p.sw * p.Hp * 2) / 256 * 256; piece = piece < most ? piece : (most ? most : 256); }
   if (grads) { const size_t most = (256ull << 20) / ((size_t)p.sg * p.rows_cap * 2) / 256 * 256; piece = piece < most ? piece : (most ? most : 256); }
   p.piece = (int)piece;
-  // dx: tiles x ranges fill whole waves of the 74 pairs; a range costs about 12 steps beside its products (sums read and written)
-  const long tiles = (long)(p.rows_cap / 256) * ((H + 255) / 256), steps = p.piece / 64;
-  const int pairs = x_fp32 ? (head_fp32 ? 6 : 3) : (head_fp32 ? 3 : 1);
-  long best = 0;
-  p.splits = 1;
-  for (int s = 1; s <= kPairClusters && s * 4 <= steps; ++s) {
-    const long cost = (tiles * s + kPairClusters - 1) / kPairClusters * ((steps + s - 1) / s * pairs + 12);
-    if (s == 1 || cost < best) { best = cost; p.splits = s; }
-    if (tiles * s > 8 * kPairClusters) break;
-  }
+  p.pairs = x_fp32 ? (head_fp32 ? 6 : 3) : (head_fp32 ? 3 : 1);
+  const size_t sums = 4ull * p.rows_cap * p.Hp;                                          // of a range of dx: 256 MB together
+  p.splits = (int)((256ull << 20) / sums < 1 ? 1 : (256ull << 20) / sums < 32 ? (256ull << 20) / sums : 32);
   size_t at = 0;
   auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
-  p.live = take(4ull * R); p.pos = take(4ull * R); p.count = take(4);
+  p.live = take(4ull * R); p.pos = take(4ull * R); p.count = take(8);
   p.flag = p.mass = p.sid = p.slp = p.off = 0;
   if (kl) { p.flag = take(4ull * R); p.mass = take(8ull * R); p.sid = take(4ull * R * K); p.slp = take(4ull * R * K); p.off = take(2ull * R * (p.nblk + 1)); }
   p.x = take(2ull * p.sx * p.rows_cap * p.Hp);
@@ -798,16 +800,17 @@ template <typename T>
 static int front_rows(const HeadCall& c, const HeadPlan& p, size_t word_bytes) {
   int *live = (int*)(c.ws + p.live), *pos = (int*)(c.ws + p.pos), *count = (int*)(c.ws + p.count), *flag = (int*)(c.ws + p.flag);
   const size_t slab = (size_t)p.rows_cap * p.Hp;
+  const DxPlan dx{(c.H + 255) / 256, p.piece / 64, p.pairs, p.acc ? p.splits : 0};
   if (c.rows.R <= kFrontRows) {
     launch_pdl(head_front_kernel<T>, dim3(blocks_of((size_t)p.rows_cap, 8)), dim3(256), 0, c.st, c.rows, (const int*)flag, live, pos, count,
-               (const T*)c.x, c.ldx, c.H, p.Hp, p.sx, slab, (__nv_bfloat16*)(c.ws + p.x), (uint4*)(c.ws + p.big), word_bytes / 16);
+               (const T*)c.x, c.ldx, c.H, p.Hp, p.sx, slab, (__nv_bfloat16*)(c.ws + p.x), (uint4*)(c.ws + p.big), word_bytes / 16, dx);
     return 0;
   }
   if (word_bytes) {
     const cudaError_t e = cudaMemsetAsync(c.ws + p.big, 0, word_bytes, c.st);
     if (e != cudaSuccess) return (int)e;
   }
-  launch_pdl(head_rows_kernel, dim3(1), dim3(1024), 0, c.st, c.rows, (const int*)flag, live, pos, count);
+  launch_pdl(head_rows_kernel, dim3(1), dim3(1024), 0, c.st, c.rows, (const int*)flag, live, pos, count, dx);
   pack_rows<T>(c.x, c.ldx, live, count, p.rows_cap, c, p, p.sx, slab, c.ws + p.x);
   return 0;
 }
@@ -871,18 +874,21 @@ static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, c
   if (rc) return rc;
   const int *live = (const int*)(c.ws + p.live), *pos = (const int*)(c.ws + p.pos), *count = (const int*)(c.ws + p.count);
   const int R = c.rows.R, H = c.H;
-  CUtensorMap xk, xmn, wk, wmn, gk, gmn, gout;
+  CUtensorMap xk, xmn, wk, wmn, gk, gmn, gout, aout, hout;
   rc = slab_map(&xk, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, 128);
   if (!rc) rc = slab_map(&xmn, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, 64);
   if (!rc) rc = slab_map(&gk, c.ws + p.G, p.sg, p.rows_cap, p.rows_cap, p.piece, p.piece, 128);
   if (!rc) rc = slab_map(&gmn, c.ws + p.G, p.sg, p.rows_cap, p.rows_cap, p.piece, p.piece, 64);
+  if (!rc && dx)
+    rc = make_tmap_3d(&aout, c.ws + p.acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.splits, p.rows_cap, p.Hp, 4ull * p.rows_cap * p.Hp, 4ull * p.Hp, 32, 32,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
   if (!rc) rc = slab_map(&gout, c.ws + p.G, p.sg, p.rows_cap, p.rows_cap, p.piece, p.piece, 32);
   if (rc) return rc;
   GradJob<CAP> gj;
   gj.count = count; gj.ksteps = p.ksteps; gj.tg = head_targets_of(c, p); gj.live = live; 
   gj.slabs = p.sg; gj.cap = c.softcap; gj.inv_cap = CAP ? 1.f / c.softcap : 0.f;
   gj.in = RowInputs{stats, dloss, c.rows.tail, (const double*)(c.ws + p.mass), R, c.rows.labels != nullptr};
-  DxJob xj{count, H, p.Hp, 0, p.splits, 1, (size_t)p.rows_cap * p.Hp, (float*)(c.ws + p.acc), {}};
+  DxJob xj{count, H, p.Hp, 0, 1, (size_t)p.rows_cap * p.Hp, (float*)(c.ws + p.acc), {}};
   const bool exact = p.sg == 3;
   for (int v0 = 0; v0 < c.rows.V; v0 += p.piece) {
     const int nv = c.rows.V - v0 < p.piece ? c.rows.V - v0 : p.piece;
@@ -901,23 +907,30 @@ static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, c
       xj.ksteps = (nv + 63) / 64;
       xj.first = v0 == 0;
       const PairLoop loop = c.x_fp32 ? pair_loop(p.sg, p.sw, 2, kExactChunk) : pair_loop(p.sg, p.sw, exact ? 1 : 0, kRoundedChunk);
-      if ((rc = launch_pair<false, true>(xj, loop, gk, wmn, gk, c))) return rc;
+      if ((rc = launch_pair<false, true>(xj, loop, gk, wmn, aout, c))) return rc;
     }
     if (dhead) {
+      const size_t es = c.head_fp32 ? 4 : 2;
+      uint8_t* out = (uint8_t*)dhead + (size_t)v0 * H * es;
+      const bool boxes = H * es % 16 == 0 && !((uintptr_t)dhead & 15);
+      if (boxes && (rc = make_tmap_3d(&hout, out, c.head_fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (int)es, 1, nv, H, nv * H * es,
+                                      H * es, 32, (uint32_t)(128 / es), CU_TENSOR_MAP_SWIZZLE_128B)))
+        return rc;
+      if (!boxes) hout = gmn;
       if (c.head_fp32) {
-        const DheadJob<float> job{count, nv, H, (float*)dhead + (size_t)v0 * H, big};
-        rc = launch_pair<true, true>(job, pair_loop(p.sg, p.sx, 2, kExactChunk), gmn, xmn, gmn, c);
+        const DheadJob<float> job{count, nv, H, (float*)out, boxes, big};
+        rc = launch_pair<true, true>(job, pair_loop(p.sg, p.sx, 2, kExactChunk), gmn, xmn, hout, c);
       } else {
-        const DheadJob<__nv_bfloat16> job{count, nv, H, (__nv_bfloat16*)dhead + (size_t)v0 * H, big};
-        rc = launch_pair<true, true>(job, pair_loop(p.sg, p.sx, exact ? 1 : 0, kRoundedChunk), gmn, xmn, gmn, c);
+        const DheadJob<__nv_bfloat16> job{count, nv, H, (__nv_bfloat16*)out, boxes, big};
+        rc = launch_pair<true, true>(job, pair_loop(p.sg, p.sx, exact ? 1 : 0, kRoundedChunk), gmn, xmn, hout, c);
       }
       if (rc) return rc;
     }
   }
   if (dx) {
     const int grid = blocks_of((size_t)R * p.Hp / 4);
-    if (c.x_fp32) launch_pdl(head_dx_kernel<float>, dim3(grid), dim3(256), 0, c.st, pos, R, H, p.Hp, p.splits, xj.slab, (const float*)xj.acc, (float*)dx);
-    else launch_pdl(head_dx_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, c.st, pos, R, H, p.Hp, p.splits, xj.slab, (const float*)xj.acc, (__nv_bfloat16*)dx);
+    if (c.x_fp32) launch_pdl(head_dx_kernel<float>, dim3(grid), dim3(256), 0, c.st, xj, pos, R, (float*)dx);
+    else launch_pdl(head_dx_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, c.st, xj, pos, R, (__nv_bfloat16*)dx);
   }
   return (int)cudaGetLastError();
 }

@@ -5,7 +5,7 @@
 //   cross entropy   nll_r = lse_r - z_ry = log(1 + exp(rest_r - z_ry))                     rest_r = log sum_{v != y} exp z_rv
 //   divergence      kl_r  = sum_k a_k (log a_k - log s_k) + t (log t - log max(rho_r, 1e-12))    rho_r = exp(rest_r - lse_r), rest over v not in K
 //   gradients       dz_rv = g_r s_rv ((A + t) - [v not in K] t / rho_r) - g_r [v in K] a_v,  A = sum_k a_k
-//                   (the label is a teacher of one token: A = 1, t = 0; its own dz is -g exp(rest - lse), which does not cancel)
+//                   (the label is a teacher of one token: A = 1, t = 0; a likely one's own dz is taken as -g exp(rest - lse), which does not cancel)
 //                   dx = (dz cap') W,  dW = (dz cap')^T x
 //
 // The logits exist a 256 x 256 tile at a time, in registers (gemm_pair.cuh). Scoring keeps of each row and 128 columns the maximum and the sum
@@ -283,11 +283,12 @@ struct LogitTiles {           // rows x a piece of the vocabulary: tiles of up t
   VE_DEVINL int row_tiles() const { return (*count + 255) >> 8; }
   VE_DEVINL int tiles() const { return row_tiles() * ((nv + 255) >> 8); }
   VE_DEVINL const uint32_t* again(const PairTile&) const { return nullptr; }
-  struct Row { int row, begin, end; };        // the caller's row (-1: behind the last one), its targets among the thread's columns
+  struct Row { int row, begin, end, first; };        // the caller's row (-1: behind the last one), its targets among the thread's columns, the first one's column
   VE_DEVINL Row row_at(const PairTile& t, int r, int c0, const int* live, const Targets& tg) const {
     const int i = t.m0 + r, col0 = t.n0 + c0;
-    Row w{i < *count ? live[i] : -1, 0, 0};
+    Row w{i < *count ? live[i] : -1, 0, 0, -1};
     if (w.row >= 0 && col0 < nv) tg.range(w.row, (v0 + col0) >> 7, (long)v0 + col0, min(128, nv - col0), w.begin, w.end);
+    if (w.begin < w.end) w.first = tg.id(w.row, w.begin) - v0 - col0;
     return w;
   }
   VE_DEVINL PairTile tile(int i) const {
@@ -297,15 +298,25 @@ struct LogitTiles {           // rows x a piece of the vocabulary: tiles of up t
   }
 };
 
-VE_DEVINL float over_cap(float z, float cap, float inv_cap) {          // z / cap to rounding: the quotient with the rounded 1 / cap, and its rest
-  const float q = z * inv_cap;
-  return fmaf(fmaf(-q, cap, z), inv_cap, q);
-}
+// A thread's logits through the cap. c tanh(z / c) = z f(x^2), x = z / c, with Lambert's continued fraction f = 1 / (1 + x^2 / (3 + x^2 / (5 + ..))) of
+// tanh(x) / x; to seven terms it is 1.1e-8 off at x = 2 and less below. Where a lane's logits reach further the library's tanh is taken (128 of those
+// are 5600 cycles a tile, these 1300).
 template <bool CAP>
 VE_DEVINL void cap_logits(float* z, float cap, float inv_cap) {
-  if (CAP) {
+  if (!CAP) return;
+  float top = 0.f;
 #pragma unroll
-    for (int j = 0; j < 128; ++j) z[j] = cap * tanhf(over_cap(z[j], cap, inv_cap));
+  for (int j = 0; j < 128; ++j) top = fmaxf(top, fabsf(z[j]));
+  if (__any_sync(0xffffffffu, !(top <= 2.f * cap))) {
+#pragma unroll
+    for (int j = 0; j < 128; ++j) z[j] = cap * tanhf(z[j] / cap);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 128; ++j) {
+      const float x = z[j] * inv_cap, y = x * x;
+      const float num = fmaf(fmaf(y + 378.f, y, 17325.f), y, 135135.f), den = fmaf(fmaf(fmaf(28.f, y, 3150.f), y, 62370.f), y, 135135.f);
+      z[j] *= num * rcp_approx(den);
+    }
   }
 }
 
@@ -334,17 +345,21 @@ struct ScoreJob : LogitTiles {
     }
     // a token of each lane at a time: selects, for branches in the body of 128 columns fetch their code anew for every tile (20 us a tile that a target
     // falls into)
-    while (__any_sync(0xffffffffu, p < end)) {
-      const int at = p < end ? tg.id(row, p) - v0 - col0 : -1;
+    int at = w.first;
+    while (__any_sync(0xffffffffu, at >= 0)) {
       float v = 0.f;
 #pragma unroll
       for (int j = 0; j < 128; ++j) {
         v = j == at ? z[j] : v;
         z[j] = j == at ? neg_inf() : z[j];
       }
-      if (p < end) {
-        do zt[(size_t)row * tg.K + p] = v;          // (a token listed twice is one token)
-        while (++p < end && tg.id(row, p) - v0 - col0 == at);
+      if (at >= 0) {
+        int next;
+        do {                                        // (a token listed twice is one token)
+          zt[(size_t)row * tg.K + p] = v;
+          next = ++p < end ? tg.id(row, p) - v0 - col0 : -1;
+        } while (next == at);
+        at = next;
       }
     }
     float m = z[0];
@@ -363,7 +378,7 @@ struct ScoreJob : LogitTiles {
   }
 };
 
-// Constants of a row's dz: at any token dense * s, at a target `at` * s - g * (teacher's mass); a label's is `at` itself.
+// Constants of a row's dz: at any token dense * s, at a target `at` * s - g * (teacher's mass); a likely label's is `at` itself.
 struct RowGrad {
   float lse2, dense, at, g;
   float large;                // dz above this is multiplied with its rounding error too
@@ -411,10 +426,14 @@ struct GradJob : LogitTiles {
   LargeBlocks big;            // (null: every slab counts everywhere)
   float cap, inv_cap;
 
-  struct Row : LogitTiles::Row { RowGrad c; };
+  struct Row : LogitTiles::Row {
+    RowGrad c;
+    float mass;               // the teacher's, of the first target
+  };
   VE_DEVINL Row begin(const PairTile& t, int r, int c0) const {
-    Row w{row_at(t, r, c0, live, tg), {0.f, 0.f, 0.f, 0.f, 0.f}};
+    Row w{row_at(t, r, c0, live, tg), {0.f, 0.f, 0.f, 0.f, 0.f}, 0.f};
     if (w.row >= 0) w.c = in.at(w.row);
+    if (!tg.labels && w.first >= 0) w.mass = expf(tg.slp[(size_t)w.row * tg.K + w.begin]);
     return w;
   }
 
@@ -425,44 +444,48 @@ struct GradJob : LogitTiles {
     int p = w.begin;
     // targets first, one of each lane at a time: their dz takes the logit's place, and its bit says that it stands there
     uint32_t set[4] = {0u, 0u, 0u, 0u};
-    const bool any = __any_sync(0xffffffffu, p < end);
-    while (__any_sync(0xffffffffu, p < end)) {
-      const int at = p < end ? tg.id(row, p) - v0 - col0 : -1;
+    cap_logits<CAP>(z, cap, inv_cap);
+    int at = w.first;
+    float mass = w.mass;
+    const bool any = __any_sync(0xffffffffu, at >= 0);
+    while (__any_sync(0xffffffffu, at >= 0)) {
       float v = 0.f, d = c.at;
 #pragma unroll
       for (int j = 0; j < 128; ++j) v = j == at ? z[j] : v;
-      if (p < end) {
-        float slope = 1.f;
-        if (CAP) {
-          const float th = tanhf(over_cap(v, cap, inv_cap));
-          v = cap * th;
-          slope = 1.f - th * th;
+      int next = -1;
+      const float s = ex2_approx(fmaf(v, kLog2e, -c.lse2));
+      if (tg.labels) {
+        if (s < 0.5f) d = fmaf(c.dense, s, -c.g);          // (an unlikely label: s - 1 keeps what exp(rest - lse) loses to two roundings)
+      } else if (at >= 0) {
+        float a = mass;
+        while (++p < end) {
+          next = tg.id(row, p) - v0 - col0;
+          mass = expf(tg.slp[(size_t)row * tg.K + p]);
+          if (next != at) break;
+          a += mass;
+          next = -1;
         }
-        if (tg.labels) {
-          ++p;
-        } else {
-          float a = 0.f;
-          do a += expf(tg.slp[(size_t)row * tg.K + p]);
-          while (++p < end && tg.id(row, p) - v0 - col0 == at);
-          d = fmaf(c.at, ex2_approx(fmaf(v, kLog2e, -c.lse2)), -c.g * a);
-        }
-        if (CAP) d *= slope;
+        d = fmaf(c.at, s, -c.g * a);
+      }
+      if (CAP) {
+        const float th = v * inv_cap;
+        d *= fmaf(-th, th, 1.f);
       }
 #pragma unroll
-      for (int w = 0; w < 4; ++w) set[w] |= at >> 5 == w ? 1u << (at & 31) : 0u;
+      for (int k = 0; k < 4; ++k) set[k] |= at >> 5 == k ? 1u << (at & 31) : 0u;
 #pragma unroll
       for (int j = 0; j < 128; ++j) z[j] = j == at ? d : z[j];
+      at = next;
     }
     const auto dz = [&](float v) {
       float f = c.dense;
       if (CAP) {
-        const float th = tanhf(over_cap(v, cap, inv_cap));
-        v = cap * th;
-        f *= 1.f - th * th;
+        const float th = v * inv_cap;
+        f *= fmaf(-th, th, 1.f);
       }
       return f * ex2_approx(fmaf(v, kLog2e, -c.lse2));
     };
-    if (CAP || any) {
+    if (any) {
 #pragma unroll
       for (int j = 0; j < 128; ++j) {
         const float d = dz(z[j]);
@@ -842,7 +865,7 @@ static Targets head_targets_of(const HeadCall& c, const HeadPlan& p) {
 
 // Steps of 64 between fp32 additions where 32 bits are asked for. Cut-off sums over a step are 5e-8 too small; this keeps that below what fp32 additions
 // along H round by (H = 128 7e-8, 1024 2.5e-7, 5120 7e-7). Shorter pieces wait for their additions: of one step 15 to 50 %, of two up to 6 %.
-static inline int exact_chunk(int H) { return H <= 256 ? 1 : H <= 1280 ? 2 : 4; }
+static inline int exact_chunk(int H) { return H <= 256 ? 1 : H <= 640 ? 2 : 4; }
 constexpr int kExactChunk = 4;         // along rows or the vocabulary: gradients in fp32
 constexpr int kRoundedChunk = 32;      // where the result is rounded to bf16 (cut-off sums over 2048: 2e-6), or a gradient's logits are (2e-6 of z: 2^-15 of s)
 

@@ -123,7 +123,7 @@ def test_refusals():
         L.head_cross_entropy(x.half(), head, lab)
     with pytest.raises(TypeError, match="head of type"):
         L.head_cross_entropy(x, head.half(), lab)
-    for cap in (-1.0, math.nan, math.inf):
+    for cap in (-1.0, 1e-50, math.nan, math.inf):
         with pytest.raises(ValueError, match="softcap"):
             L.head_cross_entropy(x, head, lab, softcap=cap)
     with pytest.raises(ValueError, match="no logits"):
@@ -265,6 +265,9 @@ def test_strides_and_starts(types):
         got = run(xs, hs, t, dl)
         for k in got:
             assert torch.equal(got[k], want[k]), k
+    # a single row of an expanded matrix, for either side
+    one = run(x[:1].expand(2, -1)[:1], head[:1].expand(3, -1)[:1], (torch.zeros(1, dtype=torch.int64, device="cuda"),), dl[:1])
+    assert float(one["loss"]) == 0 and float(one["dx"].abs().max()) == 0
     # labels of 32 bits, strided
     lab = torch.stack([t[0].int(), t[0].int() * 0], 1)[:, 0]
     got = run(x, head, (lab,), dl)

@@ -24,6 +24,7 @@ import torch
 import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
+from ..ops.kernels import check_status
 from ..train.dropout import dropout_residual
 from ..train.head_loss import head_cross_entropy_loss, head_kl_loss
 
@@ -422,6 +423,9 @@ def tune(model: TunedModel, sequences: list, teachers: list, o: E2EOptions, held
         hist["train"].append(total)
         if (step + 1) % o.eval_every == 0 or step + 1 == o.steps:
             evaluate(step + 1)
+    for d in {torch.device(d) for d in model.devices}:
+        if check_status(d):
+            raise RuntimeError(f"a kernel on {d} gave up a wait: the results of this run are not valid")
     return hist
 
 

@@ -149,6 +149,10 @@ def run(engine, seqs, chunk: int = 512, topk: int = 0, teacher: dict | None = No
             for key, j in (("ids", 0), ("logp", 1), ("tail", 2)):
                 out_t[key].append(torch.cat([p[j] for p in parts]))
         log(f"sequence {si}: {len(seq)} tokens, running ppl {math.exp(nll / max(count, 1)):.4f}")
+    if no_logits:
+        from ..ops.kernels import check_status
+        if check_status(engine.device):
+            raise RuntimeError("a kernel gave up a wait: the scores of this run are not valid")
     res = {"nll": nll / max(count, 1), "tokens": count, "ppl": math.exp(nll / max(count, 1))}
     if teacher is not None:
         res["kl"] = kl_sum / max(kl_n, 1)

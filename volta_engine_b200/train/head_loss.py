@@ -51,8 +51,8 @@ def _check(x, head, softcap, others, dloss=None, stats=None):
         raise TypeError(f"head of type {head.dtype}: bf16 and fp32 are supported")
     if head.device != device:
         raise ValueError(f"head on {head.device}, states on {device}")
-    if not 0 <= softcap < math.inf:
-        raise ValueError(f"softcap {softcap}: zero (none) or a positive number is wanted")
+    if softcap != 0 and not 1e-30 <= softcap < math.inf:
+        raise ValueError(f"softcap {softcap}: zero (none) or a number of at least 1e-30 is wanted")
     if dloss is not None:
         f = (torch.float32,) if x.is_cuda else (torch.float32, torch.float64)
         others += (("dloss", dloss, f, (rows,)), ("stats", stats, f, (2, rows)))

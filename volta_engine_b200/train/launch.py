@@ -18,7 +18,9 @@ def launch(device, name: str, sig: str, *args) -> None:
 
 def rows_of(t):
     """A matrix whose rows' elements lie side by side: ``t`` itself where they do."""
-    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] or t.shape[0] == 0 else t.contiguous()
+    if t.stride(1) == 1 and t.stride(0) >= t.shape[1] or t.shape[0] == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)          # (``contiguous`` leaves the pitch of a single row as it is, zero for an expanded one)
 
 
 def refuse_capture(t):

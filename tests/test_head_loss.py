@@ -147,7 +147,7 @@ def test_refusals():
 
 
 # ------------------------------------------------------------------------------------------------ GPU
-SIZES = [(1, 64, 300), (1, 2048, 1000), (5, 72, 1), (3, 8, 127), (130, 136, 513), (257, 320, 1025), (300, 1001, 2050), (64, 515, 4099), (700, 256, 5000), (12, 196, 2889)]
+SIZES = [(1, 64, 300), (1, 2048, 1000), (5, 72, 1), (3, 8, 127), (130, 136, 513), (257, 320, 1025), (300, 1001, 2050), (64, 515, 4099), (700, 256, 5000), (12, 196, 2889), (300, 200, 20001)]
 
 
 @pytest.mark.gpu
@@ -160,7 +160,7 @@ def test_cross_entropy(rows, hidden, vocab, types):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,hidden,vocab,topk", [(1, 64, 300, 1), (2, 128, 40, 40), (130, 136, 513, 7), (257, 320, 1025, 64), (77, 515, 5003, 17), (9, 256, 3000, 1024), (8, 132, 1877, 62)])
+@pytest.mark.parametrize("rows,hidden,vocab,topk", [(1, 64, 300, 1), (2, 128, 40, 40), (130, 136, 513, 7), (257, 320, 1025, 64), (77, 515, 5003, 17), (9, 256, 3000, 1024), (8, 132, 1877, 62), (260, 136, 19500, 33)])
 @pytest.mark.parametrize("types", ["bf16 bf16", "fp32 bf16", "fp32 fp32"])
 def test_divergence(rows, hidden, vocab, topk, types):
     xt, ht = types.split()
@@ -171,9 +171,10 @@ def test_divergence(rows, hidden, vocab, topk, types):
 @pytest.mark.gpu
 @pytest.mark.parametrize("topk", [0, 9])
 @pytest.mark.parametrize("types", ["bf16 bf16", "fp32 fp32"])
-def test_soft_cap(topk, types):
+@pytest.mark.parametrize("vocab", [777, 20100])                       # tiles of 64 columns, and of 256
+def test_soft_cap(topk, types, vocab):
     xt, ht = types.split()
-    a = make(150, 200, 777, topk, xt, ht, seed=4, left_out=0.2, device="cuda", spread=8.0)
+    a = make(300 if vocab > 777 else 150, 200, vocab, topk, xt, ht, seed=4, left_out=0.2, device="cuda", spread=8.0)
     hold(run(*a, 20.0), *a, 20.0, only=("loss", "stats"))
     # the gradients beside those of the CPU statement in 64 bits of the same inputs: the cap takes no more from dz than it gives
     got, w = run(*a, 20.0), P.wanted(*a, 20.0)
@@ -276,13 +277,13 @@ def test_strides_and_starts(types):
 
 @pytest.mark.gpu
 def test_one_gradient_alone_and_the_same_bits_again():
-    for topk in (0, 5):
-        x, head, t, dl = make(300, 264, 3000, topk, seed=8, left_out=0.1, device="cuda")
+    for topk, vocab in ((0, 3000), (5, 3000), (5, 38000)):
+        x, head, t, dl = make(300, 264, vocab, topk, seed=8, left_out=0.1, device="cuda")
         a, b = run(x, head, t, dl), run(x, head, t, dl)
         assert all(torch.equal(a[k], b[k]) for k in a)
         c, d = run(x, head, t, dl, want_dhead=False), run(x, head, t, dl, want_dx=False)
         assert c["dhead"] is None and d["dx"] is None and torch.equal(c["dx"], a["dx"]) and torch.equal(d["dhead"], a["dhead"])
-        # a row does not depend on the rows beside it
+        # a row does not depend on the rows beside it (while the tiles are of one width)
         e = run(x[40:120], head, tuple(v[40:120] for v in t), dl[40:120])
         assert torch.equal(e["loss"], a["loss"][40:120]) and torch.equal(e["stats"], a["stats"][:, 40:120])
 

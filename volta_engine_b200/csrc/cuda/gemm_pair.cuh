@@ -2,7 +2,7 @@
 //
 //   D[m, n] = sum over operand pairs (a, b) and over k of A_a[m, k] * B_b[n, k]
 //
-// Tile: 256 x 256 a pair, each CTA holds 128 rows of A, 128 of the 256 rows of B and 128 x 256 of the sums. A step of 64 along K brings
+// Tile: 256 x 256 a pair (or 256 x 64), each CTA holds 128 rows of A, 128 of the 256 rows of B and 128 x 256 of the sums. A step of 64 along K brings
 // 32 KB to each CTA for 512 cycles of its tensor core, half of what a 128 x 256 tile of one CTA asks of L2. Either operand is K-major
 // ([rows, K]) or MN-major ([K, rows]).
 //
@@ -21,10 +21,17 @@
 
 namespace ve {
 
-constexpr int kPairStages = 6, kPairHalf = 128 * 128, kPairStage = 2 * kPairHalf;       // bytes: 128 rows x 64 of A and of B
-constexpr int kPairStaging = 8 * 4096;                     // behind the ring: 32 rows x 64 bf16 columns for each summing warp's stores
-constexpr int kPairSmem = kPairStages * kPairStage + kPairStaging + 1024;
-static_assert(kPairSmem <= 227 * 1024 - 512, "shared memory (beside the barriers)");
+// A tile is 256 rows x NT columns, 256 or, for logits of few tiles, 64: four times the pairs have work, and a thread finishes 32 columns in place of 128.
+template <int NT>
+struct PairShape {
+  static constexpr int kA = 128 * 128, kB = NT / 2 * 128, kStage = kA + kB;        // bytes of a step in a CTA: 128 rows x 64 of A, NT / 2 of B
+  static constexpr int kStages = NT == 256 ? 6 : 9;
+  static constexpr int kCols = NT / 2;                                              // of a thread
+};
+constexpr int kPairRing = 6 * PairShape<256>::kStage;
+constexpr int kPairStaging = 8 * 4096;                     // behind the ring: a box of each summing warp's stores
+constexpr int kPairSmem = kPairRing + kPairStaging + 1024;
+static_assert(kPairSmem <= 227 * 1024 - 512 && 9 * PairShape<64>::kStage <= kPairRing, "shared memory (beside the barriers)");
 constexpr int kPairClusters = 74, kPairThreads = 384;
 
 VE_DEVINL uint32_t cluster_rank() {
@@ -51,16 +58,17 @@ VE_DEVINL void tma_load_3d_pair(void* smem_dst, const CUtensorMap* map, uint32_t
       ::"r"(smem_u32(smem_dst)), "l"(map), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
-// A warp's box of 32 rows x 128 bytes (64 bf16 or 32 fp32 values, `w`: those of the lane's row) to a tensor, through the warp's 4 KB of shared memory: a
-// thread's own stores would be 16 bytes of 32 different rows each. ADD: added to what stands there (fp32, in L2). Asynchronous.
-template <bool ADD>
+// A warp's box of 32 rows x ROW = 128 or 64 bytes (`w`: those of the lane's row; the map's swizzle is as wide) to a tensor, through the warp's 4 KB of
+// shared memory: a thread's own stores would be 16 bytes of 32 different rows each. ADD: added to what stands there (fp32, in L2). Asynchronous.
+template <bool ADD, int ROW = 128>
 VE_DEVINL void put_box(const CUtensorMap* map, uint8_t* staging, const uint32_t* w, int x, int y, int z) {
   const int lane = threadIdx.x & 31;
   if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");       // the box in front has been read
   __syncwarp();
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<uint4*>(staging + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  for (int j = 0; j < ROW / 16; ++j)
+    *reinterpret_cast<uint4*>(staging + lane * ROW + ((j ^ (ROW == 128 ? lane & 7 : (lane >> 1) & 3)) << 4)) =
+        make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
   fence_proxy_async_smem();
   __syncwarp();
   if (lane == 0) {
@@ -100,7 +108,7 @@ VE_DEVINL void tc_mma_f16_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, 
 
 // What one tile covers. Rows and columns count from the operands' own origins; steps of 64 along K.
 struct PairTile {
-  int m0, n0;                 // first row / column of the 256 x 256 tile
+  int m0, n0;                 // first row / column of the tile
   int k0, ksteps;             // first step and number of steps (of each pair of slabs)
   int split;
 };
@@ -142,20 +150,23 @@ static inline PairLoop pair_loop(int sa, int sb, int order, int chunk) {
 
 // Job: gives the tiles (int tiles(), PairTile tile(int i)), the words of steps to repeat (const uint32_t* again(tile), or null), what a thread loads
 // in front of its sums (Row begin(tile, row of the tile, first column)) and takes the sums: finish(tile, row of the tile, first column, Row,
-// sums[128], omap, 4 KB of shared memory of the warp).
+// sums[NT / 2], omap, 4 KB of shared memory of the warp).
 // A_MN / B_MN: the operand is MN-major.
 // wait(): the point behind which other kernels' results are read.
-template <bool A_MN, bool B_MN, class Job, class Wait>
+template <int NT, bool A_MN, bool B_MN, class Job, class Wait>
 VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap* amap, const CUtensorMap* bmap, const CUtensorMap* omap, int* status, Wait wait) {
+  static_assert(NT == 256 || !B_MN, "64 columns of an MN-major operand are one box of a CTA");
+  using S = PairShape<NT>;
+  constexpr int kStages = S::kStages, kCols = S::kCols;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
+  __shared__ uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_holder;
   __shared__ int s_fail;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank(), cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kPairStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 16); }
     s_fail = 0;
     mbar_fence_init();
@@ -178,26 +189,26 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
       bool ok = true;
       for (int t = cluster; t < ntiles && ok; t += clusters) {
         const PairTile tl = job.tile(t);
-        const int am = tl.m0 + rank * 128, bn = tl.n0 + rank * 128;
+        const int am = tl.m0 + rank * 128, bn = tl.n0 + rank * kCols;
         auto load = [&](int k, int sa, int sb) {
-          const int s = it % kPairStages;
-          if (!mbar_wait(&empty[s], ((it / kPairStages) & 1) ^ 1)) return false;
+          const int s = it % kStages;
+          if (!mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1)) return false;
           ++it;
-          uint8_t* st = smem + s * kPairStage;
-          if (rank == 0) mbar_expect_tx(&full[s], 2 * kPairStage);
+          uint8_t* st = smem + s * S::kStage;
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * S::kStage);
           const uint32_t bar = first_cta_addr(&full[s]);
           const int kk = k * 64;
           if (A_MN) {
             tma_load_3d_pair(st, amap, bar, am, kk, sa);
-            tma_load_3d_pair(st + kPairHalf / 2, amap, bar, am + 64, kk, sa);
+            tma_load_3d_pair(st + S::kA / 2, amap, bar, am + 64, kk, sa);
           } else {
             tma_load_3d_pair(st, amap, bar, kk, am, sa);
           }
           if (B_MN) {
-            tma_load_3d_pair(st + kPairHalf, bmap, bar, bn, kk, sb);
-            tma_load_3d_pair(st + kPairHalf + kPairHalf / 2, bmap, bar, bn + 64, kk, sb);
+            tma_load_3d_pair(st + S::kA, bmap, bar, bn, kk, sb);
+            tma_load_3d_pair(st + S::kA + S::kB / 2, bmap, bar, bn + 64, kk, sb);
           } else {
-            tma_load_3d_pair(st + kPairHalf, bmap, bar, kk, bn, sb);
+            tma_load_3d_pair(st + S::kA, bmap, bar, kk, bn, sb);
           }
           return true;
         };
@@ -211,7 +222,7 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
       }
       if (!ok) atomicExch(&s_fail, 1);
     } else if (warp == 1 && rank == 0 && elect_one()) {
-      constexpr uint32_t idesc = make_idesc_f16(1, 1, 256, 256) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+      constexpr uint32_t idesc = make_idesc_f16(1, 1, 256, NT) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
       int it = 0, piece = 0;
       bool ok = true;
       for (int t = cluster; t < ntiles && ok; t += clusters) {
@@ -224,16 +235,16 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
           tc_fence_after();
           const int end = min(total, i + loop.chunk);
           for (bool first = true; i < end; ++i, ++it, first = false) {
-            const int s = it % kPairStages;
-            ok = mbar_wait(&full[s], (it / kPairStages) & 1);
+            const int s = it % kStages;
+            ok = mbar_wait(&full[s], (it / kStages) & 1);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t a = smem_u32(smem + s * kPairStage), b = a + kPairHalf;
+            const uint32_t a = smem_u32(smem + s * S::kStage), b = a + S::kA;
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb) {
-              const uint64_t ad = A_MN ? make_desc_sw128_mn(a + kb * 2048, kPairHalf / 2, 1024) : make_desc_sw128(a) + kb * 2;
-              const uint64_t bd = B_MN ? make_desc_sw128_mn(b + kb * 2048, kPairHalf / 2, 1024) : make_desc_sw128(b) + kb * 2;
-              tc_mma_f16_pair(tmem_base + buf * 256, ad, bd, idesc, (first && kb == 0) ? 0u : 1u);
+              const uint64_t ad = A_MN ? make_desc_sw128_mn(a + kb * 2048, S::kA / 2, 1024) : make_desc_sw128(a) + kb * 2;
+              const uint64_t bd = B_MN ? make_desc_sw128_mn(b + kb * 2048, S::kB / 2, 1024) : make_desc_sw128(b) + kb * 2;
+              tc_mma_f16_pair(tmem_base + buf * NT, ad, bd, idesc, (first && kb == 0) ? 0u : 1u);
             }
             tc_commit_pair(&empty[s]);
           }
@@ -245,18 +256,18 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
+    const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * kCols;
     int piece = 0;
     bool ok = true;
-    const auto begin = [&](int t) { return job.begin(job.tile(t), rank * 128 + quarter * 32 + lane, half * 128); };
+    const auto begin = [&](int t) { return job.begin(job.tile(t), rank * 128 + quarter * 32 + lane, half * kCols); };
     decltype(begin(0)) row{};
     if (cluster < ntiles) row = begin(cluster);
     for (int t = cluster; t < ntiles; t += clusters) {
       const PairTile tl = job.tile(t);
       const int total = tl.ksteps * loop.pairs + step_count(job.again(tl), tl.k0, tl.k0 + tl.ksteps), pieces = (total + loop.chunk - 1) / loop.chunk;
-      float acc[128];
+      float acc[kCols];
 #pragma unroll
-      for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+      for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
 #pragma unroll 1
       for (int c = 0; c < pieces; ++c, ++piece) {
         const int buf = piece & 1;
@@ -264,9 +275,9 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
+        for (int g = 0; g < kCols / 32; ++g) {
           uint32_t r[32];
-          tmem_ld32(taddr + buf * 256 + g * 32, r);
+          tmem_ld32(taddr + buf * NT + g * 32, r);
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 32; ++j) acc[g * 32 + j] += __uint_as_float(r[j]);
@@ -278,7 +289,7 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
       if (!ok) break;
       const auto now = row;
       if (t + clusters < ntiles) row = begin(t + clusters);  // (what the next tile's rows need is under way while this one's are finished)
-      job.finish(tl, rank * 128 + quarter * 32 + lane, half * 128, now, acc, omap, smem + kPairStages * kPairStage + (warp - 4) * 4096);
+      job.finish(tl, rank * 128 + quarter * 32 + lane, half * kCols, now, acc, omap, smem + kPairRing + (warp - 4) * 4096);
     }
     put_wait();
     if (!ok) atomicExch(&s_fail, 1);

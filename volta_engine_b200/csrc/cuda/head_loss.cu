@@ -43,8 +43,8 @@ struct HeadRows {
 };
 
 // Divergence: the teacher's tokens of a row in ascending order, with their places: sid / slp [R, K] (padding behind, as INT_MAX), and at
-// off[r, b] the first one at or behind column 128 b; flag[r]: the row counts; mass[r] = sum_k a_k. One block a row, counting ranks: K is small.
-__global__ void __launch_bounds__(128) head_targets_kernel(const HeadRows p, int nblk, int* sid, float* slp, uint16_t* off, int* flag, double* mass) {
+// off[r, b] the first one at or behind column span * b; flag[r]: the row counts; mass[r] = sum_k a_k. One block a row, counting ranks: K is small.
+__global__ void __launch_bounds__(128) head_targets_kernel(const HeadRows p, int span, int nblk, int* sid, float* slp, uint16_t* off, int* flag, double* mass) {
   __shared__ int id[kMaxTopk], srt[kMaxTopk];
   __shared__ double part[4];
   grid_dep_launch();
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(128) head_targets_kernel(const HeadRows p, int
     int lo = 0, hi = p.K;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (srt[mid] < b * 128) lo = mid + 1; else hi = mid;
+      if (srt[mid] < b * span) lo = mid + 1; else hi = mid;
     }
     off[(size_t)r * (nblk + 1) + b] = (uint16_t)lo;
   }
@@ -260,7 +260,7 @@ struct Targets {              // by row of the caller
   const float* slp;
   const uint16_t* off;        // [R, nblk + 1]
   int K, nblk;
-  VE_DEVINL void range(int row, int blk, long col0, int cols, int& begin, int& end) const {      // targets of a row among 128 columns
+  VE_DEVINL void range(int row, int blk, long col0, int cols, int& begin, int& end) const {      // targets of a row among a thread's columns
     if (labels) {
       const long y = label_bytes == 8 ? (long)reinterpret_cast<const long long*>(labels)[row] : (long)reinterpret_cast<const int*>(labels)[row];
       begin = 0;
@@ -277,42 +277,44 @@ struct Targets {              // by row of the caller
   }
 };
 
+template <int C>              // columns of a thread
 struct LogitTiles {           // rows x a piece of the vocabulary: tiles of up to 16 row tiles share the head's rows while L2 holds them
+  static constexpr int NT = 2 * C;
   const int* count;
   int v0, nv, ksteps;
   VE_DEVINL int row_tiles() const { return (*count + 255) >> 8; }
-  VE_DEVINL int tiles() const { return row_tiles() * ((nv + 255) >> 8); }
+  VE_DEVINL int tiles() const { return row_tiles() * ((nv + NT - 1) / NT); }
   VE_DEVINL const uint32_t* again(const PairTile&) const { return nullptr; }
   struct Row { int row, begin, end, first; };        // the caller's row (-1: behind the last one), its targets among the thread's columns, the first one's column
   VE_DEVINL Row row_at(const PairTile& t, int r, int c0, const int* live, const Targets& tg) const {
     const int i = t.m0 + r, col0 = t.n0 + c0;
     Row w{i < *count ? live[i] : -1, 0, 0, -1};
-    if (w.row >= 0 && col0 < nv) tg.range(w.row, (v0 + col0) >> 7, (long)v0 + col0, min(128, nv - col0), w.begin, w.end);
+    if (w.row >= 0 && col0 < nv) tg.range(w.row, (v0 + col0) / C, (long)v0 + col0, min(C, nv - col0), w.begin, w.end);
     if (w.begin < w.end) w.first = tg.id(w.row, w.begin) - v0 - col0;
     return w;
   }
   VE_DEVINL PairTile tile(int i) const {
-    const int nm = row_tiles(), nn = (nv + 255) >> 8, per = 16 * nn;
+    const int nm = row_tiles(), nn = (nv + NT - 1) / NT, per = 16 * nn;
     const int g = i / per, m_first = g * 16, gm = min(16, nm - m_first), j = i - g * per;
-    return PairTile{(m_first + j % gm) * 256, (j / gm) * 256, 0, ksteps, 0};
+    return PairTile{(m_first + j % gm) * 256, (j / gm) * NT, 0, ksteps, 0};
   }
 };
 
 // A thread's logits through the cap. c tanh(z / c) = z f(x^2), x = z / c, with Lambert's continued fraction f = 1 / (1 + x^2 / (3 + x^2 / (5 + ..))) of
 // tanh(x) / x; to seven terms it is 1.1e-8 off at x = 2 and less below. Where a lane's logits reach further the library's tanh is taken (128 of those
 // are 5600 cycles a tile, these 1300).
-template <bool CAP>
+template <bool CAP, int C>
 VE_DEVINL void cap_logits(float* z, float cap, float inv_cap) {
   if (!CAP) return;
   float top = 0.f;
 #pragma unroll
-  for (int j = 0; j < 128; ++j) top = fmaxf(top, fabsf(z[j]));
+  for (int j = 0; j < C; ++j) top = fmaxf(top, fabsf(z[j]));
   if (__any_sync(0xffffffffu, !(top <= 2.f * cap))) {
 #pragma unroll
-    for (int j = 0; j < 128; ++j) z[j] = cap * tanhf(z[j] / cap);
+    for (int j = 0; j < C; ++j) z[j] = cap * tanhf(z[j] / cap);
   } else {
 #pragma unroll
-    for (int j = 0; j < 128; ++j) {
+    for (int j = 0; j < C; ++j) {
       const float x = z[j] * inv_cap, y = x * x;
       const float num = fmaf(fmaf(y + 378.f, y, 17325.f), y, 135135.f), den = fmaf(fmaf(fmaf(28.f, y, 3150.f), y, 62370.f), y, 135135.f);
       z[j] *= num * rcp_approx(den);
@@ -320,27 +322,29 @@ VE_DEVINL void cap_logits(float* z, float cap, float inv_cap) {
   }
 }
 
-template <bool CAP>
-struct ScoreJob : LogitTiles {
+template <bool CAP, int C>
+struct ScoreJob : LogitTiles<C> {
+  using Tiles = LogitTiles<C>;
+  using Tiles::nv; using Tiles::v0;
   Targets tg;
   const int* live;
   int rows_cap;               // pitch of part
-  float2* part;               // [128-column block][row]: maximum and sum of exp(z - maximum) without the targets
+  float2* part;               // [block of C columns][row]: maximum and sum of exp(z - maximum) without the targets
   float* zt;                  // [R, K] logits of the targets, in the targets' ascending order
   float cap, inv_cap;
-  using Row = LogitTiles::Row;
-  VE_DEVINL Row begin(const PairTile& t, int r, int c0) const { return row_at(t, r, c0, live, tg); }
+  using Row = typename Tiles::Row;
+  VE_DEVINL Row begin(const PairTile& t, int r, int c0) const { return this->row_at(t, r, c0, live, tg); }
 
   VE_DEVINL void finish(const PairTile& t, int r, int c0, const Row& w, float* z, const CUtensorMap* omap, uint8_t* staging) const {
-    const int i = t.m0 + r, row = w.row, col0 = t.n0 + c0, cols = min(128, nv - col0), blk = (v0 + col0) >> 7;
+    const int i = t.m0 + r, row = w.row, col0 = t.n0 + c0, cols = min(C, nv - col0), blk = (v0 + col0) / C;
     if (!__any_sync(0xffffffffu, row >= 0) || cols <= 0) return;
     const bool on = row >= 0;
     int p = w.begin;
     const int end = w.end;
-    cap_logits<CAP>(z, cap, inv_cap);
-    if (cols < 128) {
+    cap_logits<CAP, C>(z, cap, inv_cap);
+    if (cols < C) {
 #pragma unroll
-      for (int j = 0; j < 128; ++j)
+      for (int j = 0; j < C; ++j)
         if (j >= cols) z[j] = neg_inf();
     }
     // a token of each lane at a time: selects, for branches in the body of 128 columns fetch their code anew for every tile (20 us a tile that a target
@@ -349,7 +353,7 @@ struct ScoreJob : LogitTiles {
     while (__any_sync(0xffffffffu, at >= 0)) {
       float v = 0.f;
 #pragma unroll
-      for (int j = 0; j < 128; ++j) {
+      for (int j = 0; j < C; ++j) {
         v = j == at ? z[j] : v;
         z[j] = j == at ? neg_inf() : z[j];
       }
@@ -364,11 +368,11 @@ struct ScoreJob : LogitTiles {
     }
     float m = z[0];
 #pragma unroll
-    for (int j = 1; j < 128; ++j) m = fmaxf(m, z[j]);
+    for (int j = 1; j < C; ++j) m = fmaxf(m, z[j]);
     const float m2 = m == neg_inf() ? 0.f : -(m * kLog2e);
     float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
-    for (int j = 0; j < 128; j += 4) {
+    for (int j = 0; j < C; j += 4) {
       s0 += ex2_approx(fmaf(z[j], kLog2e, m2));
       s1 += ex2_approx(fmaf(z[j + 1], kLog2e, m2));
       s2 += ex2_approx(fmaf(z[j + 2], kLog2e, m2));
@@ -417,21 +421,24 @@ struct LargeBlocks {
   int row_words, col_words;   // words of a tile
 };
 
-template <bool CAP>
-struct GradJob : LogitTiles {
+template <bool CAP, int C>
+struct GradJob : LogitTiles<C> {
+  using Tiles = LogitTiles<C>;
+  using Tiles::nv; using Tiles::v0;
   Targets tg;
   const int* live;
   RowInputs in;
   int slabs;                  // of dz
+  static constexpr int kBox = C < 64 ? C : 64, kBoxes = C / kBox;        // columns that leave together
   LargeBlocks big;            // (null: every slab counts everywhere)
   float cap, inv_cap;
 
-  struct Row : LogitTiles::Row {
+  struct Row : Tiles::Row {
     RowGrad c;
     float mass;               // the teacher's, of the first target
   };
   VE_DEVINL Row begin(const PairTile& t, int r, int c0) const {
-    Row w{row_at(t, r, c0, live, tg), {0.f, 0.f, 0.f, 0.f, 0.f}, 0.f};
+    Row w{this->row_at(t, r, c0, live, tg), {0.f, 0.f, 0.f, 0.f, 0.f}, 0.f};
     if (w.row >= 0) w.c = in.at(w.row);
     if (!tg.labels && w.first >= 0) w.mass = expf(tg.slp[(size_t)w.row * tg.K + w.begin]);
     return w;
@@ -439,19 +446,19 @@ struct GradJob : LogitTiles {
 
   VE_DEVINL void finish(const PairTile& t, int r, int c0, const Row& w, float* z, const CUtensorMap* omap, uint8_t* staging) const {
     const int i = t.m0 + r, row = w.row, end = w.end;
-    const int col0 = t.n0 + c0, cols = max(0, min(128, nv - col0));
+    const int col0 = t.n0 + c0, cols = max(0, min(C, nv - col0));
     const RowGrad c = w.c;
     int p = w.begin;
     // targets first, one of each lane at a time: their dz takes the logit's place, and its bit says that it stands there
-    uint32_t set[4] = {0u, 0u, 0u, 0u};
-    cap_logits<CAP>(z, cap, inv_cap);
+    uint32_t set[C / 32] = {};
+    cap_logits<CAP, C>(z, cap, inv_cap);
     int at = w.first;
     float mass = w.mass;
     const bool any = __any_sync(0xffffffffu, at >= 0);
     while (__any_sync(0xffffffffu, at >= 0)) {
       float v = 0.f, d = c.at;
 #pragma unroll
-      for (int j = 0; j < 128; ++j) v = j == at ? z[j] : v;
+      for (int j = 0; j < C; ++j) v = j == at ? z[j] : v;
       int next = -1;
       const float s = ex2_approx(fmaf(v, kLog2e, -c.lse2));
       if (tg.labels) {
@@ -472,9 +479,9 @@ struct GradJob : LogitTiles {
         d *= fmaf(-th, th, 1.f);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) set[k] |= at >> 5 == k ? 1u << (at & 31) : 0u;
+      for (int k = 0; k < C / 32; ++k) set[k] |= at >> 5 == k ? 1u << (at & 31) : 0u;
 #pragma unroll
-      for (int j = 0; j < 128; ++j) z[j] = j == at ? d : z[j];
+      for (int j = 0; j < C; ++j) z[j] = j == at ? d : z[j];
       at = next;
     }
     const auto dz = [&](float v) {
@@ -487,25 +494,25 @@ struct GradJob : LogitTiles {
     };
     if (any) {
 #pragma unroll
-      for (int j = 0; j < 128; ++j) {
+      for (int j = 0; j < C; ++j) {
         const float d = dz(z[j]);
         z[j] = set[j >> 5] >> (j & 31) & 1u ? z[j] : d;
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 128; ++j) z[j] = dz(z[j]);
+      for (int j = 0; j < C; ++j) z[j] = dz(z[j]);
     }
-    if (__any_sync(0xffffffffu, row < 0 || cols < 128)) {        // zeros to the ends of the tile: the products along rows and columns read them
+    if (__any_sync(0xffffffffu, row < 0 || cols < C)) {        // zeros to the ends of the tile: the products along rows and columns read them
       const int width = row >= 0 ? cols : 0;
 #pragma unroll
-      for (int j = 0; j < 128; ++j) z[j] = j < width ? z[j] : 0.f;
+      for (int j = 0; j < C; ++j) z[j] = j < width ? z[j] : 0.f;
     }
     if (big.of_rows) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < kBoxes; ++h) {
         float m = 0.f;
 #pragma unroll
-        for (int j = 64 * h; j < 64 * h + 64; ++j) m = fmaxf(m, fabsf(z[j]));
+        for (int j = kBox * h; j < kBox * h + kBox; ++j) m = fmaxf(m, fabsf(z[j]));
         if (__any_sync(0xffffffffu, m > c.large) && (threadIdx.x & 31) == 0) {
           const int kc = (col0 >> 6) + h, kr = i >> 6;
           atomicOr(big.of_rows + (t.m0 >> 8) * big.row_words + (kc >> 5), 1u << (kc & 31));
@@ -515,11 +522,11 @@ struct GradJob : LogitTiles {
     }
     for (int s = 0; s < slabs; ++s)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t b[32];
+      for (int h = 0; h < kBoxes; ++h) {
+        uint32_t b[kBox / 2];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) b[j] = split_pair(z[64 * h + 2 * j], z[64 * h + 2 * j + 1]);
-        put_box<false>(omap, staging, b, col0 + 64 * h, i & ~31, s);
+        for (int j = 0; j < kBox / 2; ++j) b[j] = split_pair(z[kBox * h + 2 * j], z[kBox * h + 2 * j + 1]);
+        put_box<false, 2 * kBox>(omap, staging, b, col0 + kBox * h, i & ~31, s);
       }
   }
 };
@@ -605,12 +612,12 @@ struct DheadJob {
   }
 };
 
-template <bool A_MN, bool B_MN, class Job>
+template <int NT, bool A_MN, bool B_MN, class Job>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 head_gemm_kernel(const Job job, const PairLoop loop, const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                  const __grid_constant__ CUtensorMap omap, int* status) {
   grid_dep_launch();
-  pair_gemm<A_MN, B_MN>(job, loop, &amap, &bmap, &omap, status, [] { grid_dep_wait(); });
+  pair_gemm<NT, A_MN, B_MN>(job, loop, &amap, &bmap, &omap, status, [] { grid_dep_wait(); });
 }
 
 // ------------------------------------------------------------------------------------------------ the rows' sums
@@ -734,7 +741,8 @@ __global__ void __launch_bounds__(256) head_dx_kernel(const DxJob job, const int
 // ------------------------------------------------------------------------------------------------ host side
 struct HeadPlan {             // sizes and places in the workspace
   int Hp, sx, sw, sg;         // padded width; slabs of the states, the head, dz
-  int rows_cap, nblk, ksteps;
+  int rows_cap, ksteps;
+  int span, nblk;             // columns of a thread of the logits' tiles, and blocks of so many in the vocabulary
   bool pack_head;             // the head's rows go through slabs of their own, a piece at a time
   int piece;                  // vocabulary rows at a time
   int splits, pairs;          // most ranges of a piece that dx is summed over; products of slabs
@@ -755,7 +763,10 @@ static HeadPlan head_plan(bool grads, bool want_dx, int x_fp32, int head_fp32, b
   p.sw = head_fp32 ? 3 : 1;
   p.sg = x_fp32 || head_fp32 ? 3 : 2;
   p.rows_cap = (R + 255) / 256 * 256;
-  p.nblk = (V + 127) / 128;
+  // tiles of 256 columns where they give every pair one, otherwise of 64 (96 x 512 x 4099 in fp32 with gradients 89 us against 99, 77 x 515 x 5003 with a
+  // teacher and a cap 84 against 96)
+  p.span = (long)(p.rows_cap / 256) * ((V + 255) / 256) < kPairClusters ? 32 : 128;
+  p.nblk = (V + p.span - 1) / p.span;
   p.ksteps = (H + 63) / 64;
   p.pack_head = pack_head;
   size_t piece = ((size_t)V + 255) / 256 * 256;
@@ -800,16 +811,16 @@ struct HeadCall {
 
 static bool head_packs(const void* head, int head_fp32, long ldw, int H) { return head_fp32 || H % 8 || ldw % 8 || ((uintptr_t)head & 15); }
 
-// Boxes of 64 columns and 128 rows (an operand along its columns), 64 rows (one along its rows) or 32 (a warp's stores).
+// Boxes of 64 columns and 128 or 32 rows (an operand along its columns) or 64 rows (one along its rows).
 static int slab_map(CUtensorMap* m, const void* base, int slabs, uint64_t slab_rows, uint64_t rows, uint64_t cols, uint64_t pitch, int box_rows) {
   return make_tmap_3d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, slabs, rows, cols, slab_rows * pitch * 2, pitch * 2, box_rows, 64, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <bool A_MN, bool B_MN, class Job>
+template <int NT, bool A_MN, bool B_MN, class Job>
 static int launch_pair(const Job& job, const PairLoop& loop, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const HeadCall& c) {
-  cudaError_t e = allow_smem<head_gemm_kernel<A_MN, B_MN, Job>>(kPairSmem);
+  cudaError_t e = allow_smem<head_gemm_kernel<NT, A_MN, B_MN, Job>>(kPairSmem);
   if (e != cudaSuccess) return (int)e;
-  launch_pdl(head_gemm_kernel<A_MN, B_MN, Job>, dim3(2 * kPairClusters), dim3(kPairThreads), kPairSmem, c.st, job, loop, a, b, o, c.status);
+  launch_pdl(head_gemm_kernel<NT, A_MN, B_MN, Job>, dim3(2 * kPairClusters), dim3(kPairThreads), kPairSmem, c.st, job, loop, a, b, o, c.status);
   return (int)cudaGetLastError();
 }
 
@@ -842,7 +853,7 @@ static int front_rows(const HeadCall& c, const HeadPlan& p, size_t word_bytes) {
 static int head_front(const HeadCall& c, const HeadPlan& p) {
   const size_t word_bytes = p.big_bytes * (((size_t)c.rows.V + p.piece - 1) / p.piece);
   if (!c.rows.labels)
-    launch_pdl(head_targets_kernel, dim3(c.rows.R), dim3(128), 0, c.st, c.rows, p.nblk, (int*)(c.ws + p.sid), (float*)(c.ws + p.slp), (uint16_t*)(c.ws + p.off),
+    launch_pdl(head_targets_kernel, dim3(c.rows.R), dim3(128), 0, c.st, c.rows, p.span, p.nblk, (int*)(c.ws + p.sid), (float*)(c.ws + p.slp), (uint16_t*)(c.ws + p.off),
                (int*)(c.ws + p.flag), (double*)(c.ws + p.mass));
   return c.x_fp32 ? front_rows<float>(c, p, word_bytes) : front_rows<__nv_bfloat16>(c, p, word_bytes);
 }
@@ -869,7 +880,7 @@ static inline int exact_chunk(int H) { return H <= 256 ? 1 : H <= 640 ? 2 : 4; }
 constexpr int kExactChunk = 4;         // along rows or the vocabulary: gradients in fp32
 constexpr int kRoundedChunk = 32;      // where the result is rounded to bf16 (cut-off sums over 2048: 2e-6), or a gradient's logits are (2e-6 of z: 2^-15 of s)
 
-template <bool CAP>
+template <bool CAP, int C>
 static int head_score(const HeadCall& c, const HeadPlan& p, float* loss, float* stats) {
   int rc = head_front(c, p);
   if (rc) return rc;
@@ -877,26 +888,27 @@ static int head_score(const HeadCall& c, const HeadPlan& p, float* loss, float* 
   CUtensorMap xm, wm;
   rc = slab_map(&xm, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, 128);
   if (rc) return rc;
-  ScoreJob<CAP> job;
+  ScoreJob<CAP, C> job;
   job.count = count; job.ksteps = p.ksteps; job.tg = head_targets_of(c, p); job.live = live; job.rows_cap = p.rows_cap;
   job.part = (float2*)(c.ws + p.part); job.zt = (float*)(c.ws + p.zt); job.cap = c.softcap; job.inv_cap = CAP ? 1.f / c.softcap : 0.f;
   for (int v0 = 0; v0 < c.rows.V; v0 += p.piece) {
     job.v0 = v0;
     job.nv = c.rows.V - v0 < p.piece ? c.rows.V - v0 : p.piece;
-    if ((rc = head_rows_map(&wm, c, p, v0, job.nv, 128, true))) return rc;
-    if ((rc = launch_pair<false, false>(job, pair_loop(p.sx, p.sw, 2, exact_chunk(c.H)), xm, wm, xm, c))) return rc;
+    if ((rc = head_rows_map(&wm, c, p, v0, job.nv, C, true))) return rc;
+    if ((rc = launch_pair<2 * C, false, false>(job, pair_loop(p.sx, p.sw, 2, exact_chunk(c.H)), xm, wm, xm, c))) return rc;
   }
   launch_pdl(head_merge_kernel, dim3((c.rows.R + 31) / 32), dim3(1024), 0, c.st, c.rows, live, pos, count, p.rows_cap, p.nblk, (const float2*)job.part,
              (const float*)job.zt, job.tg.sid, job.tg.slp, loss, stats);
   return (int)cudaGetLastError();
 }
 
-template <bool CAP>
+template <bool CAP, int C>
 static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, const float* dloss, void* dx, void* dhead) {
   int rc = head_front(c, p);
   if (rc) return rc;
   const int *live = (const int*)(c.ws + p.live), *pos = (const int*)(c.ws + p.pos), *count = (const int*)(c.ws + p.count);
   const int R = c.rows.R, H = c.H;
+  GradJob<CAP, C> gj;
   CUtensorMap xk, xmn, wk, wmn, gk, gmn, gout, aout, hout;
   rc = slab_map(&xk, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, 128);
   if (!rc) rc = slab_map(&xmn, c.ws + p.x, p.sx, p.rows_cap, p.rows_cap, p.Hp, p.Hp, 64);
@@ -905,9 +917,10 @@ static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, c
   if (!rc && dx)
     rc = make_tmap_3d(&aout, c.ws + p.acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.splits, p.rows_cap, p.Hp, 4ull * p.rows_cap * p.Hp, 4ull * p.Hp, 32, 32,
                       CU_TENSOR_MAP_SWIZZLE_128B);
-  if (!rc) rc = slab_map(&gout, c.ws + p.G, p.sg, p.rows_cap, p.rows_cap, p.piece, p.piece, 32);
+  if (!rc)
+    rc = make_tmap_3d(&gout, c.ws + p.G, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.sg, p.rows_cap, p.piece, 2ull * p.rows_cap * p.piece, 2ull * p.piece, 32,
+                      gj.kBox, gj.kBox == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
   if (rc) return rc;
-  GradJob<CAP> gj;
   gj.count = count; gj.ksteps = p.ksteps; gj.tg = head_targets_of(c, p); gj.live = live; 
   gj.slabs = p.sg; gj.cap = c.softcap; gj.inv_cap = CAP ? 1.f / c.softcap : 0.f;
   gj.in = RowInputs{stats, dloss, c.rows.tail, (const double*)(c.ws + p.mass), R, c.rows.labels != nullptr};
@@ -917,20 +930,20 @@ static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, c
     const int nv = c.rows.V - v0 < p.piece ? c.rows.V - v0 : p.piece;
     gj.v0 = v0;
     gj.nv = nv;
-    if ((rc = head_rows_map(&wk, c, p, v0, nv, 128, true))) return rc;
+    if ((rc = head_rows_map(&wk, c, p, v0, nv, C, true))) return rc;
     LargeBlocks big{nullptr, nullptr, p.row_words, p.col_words};
     if (p.big_bytes) {
       big.of_rows = (uint32_t*)(c.ws + p.big + p.big_bytes * (v0 / p.piece));
       big.of_cols = big.of_rows + p.rows_cap / 256 * p.row_words;
     }
     gj.big = xj.big = big;
-    if ((rc = launch_pair<false, false>(gj, pair_loop(p.sx, p.sw, 2, exact ? exact_chunk(c.H) : kRoundedChunk), xk, wk, gout, c))) return rc;
+    if ((rc = launch_pair<2 * C, false, false>(gj, pair_loop(p.sx, p.sw, 2, exact ? exact_chunk(c.H) : kRoundedChunk), xk, wk, gout, c))) return rc;
     if (dx) {
       if ((rc = head_rows_map(&wmn, c, p, v0, nv, 64, false))) return rc;
       xj.ksteps = (nv + 63) / 64;
       xj.first = v0 == 0;
       const PairLoop loop = c.x_fp32 ? pair_loop(p.sg, p.sw, 2, kExactChunk) : pair_loop(p.sg, p.sw, exact ? 1 : 0, kRoundedChunk);
-      if ((rc = launch_pair<false, true>(xj, loop, gk, wmn, aout, c))) return rc;
+      if ((rc = launch_pair<256, false, true>(xj, loop, gk, wmn, aout, c))) return rc;
     }
     if (dhead) {
       const size_t es = c.head_fp32 ? 4 : 2;
@@ -942,10 +955,10 @@ static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, c
       if (!boxes) hout = gmn;
       if (c.head_fp32) {
         const DheadJob<float> job{count, nv, H, (float*)out, boxes, big};
-        rc = launch_pair<true, true>(job, pair_loop(p.sg, p.sx, 2, kExactChunk), gmn, xmn, hout, c);
+        rc = launch_pair<256, true, true>(job, pair_loop(p.sg, p.sx, 2, kExactChunk), gmn, xmn, hout, c);
       } else {
         const DheadJob<__nv_bfloat16> job{count, nv, H, (__nv_bfloat16*)out, boxes, big};
-        rc = launch_pair<true, true>(job, pair_loop(p.sg, p.sx, exact ? 1 : 0, kRoundedChunk), gmn, xmn, hout, c);
+        rc = launch_pair<256, true, true>(job, pair_loop(p.sg, p.sx, exact ? 1 : 0, kRoundedChunk), gmn, xmn, hout, c);
       }
       if (rc) return rc;
     }
@@ -980,7 +993,8 @@ int ve_head_loss(const void* x, int x_fp32, long ldx, const void* head, int head
   if ((size_t)ws_bytes < p.bytes) return cudaErrorInvalidValue;
   const HeadCall c{x, x_fp32, ldx, head, head_fp32, ldw, {labels, label_bytes, (const int*)ids, (const float*)logp, (const float*)tail, K, R, V}, H, softcap,
                    (uint8_t*)ws, (int*)status, st};
-  return softcap > 0.f ? head_score<true>(c, p, (float*)loss, (float*)stats) : head_score<false>(c, p, (float*)loss, (float*)stats);
+  if (p.span == 32) return softcap > 0.f ? head_score<true, 32>(c, p, (float*)loss, (float*)stats) : head_score<false, 32>(c, p, (float*)loss, (float*)stats);
+  return softcap > 0.f ? head_score<true, 128>(c, p, (float*)loss, (float*)stats) : head_score<false, 128>(c, p, (float*)loss, (float*)stats);
 }
 
 // The gradients for dloss fp32 [R]: dx [R, H] in the states' type and dhead [V, H] in the head's, either may be null.
@@ -993,8 +1007,9 @@ int ve_head_loss_grad(const void* x, int x_fp32, long ldx, const void* head, int
   if ((size_t)ws_bytes < p.bytes) return cudaErrorInvalidValue;
   const HeadCall c{x, x_fp32, ldx, head, head_fp32, ldw, {labels, label_bytes, (const int*)ids, (const float*)logp, (const float*)tail, K, R, V}, H, softcap,
                    (uint8_t*)ws, (int*)status, st};
-  return softcap > 0.f ? head_grad<true>(c, p, (const float*)stats, (const float*)dloss, dx, dhead)
-                       : head_grad<false>(c, p, (const float*)stats, (const float*)dloss, dx, dhead);
+  const float *s = (const float*)stats, *g = (const float*)dloss;
+  if (p.span == 32) return softcap > 0.f ? head_grad<true, 32>(c, p, s, g, dx, dhead) : head_grad<false, 32>(c, p, s, g, dx, dhead);
+  return softcap > 0.f ? head_grad<true, 128>(c, p, s, g, dx, dhead) : head_grad<false, 128>(c, p, s, g, dx, dhead);
 }
 
 }  // extern "C"

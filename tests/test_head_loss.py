@@ -363,9 +363,12 @@ def test_pieces_of_the_vocabulary():
 @pytest.mark.gpu
 @pytest.mark.parametrize("topk", [0, 3])
 def test_many_rows(topk):
-    """More rows than one block looks through for those that count."""
+    """More rows (or ids) than one block looks through for those that count."""
     a = make(9001, 32, 300, topk, seed=5, left_out=0.3, device="cuda")
     hold(run(*a), *a, 0.0)
+    if topk:
+        a = make(400, 32, 700, 200, seed=6, left_out=0.7, device="cuda")
+        hold(run(*a), *a, 0.0)
 
 
 @pytest.mark.gpu

@@ -29,7 +29,7 @@ namespace ve {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLogFloor = -27.631021115928547f;       // log 1e-12: the least share of "any other token"
 constexpr int kMaxTopk = 1024;
-constexpr int kFrontRows = 4096;       // rows that every block of head_front_kernel looks through
+constexpr int kFrontRows = 4096, kFrontIds = 1 << 16;       // rows, or a teacher's ids, that every block of head_front_kernel looks through
 
 VE_DEVINL float neg_inf() { return __int_as_float(0xff800000); }
 
@@ -43,13 +43,19 @@ struct HeadRows {
 };
 
 // Divergence: the teacher's tokens of a row in ascending order, with their places: sid / slp [R, K] (padding behind, as INT_MAX), and at
-// off[r, b] the first one at or behind column span * b; flag[r]: the row counts; mass[r] = sum_k a_k. One block a row, counting ranks: K is small.
-__global__ void __launch_bounds__(128) head_targets_kernel(const HeadRows p, int span, int nblk, int* sid, float* slp, uint16_t* off, int* flag, double* mass) {
+// off[r, b] the first one at or behind column span * b; flag[r]: the row counts; mass[r] = sum_k a_k.
+struct TeacherRows {
+  int span, nblk;
+  int* sid;
+  float* slp;
+  uint16_t* off;
+  int* flag;
+  double* mass;
+};
+// One block (a multiple of 32 threads, at most 256) a row, counting ranks: K is small.
+VE_DEVINL void sort_teacher(const HeadRows& p, const TeacherRows& o, int r) {
   __shared__ int id[kMaxTopk], srt[kMaxTopk];
-  __shared__ double part[4];
-  grid_dep_launch();
-  grid_dep_wait();
-  const int r = blockIdx.x;
+  __shared__ double part[8];
   int any = 0;
   double sum = 0.0;
   for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
@@ -58,12 +64,14 @@ __global__ void __launch_bounds__(128) head_targets_kernel(const HeadRows p, int
     any |= v >= 0;
     if (v >= 0) sum += exp((double)p.logp[(size_t)r * p.K + k]);
   }
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
   any = __syncthreads_or(any);
   if (threadIdx.x == 0) {
-    flag[r] = any;
-    mass[r] = part[0] + part[1] + part[2] + part[3];
+    double m = 0.0;
+    for (int w = 0; w < (int)blockDim.x >> 5; ++w) m += part[w];
+    o.flag[r] = any;
+    o.mass[r] = m;
   }
   if (!any) return;                                   // (uniform)
   for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
@@ -71,18 +79,23 @@ __global__ void __launch_bounds__(128) head_targets_kernel(const HeadRows p, int
     int at = 0;
     for (int j = 0; j < p.K; ++j) at += id[j] < v || (id[j] == v && j < k);
     srt[at] = v;
-    sid[(size_t)r * p.K + at] = v;
-    slp[(size_t)r * p.K + at] = v == INT_MAX ? neg_inf() : p.logp[(size_t)r * p.K + k];
+    o.sid[(size_t)r * p.K + at] = v;
+    o.slp[(size_t)r * p.K + at] = v == INT_MAX ? neg_inf() : p.logp[(size_t)r * p.K + k];
   }
   __syncthreads();
-  for (int b = threadIdx.x; b <= nblk; b += blockDim.x) {
+  for (int b = threadIdx.x; b <= o.nblk; b += blockDim.x) {
     int lo = 0, hi = p.K;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (srt[mid] < b * span) lo = mid + 1; else hi = mid;
+      if (srt[mid] < b * o.span) lo = mid + 1; else hi = mid;
     }
-    off[(size_t)r * (nblk + 1) + b] = (uint16_t)lo;
+    o.off[(size_t)r * (o.nblk + 1) + b] = (uint16_t)lo;
   }
+}
+__global__ void __launch_bounds__(128) head_targets_kernel(const HeadRows p, const TeacherRows o) {
+  grid_dep_launch();
+  grid_dep_wait();
+  sort_teacher(p, o, blockIdx.x);
 }
 
 VE_DEVINL long label_of(const HeadRows& p, int r) {
@@ -184,11 +197,11 @@ VE_DEVINL uint32_t split_pair(float& lo, float& hi) {
   return b;
 }
 
-// A row (null: zeros) into its slabs, by a warp.
+// Columns [c0, c1) of a row (null: zeros) into its slabs, by a warp.
 template <typename T>
-VE_DEVINL void pack_row(const T* row, int H, int Hp, int slabs, size_t slab, __nv_bfloat16* dst) {
+VE_DEVINL void pack_row(const T* row, int c0, int c1, int H, int slabs, size_t slab, __nv_bfloat16* dst) {
   const bool vec = !(reinterpret_cast<uintptr_t>(row) & 15);
-  for (int c = (threadIdx.x & 31) * 8; c < Hp; c += 256) {
+  for (int c = c0 + (threadIdx.x & 31) * 8; c < c1; c += 256) {
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (row) load8(row, c, H, vec, v);
     for (int s = 0; s < slabs; ++s) {
@@ -200,33 +213,56 @@ VE_DEVINL void pack_row(const T* row, int H, int Hp, int slabs, size_t slab, __n
   }
 }
 
-// Rows of a matrix as bf16 slabs [slabs][rows of a slab][Hp], zeros behind column H. With `live`: the gathered rows, and zeros behind the last
-// one to the end of its tile of 256 (the products along rows read them).
+struct PackedRows {             // a matrix and its slabs [slabs][rows of a slab][Hp], zeros behind column H
+  const void* src;
+  long ld;
+  int fp32, H, Hp, slabs;
+  size_t slab;
+  __nv_bfloat16* dst;
+  VE_DEVINL int chunks() const { return (Hp + 255) >> 8; }
+  VE_DEVINL void put(int row, bool there, int to, int chunk) const {        // row -> row `to` of the slabs, 256 columns, by a warp
+    __nv_bfloat16* d = dst + (size_t)to * Hp;
+    const int c0 = chunk * 256, c1 = min(Hp, c0 + 256);
+    if (fp32) pack_row(there ? (const float*)src + row * ld : nullptr, c0, c1, H, slabs, slab, d);
+    else pack_row(there ? (const __nv_bfloat16*)src + row * ld : nullptr, c0, c1, H, slabs, slab, d);
+  }
+};
+
+// A warp a row. With `live`: the gathered rows, and zeros behind the last one to the end of its tile of 256 (the products along rows read them).
 template <typename T>
-__global__ void __launch_bounds__(256) head_pack_kernel(const T* src, long ld, const int* live, const int* count, int rows, int H, int Hp, int slabs,
-                                                        size_t slab, __nv_bfloat16* dst) {
+__global__ void __launch_bounds__(256) head_pack_kernel(const PackedRows m, const int* live, const int* count, int rows) {
   grid_dep_launch();
   grid_dep_wait();
   const int n = live ? *count : rows, all = live ? (n + 255) / 256 * 256 : rows;
   for (int r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; r < all; r += gridDim.x * blockDim.x >> 5)
-    pack_row(r < n ? src + (live ? live[r] : r) * ld : (const T*)nullptr, H, Hp, slabs, slab, dst + (size_t)r * Hp);
+    pack_row(r < n ? (const T*)m.src + (live ? live[r] : r) * m.ld : (const T*)nullptr, 0, m.Hp, m.H, m.slabs, m.slab, m.dst + (size_t)r * m.Hp);
 }
 
-// head_rows_kernel and head_pack_kernel of few rows in one launch: every block finds all the rows that count and packs its share of them; the words of
-// large blocks become zero on the way.
-template <typename T>
-__global__ void __launch_bounds__(256) head_front_kernel(const HeadRows p, const int* flag, int* live, int* pos, int* count, const T* src, long ld, int H, int Hp,
-                                                         int slabs, size_t slab, __nv_bfloat16* dst, uint4* words, size_t nwords, const DxPlan dx) {
+// All of that for few rows in one launch: `teachers` blocks sort a teacher's row each; every other block finds all the rows that count and packs its
+// share of them, and of the head where all of it is packed at once; the words of large blocks become zero on the way.
+__global__ void __launch_bounds__(256) head_front_kernel(const HeadRows p, const TeacherRows teacher, int teachers, int* live, int* pos, int* count,
+                                                         const PackedRows x, const PackedRows head, int head_rows, uint4* words, size_t nwords, const DxPlan dx) {
   __shared__ int row_of[kFrontRows], part[8];
   grid_dep_launch();
   grid_dep_wait();
+  if ((int)blockIdx.x < teachers) {
+    sort_teacher(p, teacher, blockIdx.x);
+    return;
+  }
+  const int block = blockIdx.x - teachers, blocks = gridDim.x - teachers;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const size_t first = blockIdx.x * (size_t)blockDim.x + threadIdx.x, step = (size_t)gridDim.x * blockDim.x;
-  for (size_t i = first; i < nwords; i += step) words[i] = make_uint4(0u, 0u, 0u, 0u);
+  for (size_t i = block * (size_t)blockDim.x + threadIdx.x; i < nwords; i += (size_t)blocks * blockDim.x) words[i] = make_uint4(0u, 0u, 0u, 0u);
   int n = 0;
   for (int r0 = 0; r0 < p.R; r0 += 256) {
     const int r = r0 + threadIdx.x;
-    const bool on = r < p.R && (p.labels ? label_of(p, r) >= 0 : flag[r] != 0);
+    bool on = false;
+    if (r < p.R) {
+      if (p.labels) on = label_of(p, r) >= 0;
+      else
+        for (int k = 0; k < p.K && !on; k += 8)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) on |= k + e < p.K && p.ids[(size_t)r * p.K + k + e] >= 0;
+    }
     const unsigned mask = __ballot_sync(0xffffffffu, on);
     if (lane == 0) part[warp] = __popc(mask);
     __syncthreads();
@@ -237,19 +273,24 @@ __global__ void __launch_bounds__(256) head_front_kernel(const HeadRows p, const
       n += part[w];
     }
     if (on) row_of[at] = r;
-    if (blockIdx.x == 0) {
+    if (block == 0) {
       if (r < p.R) pos[r] = on ? at : -1;
       if (on) live[at] = r;
     }
     __syncthreads();
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
+  if (block == 0 && threadIdx.x == 0) {
     count[0] = n;
     count[1] = dx_splits(n, dx);
   }
-  const int all = (n + 255) / 256 * 256;
-  for (int r = (int)(first >> 5); r < all; r += (int)(step >> 5))
-    pack_row(r < n ? src + row_of[r] * ld : (const T*)nullptr, H, Hp, slabs, slab, dst + (size_t)r * Hp);
+  const int all = (n + 255) / 256 * 256, chunks = x.chunks();
+  const size_t own = (size_t)all * chunks, units = own + (size_t)head_rows * chunks;
+  for (size_t u = (size_t)block * 8 + warp; u < units; u += (size_t)blocks * 8) {
+    const size_t v = u < own ? u : u - own;
+    const int r = (int)(v / chunks), c = (int)(v - (size_t)r * chunks);
+    if (u < own) x.put(r < n ? row_of[r] : 0, r < n, r, c);
+    else head.put(r, true, r, c);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ jobs of the paired GEMM
@@ -743,6 +784,7 @@ struct HeadPlan {             // sizes and places in the workspace
   int Hp, sx, sw, sg;         // padded width; slabs of the states, the head, dz
   int rows_cap, ksteps;
   int span, nblk;             // columns of a thread of the logits' tiles, and blocks of so many in the vocabulary
+  bool few;                   // rows that one launch looks through and packs
   bool pack_head;             // the head's rows go through slabs of their own, a piece at a time
   int piece;                  // vocabulary rows at a time
   int splits, pairs;          // most ranges of a piece that dx is summed over; products of slabs
@@ -769,6 +811,7 @@ static HeadPlan head_plan(bool grads, bool want_dx, int x_fp32, int head_fp32, b
   p.nblk = (V + p.span - 1) / p.span;
   p.ksteps = (H + 63) / 64;
   p.pack_head = pack_head;
+  p.few = R <= kFrontRows && (!kl || (size_t)R * K <= kFrontIds);
   size_t piece = ((size_t)V + 255) / 256 * 256;
   if (pack_head) { const size_t most = (512ull << 20) / ((size_t)p.sw * p.Hp * 2) / 256 * 256; piece = piece < most ? piece : (most ? most : 256); }
   if (grads) { const size_t most = (256ull << 20) / ((size_t)p.sg * p.rows_cap * 2) / 256 * 256; piece = piece < most ? piece : (most ? most : 256); }
@@ -824,48 +867,50 @@ static int launch_pair(const Job& job, const PairLoop& loop, const CUtensorMap& 
   return (int)cudaGetLastError();
 }
 
-template <typename T>
-static void pack_rows(const void* src, long ld, const int* live, const int* count, int rows, const HeadCall& c, const HeadPlan& p, int slabs, size_t slab, void* dst) {
-  launch_pdl(head_pack_kernel<T>, dim3(blocks_of((size_t)rows, 8)), dim3(256), 0, c.st, (const T*)src, ld, live, count, rows, c.H, p.Hp, slabs, slab,
-             (__nv_bfloat16*)dst);
+static PackedRows states_of(const HeadCall& c, const HeadPlan& p) {
+  return PackedRows{c.x, c.ldx, c.x_fp32, c.H, p.Hp, p.sx, (size_t)p.rows_cap * p.Hp, (__nv_bfloat16*)(c.ws + p.x)};
+}
+static PackedRows head_of(const HeadCall& c, const HeadPlan& p, int v0) {
+  const size_t es = c.head_fp32 ? 4 : 2;
+  return PackedRows{(const uint8_t*)c.head + (size_t)v0 * c.ldw * es, c.ldw, c.head_fp32, c.H, p.Hp, p.sw, (size_t)p.piece * p.Hp, (__nv_bfloat16*)(c.ws + p.head)};
+}
+// (a large head is packed by a launch of its own, whose blocks have nothing else to do: 100 MB take 33 us there and 40 in front)
+static bool head_in_front(const HeadCall& c, const HeadPlan& p) { return p.pack_head && p.few && p.piece >= c.rows.V && (size_t)c.rows.V * p.Hp <= 4u << 20; }
+static int pack_blocks(const HeadPlan& p, size_t rows) { return blocks_of(rows * ((p.Hp + 255) / 256), 8); }
+static void pack_rows(const PackedRows& m, const int* live, const int* count, int rows, cudaStream_t st) {
+  const dim3 grid(blocks_of((size_t)rows, 8));
+  if (m.fp32) launch_pdl(head_pack_kernel<float>, grid, dim3(256), 0, st, m, live, count, rows);
+  else launch_pdl(head_pack_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, m, live, count, rows);
 }
 
-template <typename T>
-static int front_rows(const HeadCall& c, const HeadPlan& p, size_t word_bytes) {
+// The rows that count, their targets and their states; zeros in the words of large blocks; a head that is packed at once.
+static int head_front(const HeadCall& c, const HeadPlan& p) {
+  const size_t word_bytes = p.big_bytes * (((size_t)c.rows.V + p.piece - 1) / p.piece);
   int *live = (int*)(c.ws + p.live), *pos = (int*)(c.ws + p.pos), *count = (int*)(c.ws + p.count), *flag = (int*)(c.ws + p.flag);
-  const size_t slab = (size_t)p.rows_cap * p.Hp;
+  const TeacherRows teacher{p.span, p.nblk, (int*)(c.ws + p.sid), (float*)(c.ws + p.slp), (uint16_t*)(c.ws + p.off), flag, (double*)(c.ws + p.mass)};
   const DxPlan dx{(c.H + 255) / 256, p.piece / 64, p.pairs, p.acc ? p.splits : 0};
-  if (c.rows.R <= kFrontRows) {
-    launch_pdl(head_front_kernel<T>, dim3(blocks_of((size_t)p.rows_cap, 8)), dim3(256), 0, c.st, c.rows, (const int*)flag, live, pos, count,
-               (const T*)c.x, c.ldx, c.H, p.Hp, p.sx, slab, (__nv_bfloat16*)(c.ws + p.x), (uint4*)(c.ws + p.big), word_bytes / 16, dx);
-    return 0;
+  const int R = c.rows.R, teachers = c.rows.labels ? 0 : R;
+  if (p.few) {
+    const int heads = head_in_front(c, p) ? c.rows.V : 0;
+    launch_pdl(head_front_kernel, dim3(teachers + pack_blocks(p, (size_t)p.rows_cap + heads)), dim3(256), 0, c.st, c.rows, teacher, teachers, live, pos, count,
+               states_of(c, p), head_of(c, p, 0), heads, (uint4*)(c.ws + p.big), word_bytes / 16, dx);
+    return (int)cudaGetLastError();
   }
   if (word_bytes) {
     const cudaError_t e = cudaMemsetAsync(c.ws + p.big, 0, word_bytes, c.st);
     if (e != cudaSuccess) return (int)e;
   }
+  if (teachers) launch_pdl(head_targets_kernel, dim3(R), dim3(128), 0, c.st, c.rows, teacher);
   launch_pdl(head_rows_kernel, dim3(1), dim3(1024), 0, c.st, c.rows, (const int*)flag, live, pos, count, dx);
-  pack_rows<T>(c.x, c.ldx, live, count, p.rows_cap, c, p, p.sx, slab, c.ws + p.x);
-  return 0;
-}
-
-// The rows that count, their targets and their states; zeros in the words of large blocks.
-static int head_front(const HeadCall& c, const HeadPlan& p) {
-  const size_t word_bytes = p.big_bytes * (((size_t)c.rows.V + p.piece - 1) / p.piece);
-  if (!c.rows.labels)
-    launch_pdl(head_targets_kernel, dim3(c.rows.R), dim3(128), 0, c.st, c.rows, p.span, p.nblk, (int*)(c.ws + p.sid), (float*)(c.ws + p.slp), (uint16_t*)(c.ws + p.off),
-               (int*)(c.ws + p.flag), (double*)(c.ws + p.mass));
-  return c.x_fp32 ? front_rows<float>(c, p, word_bytes) : front_rows<__nv_bfloat16>(c, p, word_bytes);
+  pack_rows(states_of(c, p), live, count, R, c.st);
+  return (int)cudaGetLastError();
 }
 
 // The head's rows [v0, v0 + nv) as an operand: in place, or packed.
 static int head_rows_map(CUtensorMap* m, const HeadCall& c, const HeadPlan& p, int v0, int nv, int box_rows, bool pack) {
   if (!p.pack_head) return slab_map(m, (const __nv_bfloat16*)c.head + (size_t)v0 * c.ldw, 1, nv, nv, c.H, c.ldw, box_rows);
-  if (pack) {
-    const size_t slab = (size_t)p.piece * p.Hp;
-    if (c.head_fp32) pack_rows<float>((const float*)c.head + (size_t)v0 * c.ldw, c.ldw, nullptr, nullptr, nv, c, p, p.sw, slab, c.ws + p.head);
-    else pack_rows<__nv_bfloat16>((const __nv_bfloat16*)c.head + (size_t)v0 * c.ldw, c.ldw, nullptr, nullptr, nv, c, p, p.sw, slab, c.ws + p.head);
-  }
+  if (pack && !head_in_front(c, p))
+    pack_rows(head_of(c, p, v0), nullptr, nullptr, nv, c.st);
   return slab_map(m, c.ws + p.head, p.sw, p.piece, nv, p.Hp, p.Hp, box_rows);
 }
 

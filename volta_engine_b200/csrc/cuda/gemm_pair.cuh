@@ -24,14 +24,14 @@ namespace ve {
 // A tile is 256 rows x NT columns, 256 or, for logits of few tiles, 64: four times the pairs have work, and a thread finishes 32 columns in place of 128.
 template <int NT>
 struct PairShape {
-  static constexpr int kA = 128 * 128, kB = NT / 2 * 128, kStage = kA + kB;        // bytes of a step in a CTA: 128 rows x 64 of A, NT / 2 of B
-  static constexpr int kStages = NT == 256 ? 6 : 9;
+  static constexpr int kA = 128 * 128, kB = NT / 2 * 128;                           // bytes of a step and slab in a CTA: 128 rows x 64 of A, NT / 2 of B
   static constexpr int kCols = NT / 2;                                              // of a thread
 };
-constexpr int kPairRing = 6 * PairShape<256>::kStage;
+constexpr int kPairRing = 6 * (PairShape<256>::kA + PairShape<256>::kB);
+constexpr int kPairStages = kPairRing / (PairShape<64>::kA + PairShape<64>::kB);    // most steps in the ring
 constexpr int kPairStaging = 8 * 4096;                     // behind the ring: a box of each summing warp's stores
 constexpr int kPairSmem = kPairRing + kPairStaging + 1024;
-static_assert(kPairSmem <= 227 * 1024 - 512 && 9 * PairShape<64>::kStage <= kPairRing, "shared memory (beside the barriers)");
+static_assert(kPairSmem <= 227 * 1024 - 512, "shared memory (beside the barriers)");
 constexpr int kPairClusters = 74, kPairThreads = 384;
 
 VE_DEVINL uint32_t cluster_rank() {
@@ -109,18 +109,20 @@ VE_DEVINL void tc_mma_f16_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, 
 // What one tile covers. Rows and columns count from the operands' own origins; steps of 64 along K.
 struct PairTile {
   int m0, n0;                 // first row / column of the tile
-  int k0, ksteps;             // first step and number of steps (of each pair of slabs)
+  int k0, ksteps;             // first step and number of steps
   int split;
 };
 
+// A step brings `na` slabs of A and `nb` of B and multiplies the pairs of them that are listed.
 struct PairLoop {
-  int pairs;                  // pairs of slabs
+  int na, nb;
+  int pairs;
   uint32_t a_slab, b_slab;    // four bits each
   int chunk;                  // steps that a sum stays in tensor memory
 };
 
 // Steps that are worth a second look: bit k of a tile's words asks for step k once more, with the second slab of A (what the first one's rounding
-// left) and the first of B.
+// left) in place of the first. (Loops of one slab each.)
 VE_DEVINL uint32_t step_bits(const uint32_t* words, int w, int k0, int k1) {        // word w, cut to steps [k0, k1)
   uint32_t b = words[w];
   if (w == k0 >> 5) b &= 0xffffffffu << (k0 & 31);
@@ -134,13 +136,15 @@ VE_DEVINL int step_count(const uint32_t* words, int k0, int k1) {
   return n;
 }
 
-// The pairs (i, j) of `sa` x `sb` slabs with i + j <= order, the small ones first.
+// The pairs (i, j) of `sa` x `sb` slabs with i + j <= order, the small ones first: what is cut off a sum is cut by its size, so a step that is a piece by
+// itself loses as little as one of its first slabs alone. All pairs of a step work on one load of it (6 of 3 x 3 slabs: half of what the pairs one
+// after another would bring).
 static inline PairLoop pair_loop(int sa, int sb, int order, int chunk) {
-  PairLoop l{0, 0, 0, chunk};
+  PairLoop l{sa < order + 1 ? sa : order + 1, sb < order + 1 ? sb : order + 1, 0, 0, 0, chunk};
   for (int o = order; o >= 0; --o)
-    for (int i = 0; i < sa; ++i) {
+    for (int i = 0; i < l.na; ++i) {
       const int j = o - i;
-      if (j < 0 || j >= sb) continue;
+      if (j < 0 || j >= l.nb) continue;
       l.a_slab |= (uint32_t)i << (4 * l.pairs);
       l.b_slab |= (uint32_t)j << (4 * l.pairs);
       ++l.pairs;
@@ -153,20 +157,22 @@ static inline PairLoop pair_loop(int sa, int sb, int order, int chunk) {
 // sums[NT / 2], omap, 4 KB of shared memory of the warp).
 // A_MN / B_MN: the operand is MN-major.
 // wait(): the point behind which other kernels' results are read.
-template <int NT, bool A_MN, bool B_MN, class Job, class Wait>
+// ONE: one slab of either operand, known to the compiler (3 to 4 % of a step's time).
+template <int NT, bool A_MN, bool B_MN, bool ONE, class Job, class Wait>
 VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap* amap, const CUtensorMap* bmap, const CUtensorMap* omap, int* status, Wait wait) {
   static_assert(NT == 256 || !B_MN, "64 columns of an MN-major operand are one box of a CTA");
   using S = PairShape<NT>;
-  constexpr int kStages = S::kStages, kCols = S::kCols;
+  constexpr int kCols = S::kCols;
+  const int na = ONE ? 1 : loop.na, nb = ONE ? 1 : loop.nb, stage_bytes = na * S::kA + nb * S::kB, stages = kPairRing / stage_bytes;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+  __shared__ uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_holder;
   __shared__ int s_fail;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank(), cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < kPairStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 16); }
     s_fail = 0;
     mbar_fence_init();
@@ -185,68 +191,74 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
     if (warp == 0 && elect_one()) {
       prefetch_tmap(amap);
       prefetch_tmap(bmap);
-      int it = 0;
+      int s = 0, phase = 1;
       bool ok = true;
       for (int t = cluster; t < ntiles && ok; t += clusters) {
         const PairTile tl = job.tile(t);
         const int am = tl.m0 + rank * 128, bn = tl.n0 + rank * kCols;
-        auto load = [&](int k, int sa, int sb) {
-          const int s = it % kStages;
-          if (!mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1)) return false;
-          ++it;
-          uint8_t* st = smem + s * S::kStage;
-          if (rank == 0) mbar_expect_tx(&full[s], 2 * S::kStage);
+        auto load = [&](int k, int a0) {                    // a step of slabs a0, a0 + 1, .. of A
+          if (!mbar_wait(&empty[s], phase)) return false;
+          uint8_t* st = smem + s * stage_bytes;
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * stage_bytes);
           const uint32_t bar = first_cta_addr(&full[s]);
           const int kk = k * 64;
-          if (A_MN) {
-            tma_load_3d_pair(st, amap, bar, am, kk, sa);
-            tma_load_3d_pair(st + S::kA / 2, amap, bar, am + 64, kk, sa);
-          } else {
-            tma_load_3d_pair(st, amap, bar, kk, am, sa);
+          for (int i = 0; i < na; ++i, st += S::kA) {
+            if (A_MN) {
+              tma_load_3d_pair(st, amap, bar, am, kk, a0 + i);
+              tma_load_3d_pair(st + S::kA / 2, amap, bar, am + 64, kk, a0 + i);
+            } else {
+              tma_load_3d_pair(st, amap, bar, kk, am, a0 + i);
+            }
           }
-          if (B_MN) {
-            tma_load_3d_pair(st + S::kA, bmap, bar, bn, kk, sb);
-            tma_load_3d_pair(st + S::kA + S::kB / 2, bmap, bar, bn + 64, kk, sb);
-          } else {
-            tma_load_3d_pair(st + S::kA, bmap, bar, kk, bn, sb);
+          for (int j = 0; j < nb; ++j, st += S::kB) {
+            if (B_MN) {
+              tma_load_3d_pair(st, bmap, bar, bn, kk, j);
+              tma_load_3d_pair(st + S::kB / 2, bmap, bar, bn + 64, kk, j);
+            } else {
+              tma_load_3d_pair(st, bmap, bar, kk, bn, j);
+            }
           }
+          if (++s == stages) { s = 0; phase ^= 1; }
           return true;
         };
-        for (int p = 0; p < loop.pairs && ok; ++p)
-          for (int k = 0; k < tl.ksteps && ok; ++k) ok = load(tl.k0 + k, (loop.a_slab >> (4 * p)) & 15, (loop.b_slab >> (4 * p)) & 15);
+        for (int k = 0; k < tl.ksteps && ok; ++k) ok = load(tl.k0 + k, 0);
         const uint32_t* words = job.again(tl);
         const int k1 = tl.k0 + tl.ksteps;
         if (words)
           for (int w = tl.k0 >> 5; w * 32 < k1 && ok; ++w)
-            for (uint32_t bits = step_bits(words, w, tl.k0, k1); bits && ok; bits &= bits - 1) ok = load(w * 32 + __ffs(bits) - 1, 1, 0);
+            for (uint32_t bits = step_bits(words, w, tl.k0, k1); bits && ok; bits &= bits - 1) ok = load(w * 32 + __ffs(bits) - 1, 1);
       }
       if (!ok) atomicExch(&s_fail, 1);
     } else if (warp == 1 && rank == 0 && elect_one()) {
       constexpr uint32_t idesc = make_idesc_f16(1, 1, 256, NT) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
-      int it = 0, piece = 0;
+      int s = 0, phase = 0, piece = 0;
       bool ok = true;
       for (int t = cluster; t < ntiles && ok; t += clusters) {
         const PairTile tl = job.tile(t);
-        const int total = tl.ksteps * loop.pairs + step_count(job.again(tl), tl.k0, tl.k0 + tl.ksteps);
+        const int total = tl.ksteps + step_count(job.again(tl), tl.k0, tl.k0 + tl.ksteps);
         for (int i = 0; i < total && ok; ++piece) {
           const int buf = piece & 1;
           ok = mbar_wait(&acc_empty[buf], ((piece >> 1) & 1) ^ 1);
           if (!ok) break;
           tc_fence_after();
           const int end = min(total, i + loop.chunk);
-          for (bool first = true; i < end; ++i, ++it, first = false) {
-            const int s = it % kStages;
-            ok = mbar_wait(&full[s], (it / kStages) & 1);
+          for (uint32_t add = 0; i < end; ++i) {
+            ok = mbar_wait(&full[s], phase);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t a = smem_u32(smem + s * S::kStage), b = a + S::kA;
+            const uint32_t st = smem_u32(smem + s * stage_bytes), bs = st + na * S::kA;
+            for (int p = 0; p < (ONE ? 1 : loop.pairs); ++p) {
+              const uint32_t a = ONE ? st : st + ((loop.a_slab >> (4 * p)) & 15) * S::kA, b = ONE ? bs : bs + ((loop.b_slab >> (4 * p)) & 15) * S::kB;
 #pragma unroll
-            for (int kb = 0; kb < 4; ++kb) {
-              const uint64_t ad = A_MN ? make_desc_sw128_mn(a + kb * 2048, S::kA / 2, 1024) : make_desc_sw128(a) + kb * 2;
-              const uint64_t bd = B_MN ? make_desc_sw128_mn(b + kb * 2048, S::kB / 2, 1024) : make_desc_sw128(b) + kb * 2;
-              tc_mma_f16_pair(tmem_base + buf * NT, ad, bd, idesc, (first && kb == 0) ? 0u : 1u);
+              for (int kb = 0; kb < 4; ++kb) {
+                const uint64_t ad = A_MN ? make_desc_sw128_mn(a + kb * 2048, S::kA / 2, 1024) : make_desc_sw128(a) + kb * 2;
+                const uint64_t bd = B_MN ? make_desc_sw128_mn(b + kb * 2048, S::kB / 2, 1024) : make_desc_sw128(b) + kb * 2;
+                tc_mma_f16_pair(tmem_base + buf * NT, ad, bd, idesc, add);
+                add = 1;
+              }
             }
             tc_commit_pair(&empty[s]);
+            if (++s == stages) { s = 0; phase ^= 1; }
           }
           if (ok) tc_commit_pair(&acc_full[buf]);
         }
@@ -264,7 +276,7 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
     if (cluster < ntiles) row = begin(cluster);
     for (int t = cluster; t < ntiles; t += clusters) {
       const PairTile tl = job.tile(t);
-      const int total = tl.ksteps * loop.pairs + step_count(job.again(tl), tl.k0, tl.k0 + tl.ksteps), pieces = (total + loop.chunk - 1) / loop.chunk;
+      const int total = tl.ksteps + step_count(job.again(tl), tl.k0, tl.k0 + tl.ksteps), pieces = (total + loop.chunk - 1) / loop.chunk;
       float acc[kCols];
 #pragma unroll
       for (int j = 0; j < kCols; ++j) acc[j] = 0.f;

@@ -653,12 +653,12 @@ struct DheadJob {
   }
 };
 
-template <int NT, bool A_MN, bool B_MN, class Job>
+template <int NT, bool A_MN, bool B_MN, bool ONE, class Job>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 head_gemm_kernel(const Job job, const PairLoop loop, const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                  const __grid_constant__ CUtensorMap omap, int* status) {
   grid_dep_launch();
-  pair_gemm<NT, A_MN, B_MN>(job, loop, &amap, &bmap, &omap, status, [] { grid_dep_wait(); });
+  pair_gemm<NT, A_MN, B_MN, ONE>(job, loop, &amap, &bmap, &omap, status, [] { grid_dep_wait(); });
 }
 
 // ------------------------------------------------------------------------------------------------ the rows' sums
@@ -859,12 +859,16 @@ static int slab_map(CUtensorMap* m, const void* base, int slabs, uint64_t slab_r
   return make_tmap_3d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, slabs, rows, cols, slab_rows * pitch * 2, pitch * 2, box_rows, 64, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+template <int NT, bool A_MN, bool B_MN, bool ONE, class Job>
+static int launch_pair_as(const Job& job, const PairLoop& loop, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const HeadCall& c) {
+  cudaError_t e = allow_smem<head_gemm_kernel<NT, A_MN, B_MN, ONE, Job>>(kPairSmem);
+  if (e != cudaSuccess) return (int)e;
+  launch_pdl(head_gemm_kernel<NT, A_MN, B_MN, ONE, Job>, dim3(2 * kPairClusters), dim3(kPairThreads), kPairSmem, c.st, job, loop, a, b, o, c.status);
+  return (int)cudaGetLastError();
+}
 template <int NT, bool A_MN, bool B_MN, class Job>
 static int launch_pair(const Job& job, const PairLoop& loop, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const HeadCall& c) {
-  cudaError_t e = allow_smem<head_gemm_kernel<NT, A_MN, B_MN, Job>>(kPairSmem);
-  if (e != cudaSuccess) return (int)e;
-  launch_pdl(head_gemm_kernel<NT, A_MN, B_MN, Job>, dim3(2 * kPairClusters), dim3(kPairThreads), kPairSmem, c.st, job, loop, a, b, o, c.status);
-  return (int)cudaGetLastError();
+  return loop.na * loop.nb == 1 ? launch_pair_as<NT, A_MN, B_MN, true>(job, loop, a, b, o, c) : launch_pair_as<NT, A_MN, B_MN, false>(job, loop, a, b, o, c);
 }
 
 static PackedRows states_of(const HeadCall& c, const HeadPlan& p) {
@@ -920,10 +924,17 @@ static Targets head_targets_of(const HeadCall& c, const HeadPlan& p) {
 }
 
 // Steps of 64 between fp32 additions where 32 bits are asked for. Cut-off sums over a step are 5e-8 too small; this keeps that below what fp32 additions
-// along H round by (H = 128 7e-8, 1024 2.5e-7, 5120 7e-7). Shorter pieces wait for their additions: of one step 15 to 50 %, of two up to 6 %.
-static inline int exact_chunk(int H) { return H <= 256 ? 1 : H <= 640 ? 2 : 4; }
-constexpr int kExactChunk = 4;         // along rows or the vocabulary: gradients in fp32
-constexpr int kRoundedChunk = 32;      // where the result is rounded to bf16 (cut-off sums over 2048: 2e-6), or a gradient's logits are (2e-6 of z: 2^-15 of s)
+// along H round by (H = 128 7e-8, 1024 2.5e-7, 5120 7e-7). Shorter pieces wait for their additions: of one step 15 to 50 %, of two up to 6 %. Steps of
+// several slabs are long enough to be pieces by themselves.
+static inline int exact_chunk(int sa, int sb, int H) { return sa * sb > 1 ? 1 : H <= 256 ? 1 : H <= 640 ? 2 : 4; }
+// Where the result is rounded to bf16 (cut-off sums over 2048: 2e-6), or a gradient's logits are (2e-6 of z: 2^-15 of s): about 32 steps of one pair.
+static inline PairLoop rounded_loop(int sa, int sb) {
+  const int order = sa * sb > 1 ? 1 : 0;
+  PairLoop l = pair_loop(sa, sb, order, 32);
+  l.chunk = 32 / l.pairs;
+  return l;
+}
+static inline PairLoop exact_loop(int sa, int sb, int H) { return pair_loop(sa, sb, 2, exact_chunk(sa, sb, H)); }
 
 template <bool CAP, int C>
 static int head_score(const HeadCall& c, const HeadPlan& p, float* loss, float* stats) {
@@ -940,7 +951,7 @@ static int head_score(const HeadCall& c, const HeadPlan& p, float* loss, float* 
     job.v0 = v0;
     job.nv = c.rows.V - v0 < p.piece ? c.rows.V - v0 : p.piece;
     if ((rc = head_rows_map(&wm, c, p, v0, job.nv, C, true))) return rc;
-    if ((rc = launch_pair<2 * C, false, false>(job, pair_loop(p.sx, p.sw, 2, exact_chunk(c.H)), xm, wm, xm, c))) return rc;
+    if ((rc = launch_pair<2 * C, false, false>(job, exact_loop(p.sx, p.sw, c.H), xm, wm, xm, c))) return rc;
   }
   launch_pdl(head_merge_kernel, dim3((c.rows.R + 31) / 32), dim3(1024), 0, c.st, c.rows, live, pos, count, p.rows_cap, p.nblk, (const float2*)job.part,
              (const float*)job.zt, job.tg.sid, job.tg.slp, loss, stats);
@@ -982,12 +993,12 @@ static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, c
       big.of_cols = big.of_rows + p.rows_cap / 256 * p.row_words;
     }
     gj.big = xj.big = big;
-    if ((rc = launch_pair<2 * C, false, false>(gj, pair_loop(p.sx, p.sw, 2, exact ? exact_chunk(c.H) : kRoundedChunk), xk, wk, gout, c))) return rc;
+    if ((rc = launch_pair<2 * C, false, false>(gj, exact ? exact_loop(p.sx, p.sw, c.H) : rounded_loop(1, 1), xk, wk, gout, c))) return rc;
     if (dx) {
       if ((rc = head_rows_map(&wmn, c, p, v0, nv, 64, false))) return rc;
       xj.ksteps = (nv + 63) / 64;
       xj.first = v0 == 0;
-      const PairLoop loop = c.x_fp32 ? pair_loop(p.sg, p.sw, 2, kExactChunk) : pair_loop(p.sg, p.sw, exact ? 1 : 0, kRoundedChunk);
+      const PairLoop loop = c.x_fp32 ? exact_loop(p.sg, p.sw, 1 << 30) : exact ? rounded_loop(p.sg, p.sw) : rounded_loop(1, 1);
       if ((rc = launch_pair<256, false, true>(xj, loop, gk, wmn, aout, c))) return rc;
     }
     if (dhead) {
@@ -1000,10 +1011,10 @@ static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, c
       if (!boxes) hout = gmn;
       if (c.head_fp32) {
         const DheadJob<float> job{count, nv, H, (float*)out, boxes, big};
-        rc = launch_pair<256, true, true>(job, pair_loop(p.sg, p.sx, 2, kExactChunk), gmn, xmn, hout, c);
+        rc = launch_pair_as<256, true, true, false>(job, exact_loop(p.sg, p.sx, 1 << 30), gmn, xmn, hout, c);
       } else {
         const DheadJob<__nv_bfloat16> job{count, nv, H, (__nv_bfloat16*)out, boxes, big};
-        rc = launch_pair<256, true, true>(job, pair_loop(p.sg, p.sx, exact ? 1 : 0, kRoundedChunk), gmn, xmn, hout, c);
+        rc = launch_pair<256, true, true>(job, exact ? rounded_loop(p.sg, p.sx) : rounded_loop(1, 1), gmn, xmn, hout, c);
       }
       if (rc) return rc;
     }

@@ -7,9 +7,10 @@
 // ([rows, K]) or MN-major ([K, rows]).
 //
 // Sums. The tensor core cuts each addition to its accumulator off instead of rounding it: against 64 bits a sum over K = 5120 of random
-// products is 5.6e-6 too small (4.7e-6 of that is bias), over 16384 it is 1.9e-5, where fp32 FMAs are 7e-7 and 1.5e-6 off; pieces of 256
-// along K are 2.2e-7 off. So a sum stays in tensor memory for `chunk` steps only; two buffers of 256 columns alternate, and eight warps add
-// each finished piece to registers (128 sums a thread) with ordinary rounding while the next one runs.
+// products is 5.6e-6 off (4.7e-6 of that too small), over 16384 it is 1.9e-5, where fp32 FMAs are 7e-7 and 1.5e-6 off; over 128 it is 1.2e-7, and
+// pieces of 512 added in fp32 are 4.8e-7 off whatever K is. So a sum stays in tensor memory for `chunk` steps only; two buffers alternate, and eight
+// warps add each finished piece to registers (128 sums a thread) with ordinary rounding while the next one runs (456 cycles a piece of 256 columns; a
+// step of 64 along K is 512).
 //
 // Operands of more than bf16 precision come as slabs: an fp32 value is the exact sum of three bf16 values (8 + 8 + 8 bits), and the product
 // is summed over the pairs of slabs whose orders add up to two at most (what is left out is below 2^-24 of the product).
@@ -48,6 +49,7 @@ VE_DEVINL void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
+// (Without the release at cluster scope, which waits for the thread's stores, 1300 cycles: what has been read from tensor memory is ordered by its fences.)
 VE_DEVINL void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }

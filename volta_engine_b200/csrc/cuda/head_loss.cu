@@ -252,33 +252,45 @@ __global__ void __launch_bounds__(256) head_front_kernel(const HeadRows p, const
   const int block = blockIdx.x - teachers, blocks = gridDim.x - teachers;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (size_t i = block * (size_t)blockDim.x + threadIdx.x; i < nwords; i += (size_t)blocks * blockDim.x) words[i] = make_uint4(0u, 0u, 0u, 0u);
-  int n = 0;
-  for (int r0 = 0; r0 < p.R; r0 += 256) {
-    const int r = r0 + threadIdx.x;
+  // a thread looks at consecutive rows, 16 at most
+  const int each = (p.R + 255) / 256, r0 = threadIdx.x * each;
+  uint32_t mine = 0;
+#pragma unroll 4
+  for (int e = 0; e < each; ++e) {
+    const int r = r0 + e;
     bool on = false;
     if (r < p.R) {
       if (p.labels) on = label_of(p, r) >= 0;
       else
         for (int k = 0; k < p.K && !on; k += 8)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) on |= k + e < p.K && p.ids[(size_t)r * p.K + k + e] >= 0;
+          for (int g = 0; g < 8; ++g) on |= k + g < p.K && p.ids[(size_t)r * p.K + k + g] >= 0;
     }
-    const unsigned mask = __ballot_sync(0xffffffffu, on);
-    if (lane == 0) part[warp] = __popc(mask);
-    __syncthreads();
-    int at = n + __popc(mask & ((1u << lane) - 1));
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      if (w < warp) at += part[w];
-      n += part[w];
-    }
-    if (on) row_of[at] = r;
-    if (block == 0) {
-      if (r < p.R) pos[r] = on ? at : -1;
-      if (on) live[at] = r;
-    }
-    __syncthreads();
+    mine |= (uint32_t)on << e;
   }
+  int at = __popc(mine), n = 0;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, at, o);
+    if (lane >= o) at += v;
+  }
+  if (lane == 31) part[warp] = at;
+  at -= __popc(mine);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    if (w < warp) at += part[w];
+    n += part[w];
+  }
+  for (int e = 0; e < each && r0 + e < p.R; ++e) {
+    const bool on = mine >> e & 1u;
+    if (on) row_of[at] = r0 + e;
+    if (block == 0) {
+      pos[r0 + e] = on ? at : -1;
+      if (on) live[at] = r0 + e;
+    }
+    at += on;
+  }
+  __syncthreads();
   if (block == 0 && threadIdx.x == 0) {
     count[0] = n;
     count[1] = dx_splits(n, dx);
@@ -797,7 +809,8 @@ static inline int blocks_of(size_t n, int per = 256) {
   return (int)(b < 148 * 16 ? (b ? b : 1) : 148 * 16);
 }
 
-// Sizes of pieces: dz of a piece takes 256 MB at most, packed rows of the head 512 MB.
+// Sizes of pieces: dz of a piece takes 256 MB at most, packed rows of the head 512 MB (pieces that stay in L2 are slower: 1 x 838 x 77594 in fp32 378 us
+// at 64 MB, 295 at 512: short waves).
 static HeadPlan head_plan(bool grads, bool want_dx, int x_fp32, int head_fp32, bool pack_head, int R, int H, int V, int K, bool kl) {
   HeadPlan p;
   p.Hp = (H + 7) / 8 * 8;
@@ -805,17 +818,17 @@ static HeadPlan head_plan(bool grads, bool want_dx, int x_fp32, int head_fp32, b
   p.sw = head_fp32 ? 3 : 1;
   p.sg = x_fp32 || head_fp32 ? 3 : 2;
   p.rows_cap = (R + 255) / 256 * 256;
-  // tiles of 256 columns where they give every pair one, otherwise of 64 (96 x 512 x 4099 in fp32 with gradients 89 us against 99, 77 x 515 x 5003 with a
-  // teacher and a cap 84 against 96)
-  p.span = (long)(p.rows_cap / 256) * ((V + 255) / 256) < kPairClusters ? 32 : 128;
-  p.nblk = (V + p.span - 1) / p.span;
-  p.ksteps = (H + 63) / 64;
-  p.pack_head = pack_head;
-  p.few = R <= kFrontRows && (!kl || (size_t)R * K <= kFrontIds);
   size_t piece = ((size_t)V + 255) / 256 * 256;
   if (pack_head) { const size_t most = (512ull << 20) / ((size_t)p.sw * p.Hp * 2) / 256 * 256; piece = piece < most ? piece : (most ? most : 256); }
   if (grads) { const size_t most = (256ull << 20) / ((size_t)p.sg * p.rows_cap * 2) / 256 * 256; piece = piece < most ? piece : (most ? most : 256); }
   p.piece = (int)piece;
+  // tiles of 256 columns where they give every pair one, otherwise of 64 (96 x 512 x 4099 in fp32 with gradients 89 us against 99, 77 x 515 x 5003 with a
+  // teacher and a cap 84 against 96)
+  p.span = (long)(p.rows_cap / 256) * (p.piece / 256) < kPairClusters ? 32 : 128;
+  p.nblk = (V + p.span - 1) / p.span;
+  p.ksteps = (H + 63) / 64;
+  p.pack_head = pack_head;
+  p.few = R <= kFrontRows && (!kl || (size_t)R * K <= kFrontIds);
   p.pairs = x_fp32 ? (head_fp32 ? 6 : 3) : (head_fp32 ? 3 : 1);
   const size_t sums = 4ull * p.rows_cap * p.Hp;                                          // of a range of dx: 256 MB together
   p.splits = (int)((256ull << 20) / sums < 1 ? 1 : (256ull << 20) / sums < 32 ? (256ull << 20) / sums : 32);

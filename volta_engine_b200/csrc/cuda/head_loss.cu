@@ -990,7 +990,7 @@ static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, c
     rc = make_tmap_3d(&gout, c.ws + p.G, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.sg, p.rows_cap, p.piece, 2ull * p.rows_cap * p.piece, 2ull * p.piece, 32,
                       gj.kBox, gj.kBox == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
   if (rc) return rc;
-  gj.count = count; gj.ksteps = p.ksteps; gj.tg = head_targets_of(c, p); gj.live = live; 
+  gj.count = count; gj.ksteps = p.ksteps; gj.tg = head_targets_of(c, p); gj.live = live;
   gj.slabs = p.sg; gj.cap = c.softcap; gj.inv_cap = CAP ? 1.f / c.softcap : 0.f;
   gj.in = RowInputs{stats, dloss, c.rows.tail, (const double*)(c.ws + p.mass), R, c.rows.labels != nullptr};
   DxJob xj{count, H, p.Hp, 0, 1, (size_t)p.rows_cap * p.Hp, (float*)(c.ws + p.acc), {}};

@@ -391,3 +391,41 @@ def test_offsets_that_pass_32_bits():
     assert float((got["dx"].double() - dx).norm() / dx.norm()) < 2.0 ** -8
     tail = s[:, -100:].t() @ x.double()
     assert float((got["dhead"][-100:].double() - tail).norm() / tail.norm()) < 2.0 ** -8
+
+
+def near(rows, hidden, vocab, topk, noise, common, device, seed=0, spread=2.5):
+    """bf16 inputs whose head rows have a part in common (``common`` times their spread), as the rows of trained heads do; a teacher of the same states
+    but for ``noise``."""
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(vocab, hidden, generator=g) + common * torch.randn(1, hidden, generator=g)
+    w = (w * spread / math.sqrt(hidden)).bfloat16()
+    labels = torch.randint(0, vocab, (rows,), generator=g)
+    x = torch.randn(rows, hidden, generator=g) + 6 * torch.rand(rows, 1, generator=g) * torch.nn.functional.normalize(w[labels].float(), dim=1)
+    x, dloss = x.bfloat16(), torch.rand(rows, generator=g) + 0.5
+    targets = (labels,)
+    if topk:
+        lp = torch.log_softmax((x.double() + noise * torch.randn(rows, hidden, generator=g).double()) @ w.double().t(), 1)
+        logp, ids = lp.topk(topk, 1)
+        targets = (ids.int(), logp.float(), (1 - logp.exp().sum(1)).clamp(min=1e-9).log().float())
+    return x.to(device), w.to(device), tuple(t.to(device) for t in targets), dloss.to(device)
+
+
+def beside_rounding(got, want):
+    """Errors of a bf16 result's rows over what rounding the 64-bit result to bf16 would be off by."""
+    return (got.double() - want).norm(dim=1) / (want.to(torch.bfloat16).double() - want).norm(dim=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,hidden,vocab,topk,softcap", [(40, 256, 3000, 0, 0.0), (300, 264, 20100, 0, 20.0), (1300, 64, 50000, 0, 0.0), (40, 256, 3000, 8, 0.0),
+                                                            (300, 264, 20100, 16, 0.0)])
+def test_bf16_gradients_are_off_by_their_rounding(rows, hidden, vocab, topk, softcap):
+    """Rows of dx and dhead (those of nobody's label too) in 47 to 682 blocks of 64 columns, in ranges of the vocabulary, in two pieces of it, with a cap:
+    what stands in front of the last rounding adds less than a tenth to it. dz comes in two slabs, 2^-18 of a value, where the result's rounding is 2^-9
+    of its own, and a common part of three times the spread makes 2^-18 of dz about 2^-16 of dx; the logits' share is below 2^-13 of s, an
+    eighth of the rounding even beside that part: sqrt(1 + 1/64). Near a teacher (noise 0.1) a row's dz is a difference of two nearly equal shares, in some
+    rows to the logits' own error: the middle row is looked at."""
+    a = near(rows, hidden, vocab, topk, 0.1, 3.0, "cuda")
+    got, want = run(*a, softcap), P.wanted(*a, softcap)
+    for k in ("dx", "dhead"):
+        r = beside_rounding(got[k], want[k])
+        assert float(r.median() if topk else r.max()) < 1.1, (k, float(r.median()), float(r.max()))

@@ -123,21 +123,6 @@ struct PairLoop {
   int chunk;                  // steps that a sum stays in tensor memory
 };
 
-// Steps that are worth a second look: bit k of a tile's words asks for step k once more, with the second slab of A (what the first one's rounding
-// left) in place of the first. (Loops of one slab each.)
-VE_DEVINL uint32_t step_bits(const uint32_t* words, int w, int k0, int k1) {        // word w, cut to steps [k0, k1)
-  uint32_t b = words[w];
-  if (w == k0 >> 5) b &= 0xffffffffu << (k0 & 31);
-  if (w == k1 >> 5) b &= (1u << (k1 & 31)) - 1u;
-  return b;
-}
-VE_DEVINL int step_count(const uint32_t* words, int k0, int k1) {
-  int n = 0;
-  if (words)
-    for (int w = k0 >> 5; w * 32 < k1; ++w) n += __popc(step_bits(words, w, k0, k1));
-  return n;
-}
-
 // The pairs (i, j) of `sa` x `sb` slabs with i + j <= order, the small ones first: what is cut off a sum is cut by its size, so a step that is a piece by
 // itself loses as little as one of its first slabs alone. All pairs of a step work on one load of it (6 of 3 x 3 slabs: half of what the pairs one
 // after another would bring).
@@ -154,9 +139,8 @@ static inline PairLoop pair_loop(int sa, int sb, int order, int chunk) {
   return l;
 }
 
-// Job: gives the tiles (int tiles(), PairTile tile(int i)), the words of steps to repeat (const uint32_t* again(tile), or null), what a thread loads
-// in front of its sums (Row begin(tile, row of the tile, first column)) and takes the sums: finish(tile, row of the tile, first column, Row,
-// sums[NT / 2], omap, 4 KB of shared memory of the warp).
+// Job: gives the tiles (int tiles(), PairTile tile(int i)), what a thread loads in front of its sums (Row begin(tile, row of the tile, first column))
+// and takes the sums: finish(tile, row of the tile, first column, Row, sums[NT / 2], omap, 4 KB of shared memory of the warp).
 // A_MN / B_MN: the operand is MN-major.
 // wait(): the point behind which other kernels' results are read.
 // ONE: one slab of either operand, known to the compiler (3 to 4 % of a step's time).
@@ -198,18 +182,19 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
       for (int t = cluster; t < ntiles && ok; t += clusters) {
         const PairTile tl = job.tile(t);
         const int am = tl.m0 + rank * 128, bn = tl.n0 + rank * kCols;
-        auto load = [&](int k, int a0) {                    // a step of slabs a0, a0 + 1, .. of A
-          if (!mbar_wait(&empty[s], phase)) return false;
+        for (int k = 0; k < tl.ksteps; ++k) {
+          ok = mbar_wait(&empty[s], phase);
+          if (!ok) break;
           uint8_t* st = smem + s * stage_bytes;
           if (rank == 0) mbar_expect_tx(&full[s], 2 * stage_bytes);
           const uint32_t bar = first_cta_addr(&full[s]);
-          const int kk = k * 64;
+          const int kk = (tl.k0 + k) * 64;
           for (int i = 0; i < na; ++i, st += S::kA) {
             if (A_MN) {
-              tma_load_3d_pair(st, amap, bar, am, kk, a0 + i);
-              tma_load_3d_pair(st + S::kA / 2, amap, bar, am + 64, kk, a0 + i);
+              tma_load_3d_pair(st, amap, bar, am, kk, i);
+              tma_load_3d_pair(st + S::kA / 2, amap, bar, am + 64, kk, i);
             } else {
-              tma_load_3d_pair(st, amap, bar, kk, am, a0 + i);
+              tma_load_3d_pair(st, amap, bar, kk, am, i);
             }
           }
           for (int j = 0; j < nb; ++j, st += S::kB) {
@@ -221,14 +206,7 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
             }
           }
           if (++s == stages) { s = 0; phase ^= 1; }
-          return true;
-        };
-        for (int k = 0; k < tl.ksteps && ok; ++k) ok = load(tl.k0 + k, 0);
-        const uint32_t* words = job.again(tl);
-        const int k1 = tl.k0 + tl.ksteps;
-        if (words)
-          for (int w = tl.k0 >> 5; w * 32 < k1 && ok; ++w)
-            for (uint32_t bits = step_bits(words, w, tl.k0, k1); bits && ok; bits &= bits - 1) ok = load(w * 32 + __ffs(bits) - 1, 1);
+        }
       }
       if (!ok) atomicExch(&s_fail, 1);
     } else if (warp == 1 && rank == 0 && elect_one()) {
@@ -236,8 +214,7 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
       int s = 0, phase = 0, piece = 0;
       bool ok = true;
       for (int t = cluster; t < ntiles && ok; t += clusters) {
-        const PairTile tl = job.tile(t);
-        const int total = tl.ksteps + step_count(job.again(tl), tl.k0, tl.k0 + tl.ksteps);
+        const int total = job.tile(t).ksteps;
         for (int i = 0; i < total && ok; ++piece) {
           const int buf = piece & 1;
           ok = mbar_wait(&acc_empty[buf], ((piece >> 1) & 1) ^ 1);
@@ -278,7 +255,7 @@ VE_DEVINL void pair_gemm(const Job& job, const PairLoop& loop, const CUtensorMap
     if (cluster < ntiles) row = begin(cluster);
     for (int t = cluster; t < ntiles; t += clusters) {
       const PairTile tl = job.tile(t);
-      const int total = tl.ksteps + step_count(job.again(tl), tl.k0, tl.k0 + tl.ksteps), pieces = (total + loop.chunk - 1) / loop.chunk;
+      const int pieces = (tl.ksteps + loop.chunk - 1) / loop.chunk;
       float acc[kCols];
 #pragma unroll
       for (int j = 0; j < kCols; ++j) acc[j] = 0.f;

@@ -12,10 +12,10 @@
 // of exponentials without the targets, and the targets' logits; one more pass over these few numbers gives the loss. The targets are left
 // out of the sums so that log(1 + exp(..)) and log(rho) do not come from the difference of two nearly equal numbers. The gradient computes the
 // logits again, a piece of the vocabulary at a time, writes dz of that piece in bf16 slabs (rows x piece: the only array of that kind) and
-// multiplies it with the head's rows and with the states. dz beside fp32 operands is three bf16 slabs (fp32's 24 bits). Beside bf16 operands it is one
-// slab, and what its rounding left (up to 2^-8 of a value: as much as the rounding of the gradients, whose error it would raise by 1.41, with few
-// rows by up to 2.5) in a second one that is multiplied only where it matters: blocks of 64 x 64 in which an element is above a sixteenth of its
-// row's largest (a label's own dz is at least every other's; beside a teacher, above a 64th of the row's weight). Those are few: a label a row.
+// multiplies it with the head's rows and with the states. dz beside fp32 operands is three bf16 slabs (fp32's 24 bits), beside bf16 operands two
+// (2^-18 of a value, and gradients are rounded to 2^-9 of theirs). One slab alone would be 2^-9 off as the gradients are, but of every addend: a row of dz
+// sums to zero, so what the head's rows have in common leaves dx except for that rounding, and near a teacher the addends are far above their sum
+// (errors of 2 to 6 times the gradients' own rounding; rows of dhead 1.3 to 2.9 times it).
 // Sums run in a fixed order: the same call gives the same bits.
 //
 // Rows that are left out (label below zero, a teacher row of padding) are taken out in front: the states of the others are gathered, so what
@@ -239,9 +239,9 @@ __global__ void __launch_bounds__(256) head_pack_kernel(const PackedRows m, cons
 }
 
 // All of that for few rows in one launch: `teachers` blocks sort a teacher's row each; every other block finds all the rows that count and packs its
-// share of them, and of the head where all of it is packed at once; the words of large blocks become zero on the way.
+// share of them, and of the head where all of it is packed at once.
 __global__ void __launch_bounds__(256) head_front_kernel(const HeadRows p, const TeacherRows teacher, int teachers, int* live, int* pos, int* count,
-                                                         const PackedRows x, const PackedRows head, int head_rows, uint4* words, size_t nwords, const DxPlan dx) {
+                                                         const PackedRows x, const PackedRows head, int head_rows, const DxPlan dx) {
   __shared__ int row_of[kFrontRows], part[8];
   grid_dep_launch();
   grid_dep_wait();
@@ -251,7 +251,6 @@ __global__ void __launch_bounds__(256) head_front_kernel(const HeadRows p, const
   }
   const int block = blockIdx.x - teachers, blocks = gridDim.x - teachers;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (size_t i = block * (size_t)blockDim.x + threadIdx.x; i < nwords; i += (size_t)blocks * blockDim.x) words[i] = make_uint4(0u, 0u, 0u, 0u);
   // a thread looks at consecutive rows, 16 at most
   const int each = (p.R + 255) / 256, r0 = threadIdx.x * each;
   uint32_t mine = 0;
@@ -337,7 +336,6 @@ struct LogitTiles {           // rows x a piece of the vocabulary: tiles of up t
   int v0, nv, ksteps;
   VE_DEVINL int row_tiles() const { return (*count + 255) >> 8; }
   VE_DEVINL int tiles() const { return row_tiles() * ((nv + NT - 1) / NT); }
-  VE_DEVINL const uint32_t* again(const PairTile&) const { return nullptr; }
   struct Row { int row, begin, end, first; };        // the caller's row (-1: behind the last one), its targets among the thread's columns, the first one's column
   VE_DEVINL Row row_at(const PairTile& t, int r, int c0, const int* live, const Targets& tg) const {
     const int i = t.m0 + r, col0 = t.n0 + c0;
@@ -438,7 +436,6 @@ struct ScoreJob : LogitTiles<C> {
 // Constants of a row's dz: at any token dense * s, at a target `at` * s - g * (teacher's mass); a likely label's is `at` itself.
 struct RowGrad {
   float lse2, dense, at, g;
-  float large;                // dz above this is multiplied with its rounding error too
 };
 
 struct RowInputs {            // by row of the caller
@@ -456,22 +453,13 @@ struct RowInputs {            // by row of the caller
     if (labels) {
       c.dense = g * fix;
       c.at = -g * expf(rest - lse);
-      c.large = fabsf(c.at) * (1.f / 16.f);
     } else {
       const double a = mass[row], lr = (double)rest - (double)lse, t = lr >= (double)kLogFloor ? exp((double)tail[row]) : 0.0;
       c.at = (float)((double)g * (a + t)) * fix;
       c.dense = (float)((double)g * (t > 0.0 ? a + t - t * exp(-lr) : a)) * fix;       // (a difference: in 64 bits)
-      c.large = fabsf(g) * (1.f / 64.f);
     }
     return c;
   }
-};
-
-// Blocks of 64 x 64 of a piece's dz with large elements: by tiles of 256 rows, bits over the columns' blocks (dx), and by tiles of 256 columns,
-// bits over the rows' blocks (dhead).
-struct LargeBlocks {
-  uint32_t *of_rows, *of_cols;
-  int row_words, col_words;   // words of a tile
 };
 
 template <bool CAP, int C>
@@ -483,7 +471,6 @@ struct GradJob : LogitTiles<C> {
   RowInputs in;
   int slabs;                  // of dz
   static constexpr int kBox = C < 64 ? C : 64, kBoxes = C / kBox;        // columns that leave together
-  LargeBlocks big;            // (null: every slab counts everywhere)
   float cap, inv_cap;
 
   struct Row : Tiles::Row {
@@ -491,7 +478,7 @@ struct GradJob : LogitTiles<C> {
     float mass;               // the teacher's, of the first target
   };
   VE_DEVINL Row begin(const PairTile& t, int r, int c0) const {
-    Row w{this->row_at(t, r, c0, live, tg), {0.f, 0.f, 0.f, 0.f, 0.f}, 0.f};
+    Row w{this->row_at(t, r, c0, live, tg), {0.f, 0.f, 0.f, 0.f}, 0.f};
     if (w.row >= 0) w.c = in.at(w.row);
     if (!tg.labels && w.first >= 0) w.mass = expf(tg.slp[(size_t)w.row * tg.K + w.begin]);
     return w;
@@ -560,19 +547,6 @@ struct GradJob : LogitTiles<C> {
 #pragma unroll
       for (int j = 0; j < C; ++j) z[j] = j < width ? z[j] : 0.f;
     }
-    if (big.of_rows) {
-#pragma unroll
-      for (int h = 0; h < kBoxes; ++h) {
-        float m = 0.f;
-#pragma unroll
-        for (int j = kBox * h; j < kBox * h + kBox; ++j) m = fmaxf(m, fabsf(z[j]));
-        if (__any_sync(0xffffffffu, m > c.large) && (threadIdx.x & 31) == 0) {
-          const int kc = (col0 >> 6) + h, kr = i >> 6;
-          atomicOr(big.of_rows + (t.m0 >> 8) * big.row_words + (kc >> 5), 1u << (kc & 31));
-          atomicOr(big.of_cols + (t.n0 >> 8) * big.col_words + (kr >> 5), 1u << (kr & 31));
-        }
-      }
-    }
     for (int s = 0; s < slabs; ++s)
 #pragma unroll
       for (int h = 0; h < kBoxes; ++h) {
@@ -590,10 +564,8 @@ struct DxJob {
   int H, Hp, ksteps, first;
   size_t slab;
   float* acc;                 // [ranges][rows_cap][Hp]
-  LargeBlocks big;
   struct Row {};
   VE_DEVINL Row begin(const PairTile&, int, int) const { return {}; }
-  VE_DEVINL const uint32_t* again(const PairTile& t) const { return big.of_rows ? big.of_rows + (t.m0 >> 8) * big.row_words : nullptr; }
   VE_DEVINL int row_tiles() const { return (*count + 255) >> 8; }
   VE_DEVINL int splits() const { return count[1]; }
   VE_DEVINL int tiles() const { return row_tiles() * ((H + 255) >> 8) * splits(); }
@@ -624,10 +596,8 @@ struct DheadJob {
   T* out;                     // [nv, H], contiguous rows
   bool boxes;                 // rows on 16-byte boundaries: written by TMA (omap)
   static constexpr int kBox = 128 / sizeof(T);
-  LargeBlocks big;
   struct Row {};
   VE_DEVINL Row begin(const PairTile&, int, int) const { return {}; }
-  VE_DEVINL const uint32_t* again(const PairTile& t) const { return big.of_cols ? big.of_cols + (t.m0 >> 8) * big.col_words : nullptr; }
   VE_DEVINL int tiles() const { return ((nv + 255) >> 8) * ((H + 255) >> 8); }
   VE_DEVINL PairTile tile(int i) const {
     const int nn = (H + 255) >> 8;
@@ -800,8 +770,7 @@ struct HeadPlan {             // sizes and places in the workspace
   bool pack_head;             // the head's rows go through slabs of their own, a piece at a time
   int piece;                  // vocabulary rows at a time
   int splits, pairs;          // most ranges of a piece that dx is summed over; products of slabs
-  int row_words, col_words;   // of LargeBlocks
-  size_t live, pos, count, flag, mass, sid, slp, off, x, part, zt, head, G, acc, big, big_bytes, bytes;      // (big_bytes: of a piece)
+  size_t live, pos, count, flag, mass, sid, slp, off, x, part, zt, head, G, acc, bytes;
 };
 
 static inline int blocks_of(size_t n, int per = 256) {
@@ -829,7 +798,7 @@ static HeadPlan head_plan(bool grads, bool want_dx, int x_fp32, int head_fp32, b
   p.ksteps = (H + 63) / 64;
   p.pack_head = pack_head;
   p.few = R <= kFrontRows && (!kl || (size_t)R * K <= kFrontIds);
-  p.pairs = x_fp32 ? (head_fp32 ? 6 : 3) : (head_fp32 ? 3 : 1);
+  p.pairs = x_fp32 ? (head_fp32 ? 6 : 3) : (head_fp32 ? 3 : 2);
   const size_t sums = 4ull * p.rows_cap * p.Hp;                                          // of a range of dx: 256 MB together
   p.splits = (int)((256ull << 20) / sums < 1 ? 1 : (256ull << 20) / sums < 32 ? (256ull << 20) / sums : 32);
   size_t at = 0;
@@ -839,15 +808,10 @@ static HeadPlan head_plan(bool grads, bool want_dx, int x_fp32, int head_fp32, b
   if (kl) { p.flag = take(4ull * R); p.mass = take(8ull * R); p.sid = take(4ull * R * K); p.slp = take(4ull * R * K); p.off = take(2ull * R * (p.nblk + 1)); }
   p.x = take(2ull * p.sx * p.rows_cap * p.Hp);
   p.head = pack_head ? take(2ull * p.sw * p.piece * p.Hp) : 0;
-  p.part = p.zt = p.G = p.acc = p.big = p.big_bytes = 0;
-  p.row_words = p.col_words = 0;
+  p.part = p.zt = p.G = p.acc = 0;
   if (!grads) { p.part = take(8ull * p.nblk * p.rows_cap); p.zt = take(4ull * R * (kl ? K : 1)); }
   else {
     p.G = take(2ull * p.sg * p.rows_cap * p.piece);
-    p.row_words = (p.piece / 64 + 31) / 32;
-    p.col_words = (p.rows_cap / 64 + 31) / 32;
-    p.big_bytes = p.sg == 2 ? (4ull * (p.rows_cap / 256 * p.row_words + p.piece / 256 * p.col_words) + 15) / 16 * 16 : 0;
-    p.big = take(p.big_bytes * (((size_t)V + p.piece - 1) / p.piece));
     if (want_dx) p.acc = take(4ull * p.splits * p.rows_cap * p.Hp);
   }
   p.bytes = at;
@@ -900,9 +864,8 @@ static void pack_rows(const PackedRows& m, const int* live, const int* count, in
   else launch_pdl(head_pack_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, m, live, count, rows);
 }
 
-// The rows that count, their targets and their states; zeros in the words of large blocks; a head that is packed at once.
+// The rows that count, their targets and their states; a head that is packed at once.
 static int head_front(const HeadCall& c, const HeadPlan& p) {
-  const size_t word_bytes = p.big_bytes * (((size_t)c.rows.V + p.piece - 1) / p.piece);
   int *live = (int*)(c.ws + p.live), *pos = (int*)(c.ws + p.pos), *count = (int*)(c.ws + p.count), *flag = (int*)(c.ws + p.flag);
   const TeacherRows teacher{p.span, p.nblk, (int*)(c.ws + p.sid), (float*)(c.ws + p.slp), (uint16_t*)(c.ws + p.off), flag, (double*)(c.ws + p.mass)};
   const DxPlan dx{(c.H + 255) / 256, p.piece / 64, p.pairs, p.acc ? p.splits : 0};
@@ -910,12 +873,8 @@ static int head_front(const HeadCall& c, const HeadPlan& p) {
   if (p.few) {
     const int heads = head_in_front(c, p) ? c.rows.V : 0;
     launch_pdl(head_front_kernel, dim3(teachers + pack_blocks(p, (size_t)p.rows_cap + heads)), dim3(256), 0, c.st, c.rows, teacher, teachers, live, pos, count,
-               states_of(c, p), head_of(c, p, 0), heads, (uint4*)(c.ws + p.big), word_bytes / 16, dx);
+               states_of(c, p), head_of(c, p, 0), heads, dx);
     return (int)cudaGetLastError();
-  }
-  if (word_bytes) {
-    const cudaError_t e = cudaMemsetAsync(c.ws + p.big, 0, word_bytes, c.st);
-    if (e != cudaSuccess) return (int)e;
   }
   if (teachers) launch_pdl(head_targets_kernel, dim3(R), dim3(128), 0, c.st, c.rows, teacher);
   launch_pdl(head_rows_kernel, dim3(1), dim3(1024), 0, c.st, c.rows, (const int*)flag, live, pos, count, dx);
@@ -993,26 +952,20 @@ static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, c
   gj.count = count; gj.ksteps = p.ksteps; gj.tg = head_targets_of(c, p); gj.live = live;
   gj.slabs = p.sg; gj.cap = c.softcap; gj.inv_cap = CAP ? 1.f / c.softcap : 0.f;
   gj.in = RowInputs{stats, dloss, c.rows.tail, (const double*)(c.ws + p.mass), R, c.rows.labels != nullptr};
-  DxJob xj{count, H, p.Hp, 0, 1, (size_t)p.rows_cap * p.Hp, (float*)(c.ws + p.acc), {}};
+  DxJob xj{count, H, p.Hp, 0, 1, (size_t)p.rows_cap * p.Hp, (float*)(c.ws + p.acc)};
   const bool exact = p.sg == 3;
   for (int v0 = 0; v0 < c.rows.V; v0 += p.piece) {
     const int nv = c.rows.V - v0 < p.piece ? c.rows.V - v0 : p.piece;
     gj.v0 = v0;
     gj.nv = nv;
     if ((rc = head_rows_map(&wk, c, p, v0, nv, C, true))) return rc;
-    LargeBlocks big{nullptr, nullptr, p.row_words, p.col_words};
-    if (p.big_bytes) {
-      big.of_rows = (uint32_t*)(c.ws + p.big + p.big_bytes * (v0 / p.piece));
-      big.of_cols = big.of_rows + p.rows_cap / 256 * p.row_words;
-    }
-    gj.big = xj.big = big;
     if ((rc = launch_pair<2 * C, false, false>(gj, exact ? exact_loop(p.sx, p.sw, c.H) : rounded_loop(1, 1), xk, wk, gout, c))) return rc;
     if (dx) {
       if ((rc = head_rows_map(&wmn, c, p, v0, nv, 64, false))) return rc;
       xj.ksteps = (nv + 63) / 64;
       xj.first = v0 == 0;
-      const PairLoop loop = c.x_fp32 ? exact_loop(p.sg, p.sw, 1 << 30) : exact ? rounded_loop(p.sg, p.sw) : rounded_loop(1, 1);
-      if ((rc = launch_pair<256, false, true>(xj, loop, gk, wmn, aout, c))) return rc;
+      const PairLoop loop = c.x_fp32 ? exact_loop(p.sg, p.sw, 1 << 30) : rounded_loop(p.sg, p.sw);
+      if ((rc = launch_pair_as<256, false, true, false>(xj, loop, gk, wmn, aout, c))) return rc;
     }
     if (dhead) {
       const size_t es = c.head_fp32 ? 4 : 2;
@@ -1023,11 +976,11 @@ static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, c
         return rc;
       if (!boxes) hout = gmn;
       if (c.head_fp32) {
-        const DheadJob<float> job{count, nv, H, (float*)out, boxes, big};
+        const DheadJob<float> job{count, nv, H, (float*)out, boxes};
         rc = launch_pair_as<256, true, true, false>(job, exact_loop(p.sg, p.sx, 1 << 30), gmn, xmn, hout, c);
       } else {
-        const DheadJob<__nv_bfloat16> job{count, nv, H, (__nv_bfloat16*)out, boxes, big};
-        rc = launch_pair<256, true, true>(job, exact ? rounded_loop(p.sg, p.sx) : rounded_loop(1, 1), gmn, xmn, hout, c);
+        const DheadJob<__nv_bfloat16> job{count, nv, H, (__nv_bfloat16*)out, boxes};
+        rc = launch_pair_as<256, true, true, false>(job, rounded_loop(p.sg, p.sx), gmn, xmn, hout, c);
       }
       if (rc) return rc;
     }

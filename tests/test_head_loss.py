@@ -429,3 +429,15 @@ def test_bf16_gradients_are_off_by_their_rounding(rows, hidden, vocab, topk, sof
     for k in ("dx", "dhead"):
         r = beside_rounding(got[k], want[k])
         assert float(r.median() if topk else r.max()) < 1.1, (k, float(r.median()), float(r.max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,hidden,vocab,common", [(60, 4096, 5000, 0.0), (500, 1024, 20100, 0.0), (60, 4096, 5000, 3.0), (300, 264, 20100, 0.0)])
+def test_logits_of_gradients_are_those_of_the_loss(rows, hidden, vocab, common):
+    """Every row of the gradients beside an ordinary teacher, those of a confident model among them, whose dz is 2^-7 and less of what it is the difference
+    of: logits to 2^-21 of theirs, as the loss takes them, are some 2^-12 of such rows, an eighth of the rounding; 2^-19 would be half of it and more."""
+    a = near(rows, hidden, vocab, 16, 0.9, common, "cuda")
+    got, want = run(*a), P.wanted(*a, 0.0)
+    for k in ("dx", "dhead"):
+        r = beside_rounding(got[k], want[k])
+        assert float(r.max()) < 1.1, (k, float(r.max()))

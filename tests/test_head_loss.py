@@ -441,3 +441,18 @@ def test_logits_of_gradients_are_those_of_the_loss(rows, hidden, vocab, common):
     for k in ("dx", "dhead"):
         r = beside_rounding(got[k], want[k])
         assert float(r.max()) < 1.1, (k, float(r.max()))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("vocab,gone", [(257, (256, 257)), (300, (32, 64)), (700, (128, 256)), (3000, (384, 512)), (20100, (20096, 20100))])
+@pytest.mark.parametrize("topk", [0, 3])
+def test_nan_in_the_head(vocab, gone, topk, device):
+    """NaN logits of tokens that are no targets, alone in a block of columns: every loss is NaN, as its gradients are."""
+    x, head, targets, dl = make(300 if vocab > 20000 else 6, 72, vocab, topk, seed=1, device=device)
+    if topk:
+        targets = (torch.arange(topk, dtype=torch.int32, device=device).expand(x.shape[0], topk).contiguous(), *targets[1:])
+    else:
+        targets = (targets[0].clamp(max=gone[0] - 1),)
+    head[gone[0]:gone[1]] = math.nan
+    got = run(x, head, targets, dl)
+    assert torch.isnan(got["loss"]).all() and torch.isnan(got["stats"]).all() and torch.isnan(got["dx"]).all()

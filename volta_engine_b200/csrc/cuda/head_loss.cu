@@ -668,12 +668,12 @@ __global__ void __launch_bounds__(1024) head_merge_kernel(const HeadRows p, cons
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) mx = fmaxf(mx, v[e].x);
-      if (mx != neg_inf()) {
-        s *= exp2f((m - mx) * kLog2e);
+      // (maxima pass NaN over, sums keep it: a block of NaN alone has a maximum of minus infinity or NaN, and counts)
+      const float at = mx == neg_inf() ? 0.f : mx;
+      s *= exp2f((m - at) * kLog2e);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s += v[e].y * exp2f((v[e].x - mx) * kLog2e);
-        m = mx;
-      }
+      for (int e = 0; e < 8; ++e) s += v[e].y * exp2f((v[e].x - at) * kLog2e);
+      m = mx;
     }
   }
   sm[warp][lane] = m;
@@ -684,7 +684,7 @@ __global__ void __launch_bounds__(1024) head_merge_kernel(const HeadRows p, cons
   const float wm = sm[lane][warp];
   const float top = warp_max(wm);
   const double sum = [&] {
-    double v = wm == neg_inf() ? 0.0 : (double)ss[lane][warp] * exp2((double)(wm - top) * 1.4426950408889634);
+    double v = (double)ss[lane][warp] * exp2((double)(wm - (top == neg_inf() ? 0.f : top)) * 1.4426950408889634);
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
   }();

@@ -456,3 +456,12 @@ def test_nan_in_the_head(vocab, gone, topk, device):
     head[gone[0]:gone[1]] = math.nan
     got = run(x, head, targets, dl)
     assert torch.isnan(got["loss"]).all() and torch.isnan(got["stats"]).all() and torch.isnan(got["dx"]).all()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_the_largest_id_is_behind_the_vocabulary(device):
+    x, head, t, dl = make(20, 72, 300, 4, seed=2, device=device)
+    t[0][5, 2] = 2 ** 31 - 1
+    got = run(x, head, t, dl)
+    assert torch.isnan(got["loss"][5]) and int(torch.isnan(got["loss"]).sum()) == 1
+    assert torch.isnan(got["dx"][5]).all() and int(torch.isnan(got["dx"]).any(1).sum()) == 1

@@ -60,7 +60,7 @@ VE_DEVINL void sort_teacher(const HeadRows& p, const TeacherRows& o, int r) {
   double sum = 0.0;
   for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
     const int v = p.ids[(size_t)r * p.K + k];
-    id[k] = v < 0 ? INT_MAX : v;
+    id[k] = v < 0 ? INT_MAX : min(v, INT_MAX - 1);          // (any id behind the vocabulary is as wrong as the last)
     any |= v >= 0;
     if (v >= 0) sum += exp((double)p.logp[(size_t)r * p.K + k]);
   }

@@ -465,3 +465,18 @@ def test_the_largest_id_is_behind_the_vocabulary(device):
     got = run(x, head, t, dl)
     assert torch.isnan(got["loss"][5]) and int(torch.isnan(got["loss"]).sum()) == 1
     assert torch.isnan(got["dx"][5]).all() and int(torch.isnan(got["dx"]).any(1).sum()) == 1
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_a_token_listed_twice_is_one_in_the_loss_too(device):
+    """Each result as of the teacher whose masses are added first. fp32 sums of the same numbers in another order: 2^-20, and bf16 gradients one step of theirs."""
+    x, head, _, dl = make(3, 72, 300, 0, seed=3, device=device)
+    two = (torch.tensor([[1, 1, 3, -1, 1], [9, 7, 9, 7, 8], [2, 2, 2, 2, 2]], dtype=torch.int32),
+           torch.log(torch.tensor([[0.1, 0.2, 0.4, 0.9, 0.1], [0.1, 0.1, 0.1, 0.1, 0.0], [0.1, 0.2, 0.0, 0.3, 0.1]])), torch.log(torch.tensor([0.2, 0.6, 0.3])))
+    one = (torch.tensor([[1, 3, -1], [9, 7, 8], [2, -1, -1]], dtype=torch.int32),
+           torch.log(torch.tensor([[0.4, 0.4, 1.0], [0.2, 0.2, 0.0], [0.7, 1.0, 1.0]])), two[2])
+    a, b = (run(x, head, tuple(v.to(device) for v in t), dl) for t in (two, one))
+    for k in a:
+        assert torch.allclose(a[k].float(), b[k].float(), rtol=2.0 ** -7 if k in ("dx", "dhead") else 2.0 ** -20, atol=1e-6), k
+    w = P.wanted(x, head, tuple(v.to(device) for v in one), dl, 0.0)
+    assert torch.allclose(a["loss"].double(), w["loss"], rtol=1e-5, atol=1e-6)

@@ -715,8 +715,15 @@ __global__ void __launch_bounds__(1024) head_merge_kernel(const HeadRows p, cons
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     lse = mx + log(v + (rest == -INFINITY ? 0.0 : exp(rest - mx)));
     out = 0.0;
-    for (int k = lane; k < p.K; k += 32)
-      if (id[k] < p.V && lp[k] != neg_inf()) out += exp((double)lp[k]) * ((double)lp[k] - ((double)z[k] - lse));
+    for (int k = lane; k < p.K; k += 32) {
+      if (id[k] >= p.V || (k > 0 && id[k - 1] == id[k])) continue;
+      double a = exp((double)lp[k]), la = lp[k];
+      if (k + 1 < p.K && id[k + 1] == id[k]) {          // (listed again: its mass is the sum)
+        for (int j = k + 1; j < p.K && id[j] == id[k]; ++j) a += exp((double)lp[j]);
+        la = log(a);
+      }
+      if (a != 0.0) out += a * (la - ((double)z[k] - lse));
+    }
     for (int o = 16; o > 0; o >>= 1) out += __shfl_xor_sync(0xffffffffu, out, o);
     const float lt = p.tail[row];
     if (lt != neg_inf()) out += exp((double)lt) * ((double)lt - fmax(rest - lse, (double)kLogFloor));

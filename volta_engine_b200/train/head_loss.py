@@ -4,7 +4,7 @@ K most likely tokens and the mass of the rest (what ``volta_ppl --topk-out`` wri
     z = cap(x head^T),  cap(z) = softcap * tanh(z / softcap) (softcap 0: z as it is)        s = softmax(z)
     cross entropy   nll = log sum_v exp z_v - z_label
     divergence      kl  = sum_k a_k (log a_k - log s_k) + t (log t - log max(r, 1e-12)),  a = exp(logp), t = exp(tail),
-                    r = the model's mass outside the teacher's tokens
+                    r = the model's mass outside the teacher's tokens, k over the tokens that the teacher lists
 
 ``x`` [rows, hidden] and ``head`` [vocab, hidden] are bf16 or fp32, each by itself; sums are 32 bits wide and the products of fp32 operands exact to
 2^-24. Rows may be strided. Losses and their sums are fp32; dx has the type of x, dhead that of head.
@@ -209,7 +209,8 @@ def _cpu_kl(x, head, ids, logp, tail, softcap):
     bad, at, a, logp, tail, hit = _cpu_teacher(z, ids[live], logp[live], tail[live])
     lse, rest = _sums(z, hit)
     zero = torch.zeros((), dtype=z.dtype)
-    kl = torch.where(a > 0, a * (logp - (z.gather(1, at) - lse[:, None])), zero).sum(1)
+    whole = torch.zeros_like(z).scatter_add_(1, at, a).gather(1, at)             # the mass of an entry's token (more than its own where it is listed again)
+    kl = torch.where(a == 0, zero, a * (torch.where(whole > a, torch.log(whole), logp) - (z.gather(1, at) - lse[:, None]))).sum(1)
     kl = kl + torch.where(tail > -math.inf, torch.exp(tail) * (tail - (rest - lse).clamp(min=math.log(REST_FLOOR))), zero)
     nan = torch.full_like(kl, math.nan)
     return _spread(torch.where(bad, nan, kl), live), torch.stack([_spread(torch.where(bad, nan, lse), live), _spread(rest, live)])

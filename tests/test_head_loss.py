@@ -480,3 +480,20 @@ def test_a_token_listed_twice_is_one_in_the_loss_too(device):
         assert torch.allclose(a[k].float(), b[k].float(), rtol=2.0 ** -7 if k in ("dx", "dhead") else 2.0 ** -20, atol=1e-6), k
     w = P.wanted(x, head, tuple(v.to(device) for v in one), dl, 0.0)
     assert torch.allclose(a["loss"].double(), w["loss"], rtol=1e-5, atol=1e-6)
+
+
+@pytest.mark.gpu
+def test_a_piece_of_more_than_2_31_values():
+    """dhead of 256000 x 8448 in one piece, its pitch in bytes beyond 32 bits."""
+    vocab, hidden = 256000, 8448
+    g = torch.Generator(device="cuda").manual_seed(0)
+    head = torch.empty(vocab, hidden, dtype=torch.bfloat16, device="cuda")
+    for lo in range(0, vocab, 32000):
+        head[lo:lo + 32000] = torch.randn(32000, hidden, generator=g, device="cuda") * (2.0 / math.sqrt(hidden))
+    x = torch.randn(3, hidden, generator=g, device="cuda").to(torch.bfloat16)
+    labels = torch.tensor([vocab - 1, 5, vocab - 1700], device="cuda")
+    got = run(x, head, (labels,), torch.ones(3, device="cuda"))
+    z = torch.cat([x.double() @ head[lo:lo + 32000].double().t() for lo in range(0, vocab, 32000)], 1)
+    dz = torch.softmax(z, 1).scatter_add_(1, labels[:, None], torch.full((3, 1), -1.0, dtype=torch.float64, device="cuda"))
+    for lo in (0, vocab - 1750, vocab - 100):                    # (and labels among them)
+        assert float(beside_rounding(got["dhead"][lo:lo + 100], dz[:, lo:lo + 100].t() @ x.double()).max()) < 1.1

@@ -978,7 +978,7 @@ static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, c
       const size_t es = c.head_fp32 ? 4 : 2;
       uint8_t* out = (uint8_t*)dhead + (size_t)v0 * H * es;
       const bool boxes = H * es % 16 == 0 && !((uintptr_t)dhead & 15);
-      if (boxes && (rc = make_tmap_3d(&hout, out, c.head_fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (int)es, 1, nv, H, nv * H * es,
+      if (boxes && (rc = make_tmap_3d(&hout, out, c.head_fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (int)es, 1, nv, H, (uint64_t)nv * H * es,
                                       H * es, 32, (uint32_t)(128 / es), CU_TENSOR_MAP_SWIZZLE_128B)))
         return rc;
       if (!boxes) hout = gmn;

@@ -497,3 +497,14 @@ def test_a_piece_of_more_than_2_31_values():
     dz = torch.softmax(z, 1).scatter_add_(1, labels[:, None], torch.full((3, 1), -1.0, dtype=torch.float64, device="cuda"))
     for lo in (0, vocab - 1750, vocab - 100):                    # (and labels among them)
         assert float(beside_rounding(got["dhead"][lo:lo + 100], dz[:, lo:lo + 100].t() @ x.double()).max()) < 1.1
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_nan_of_a_teacher(device):
+    """A log-probability or a rest of NaN in a row that counts is its loss; beside a padded id it is nothing."""
+    x, head, (ids, logp, tail), dl = make(6, 72, 300, 4, seed=5, device=device)
+    logp[2, 1], tail[4] = math.nan, math.nan
+    ids[5, 3], logp[5, 3] = -1, math.nan
+    got = run(x, head, (ids, logp, tail), dl)
+    bad = torch.tensor([False, False, True, False, True, False], device=device)
+    assert torch.equal(torch.isnan(got["loss"]), bad) and torch.equal(torch.isnan(got["dx"]).all(1), bad) and torch.equal(torch.isnan(got["dx"]).any(1), bad)

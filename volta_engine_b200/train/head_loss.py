@@ -211,7 +211,7 @@ def _cpu_kl(x, head, ids, logp, tail, softcap):
     zero = torch.zeros((), dtype=z.dtype)
     whole = torch.zeros_like(z).scatter_add_(1, at, a).gather(1, at)             # the mass of an entry's token (more than its own where it is listed again)
     kl = torch.where(a == 0, zero, a * (torch.where(whole > a, torch.log(whole), logp) - (z.gather(1, at) - lse[:, None]))).sum(1)
-    kl = kl + torch.where(tail > -math.inf, torch.exp(tail) * (tail - (rest - lse).clamp(min=math.log(REST_FLOOR))), zero)
+    kl = kl + torch.where(tail == -math.inf, zero, torch.exp(tail) * (tail - (rest - lse).clamp(min=math.log(REST_FLOOR))))
     nan = torch.full_like(kl, math.nan)
     return _spread(torch.where(bad, nan, kl), live), torch.stack([_spread(torch.where(bad, nan, lse), live), _spread(rest, live)])
 

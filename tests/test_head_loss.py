@@ -508,3 +508,25 @@ def test_nan_of_a_teacher(device):
     got = run(x, head, (ids, logp, tail), dl)
     bad = torch.tensor([False, False, True, False, True, False], device=device)
     assert torch.equal(torch.isnan(got["loss"]), bad) and torch.equal(torch.isnan(got["dx"]).all(1), bad) and torch.equal(torch.isnan(got["dx"]).any(1), bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [900, 20100])
+@pytest.mark.parametrize("topk", [0, 3])
+def test_sums_beside_large_logits(vocab, topk):
+    """Logits of 60 to 140 that 32 bits hold (quarters times quarters, and a column that adds a hundred): the log-sums are off by the exponentials, 2^-22 of
+    their terms, the rounding of their arguments, 2^-22, and their own rounding, 2^-18 at most; the loss, a difference of a few units, by 2^-20 in all and
+    a rounding of its own."""
+    g = torch.Generator().manual_seed(vocab)
+    x = (torch.randint(-8, 9, (200, 16), generator=g) / 4).to(torch.bfloat16)
+    head = (torch.randint(-8, 9, (vocab, 16), generator=g) / 4).to(torch.bfloat16)
+    x[:, 0], head[:, 0] = 100.0, 1.0
+    z = x.double() @ head.double().t()
+    labels = (z + 3 * torch.randn(z.shape, generator=g).double()).argmax(1)
+    targets = (labels,) if not topk else (z.topk(topk, 1)[1].int(), torch.full((200, topk), math.log(0.9 / topk)), torch.full((200,), math.log(0.1)))
+    targets = tuple(t.cuda() for t in targets)
+    x, head = x.cuda(), head.cuda()
+    w = P.wanted(x, head, targets, torch.ones(200, device="cuda"), 0.0)
+    loss, stats = (L.head_cross_entropy if not topk else L.head_kl)(x, head, *targets)
+    assert bool(((loss.double() - w["loss"]).abs() <= 2.0 ** -20 + w["loss"].abs() * 2.0 ** -24).all()), float((loss.double() - w["loss"]).abs().max()) * 2 ** 20
+    assert bool(((stats.double() - w["stats"]).abs() <= 2.0 ** -20 + w["stats"].abs() * 2.0 ** -24).all())

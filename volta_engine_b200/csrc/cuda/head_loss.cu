@@ -429,7 +429,8 @@ struct ScoreJob : LogitTiles<C> {
       s2 += ex2_approx(fmaf(z[j + 2], kLog2e, m2));
       s3 += ex2_approx(fmaf(z[j + 3], kLog2e, m2));
     }
-    if (on) part[(size_t)blk * rows_cap + i] = make_float2(m, (s0 + s1) + (s2 + s3));
+    // (what the product m log2e lost to rounding is in every term: 2^-18 of a sum beside logits of 100)
+    if (on) part[(size_t)blk * rows_cap + i] = make_float2(m, ((s0 + s1) + (s2 + s3)) * exp2f(m == neg_inf() ? 0.f : -fmaf(m, kLog2e, m2)));
   }
 };
 

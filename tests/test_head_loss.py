@@ -530,3 +530,39 @@ def test_sums_beside_large_logits(vocab, topk):
     loss, stats = (L.head_cross_entropy if not topk else L.head_kl)(x, head, *targets)
     assert bool(((loss.double() - w["loss"]).abs() <= 2.0 ** -20 + w["loss"].abs() * 2.0 ** -24).all()), float((loss.double() - w["loss"]).abs().max()) * 2 ** 20
     assert bool(((stats.double() - w["stats"]).abs() <= 2.0 ** -20 + w["stats"].abs() * 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("topk", [0, 5])
+def test_fine_statistics_on_the_cpu(topk):
+    x, head, t, dl = make(7, 12, 33, topk, "fp32", "fp32", seed=1, left_out=0.3)
+    f, b = (L.head_cross_entropy, L.head_cross_entropy_backward) if not topk else (L.head_kl, L.head_kl_backward)
+    (l1, s1), (l2, s2) = f(x, head, *t), f(x, head, *t, fine=True)
+    assert s2.shape == (4, 7) and torch.equal(l1, l2) and torch.equal(s1, s2[:2]) and not s2[2:].any()
+    assert all(torch.equal(u, v) for u, v in zip(b(x, head, *t, s1, dl), b(x, head, *t, s2, dl)))
+    s2[2:] = 0.25                                          # and they are added
+    s1 = s1 + 0.25
+    assert all(torch.equal(u, v) for u, v in zip(b(x, head, *t, s1, dl), b(x, head, *t, s2, dl)))
+    for bad in (s2[:3], s2[:, :5], s2[0]):
+        with pytest.raises(ValueError, match="stats of shape"):
+            b(x, head, *t, bad, dl)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("topk", [0, 6])
+@pytest.mark.parametrize("vocab", [900, 20100])
+def test_fine_statistics_keep_what_sums_lose(topk, vocab):
+    """Column 0 of the head is one and that column of the states a hundred, so that log-sums lie in 64 to 128, where 32 bits round by up to 2^-18, and column 0
+    of dx is the sum of the row's dz: zero. Exponentials are off by 2^-22 here and in the sums, their arguments' rounding by as much, and the sum
+    of a row's |dz| (two dloss at most) by 2^-23 of it: 1.25 * 2^-20 dloss with the lower parts; without them some row is off by twice that."""
+    x, head, t, dl = make(200, 72, vocab, topk, "fp32", "fp32", seed=2, left_out=0.1, device="cuda")
+    x[:, 0], head[:, 0] = 100.0, 1.0
+    f, b = (L.head_cross_entropy, L.head_cross_entropy_backward) if not topk else (L.head_kl, L.head_kl_backward)
+    (l1, s1), (l2, s2) = f(x, head, *t), f(x, head, *t, fine=True)
+    assert torch.equal(l1, l2) and torch.equal(s1, s2[:2])
+    assert bool((s2[2:].abs() <= s2[:2].abs() * 2.0 ** -24).all()) and bool(s2[2:].any())
+    off = [(b(x, head, *t, s, dl, want_dhead=False)[0][:, 0].abs() / dl) for s in (s1, s2)]
+    assert float(off[1].max()) < 1.25 * 2.0 ** -20 < float(off[0].max()) / 2, [float(v.max()) * 2 ** 20 for v in off]
+    # the differentiable call with them
+    xs = x.clone().requires_grad_()
+    (L.head_cross_entropy_loss if not topk else L.head_kl_loss)(xs, head, *t, fine=True).backward(dl)
+    assert torch.equal(xs.grad, b(x, head, *t, s2, dl, want_dhead=False)[0])

@@ -443,19 +443,20 @@ struct RowInputs {            // by row of the caller
   const float *stats, *dloss, *tail;
   const double* mass;
   int R;
-  bool labels;
+  bool labels, fine;          // fine: the statistics' lower parts stand behind them
   VE_DEVINL RowGrad at(int row) const {
-    const float lse = stats[row], rest = stats[R + row], g = dloss[row];
+    const double lse = (double)stats[row] + (fine ? (double)stats[2 * R + row] : 0.0), rest = (double)stats[R + row] + (fine ? (double)stats[3 * R + row] : 0.0);
+    const float g = dloss[row];
     RowGrad c;
     // exp(z - lse) as 2^(z log2e - lse2): what the product lse log2e loses to rounding goes into the factors
-    c.lse2 = lse * kLog2e;
-    const float fix = exp2f(-fmaf(lse, kLog2e, -c.lse2));
+    c.lse2 = (float)(lse * (double)kLog2e);
+    const float fix = exp2f((float)((double)c.lse2 - lse * (double)kLog2e));
     c.g = g;
     if (labels) {
       c.dense = g * fix;
-      c.at = -g * expf(rest - lse);
+      c.at = -g * expf((float)(rest - lse));
     } else {
-      const double a = mass[row], lr = (double)rest - (double)lse, t = lr >= (double)kLogFloor ? exp((double)tail[row]) : 0.0;
+      const double a = mass[row], lr = rest - lse, t = lr >= (double)kLogFloor ? exp((double)tail[row]) : 0.0;
       c.at = (float)((double)g * (a + t)) * fix;
       c.dense = (float)((double)g * (t > 0.0 ? a + t - t * exp(-lr) : a)) * fix;       // (a difference: in 64 bits)
     }
@@ -648,13 +649,16 @@ head_gemm_kernel(const Job job, const PairLoop loop, const __grid_constant__ CUt
 // Joins a row's blocks and computes its loss, 32 rows a block of 1024 threads: the warps share the blocks of columns, lanes are rows; then a
 // warp takes a row's targets. The few numbers behind the sums are in 64 bits: losses near zero, and divergences of near models, are differences.
 __global__ void __launch_bounds__(1024) head_merge_kernel(const HeadRows p, const int* live, const int* pos, const int* count, int rows_cap, int nblk,
-                                                          const float2* part, const float* zt, const int* sid, const float* slp, float* loss, float* stats) {
+                                                          const float2* part, const float* zt, const int* sid, const float* slp, float* loss, float* stats, int fine) {
   __shared__ float sm[32][33], ss[32][33];
   grid_dep_launch();
   grid_dep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = *count;
   const int r = blockIdx.x * 32 + lane;
-  if (warp == 0 && r < p.R && pos[r] < 0) loss[r] = stats[r] = stats[p.R + r] = 0.f;          // left out
+  if (warp == 0 && r < p.R && pos[r] < 0) {          // left out
+    loss[r] = stats[r] = stats[p.R + r] = 0.f;
+    if (fine) stats[2 * p.R + r] = stats[3 * p.R + r] = 0.f;
+  }
   if (blockIdx.x * 32 >= n) return;
   const int i = blockIdx.x * 32 + lane;
   float m = neg_inf(), s = 0.f;
@@ -734,6 +738,10 @@ __global__ void __launch_bounds__(1024) head_merge_kernel(const HeadRows p, cons
     loss[row] = (float)out;
     stats[row] = (float)lse;
     stats[p.R + row] = (float)rest;
+    if (fine) {          // what the rounding left
+      stats[2 * p.R + row] = isinf(lse) ? 0.f : (float)(lse - (double)(float)lse);
+      stats[3 * p.R + row] = isinf(rest) ? 0.f : (float)(rest - (double)(float)rest);
+    }
   }
 }
 
@@ -916,7 +924,7 @@ static inline PairLoop rounded_loop(int sa, int sb) {
 static inline PairLoop exact_loop(int sa, int sb, int H) { return pair_loop(sa, sb, 2, exact_chunk(sa, sb, H)); }
 
 template <bool CAP, int C>
-static int head_score(const HeadCall& c, const HeadPlan& p, float* loss, float* stats) {
+static int head_score(const HeadCall& c, const HeadPlan& p, float* loss, float* stats, int fine) {
   int rc = head_front(c, p);
   if (rc) return rc;
   const int *live = (const int*)(c.ws + p.live), *pos = (const int*)(c.ws + p.pos), *count = (const int*)(c.ws + p.count);
@@ -933,12 +941,12 @@ static int head_score(const HeadCall& c, const HeadPlan& p, float* loss, float* 
     if ((rc = launch_pair<2 * C, false, false>(job, exact_loop(p.sx, p.sw, c.H), xm, wm, xm, c))) return rc;
   }
   launch_pdl(head_merge_kernel, dim3((c.rows.R + 31) / 32), dim3(1024), 0, c.st, c.rows, live, pos, count, p.rows_cap, p.nblk, (const float2*)job.part,
-             (const float*)job.zt, job.tg.sid, job.tg.slp, loss, stats);
+             (const float*)job.zt, job.tg.sid, job.tg.slp, loss, stats, fine);
   return (int)cudaGetLastError();
 }
 
 template <bool CAP, int C>
-static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, const float* dloss, void* dx, void* dhead) {
+static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, int fine, const float* dloss, void* dx, void* dhead) {
   int rc = head_front(c, p);
   if (rc) return rc;
   const int *live = (const int*)(c.ws + p.live), *pos = (const int*)(c.ws + p.pos), *count = (const int*)(c.ws + p.count);
@@ -958,7 +966,7 @@ static int head_grad(const HeadCall& c, const HeadPlan& p, const float* stats, c
   if (rc) return rc;
   gj.count = count; gj.ksteps = p.ksteps; gj.tg = head_targets_of(c, p); gj.live = live;
   gj.slabs = p.sg; gj.cap = c.softcap; gj.inv_cap = CAP ? 1.f / c.softcap : 0.f;
-  gj.in = RowInputs{stats, dloss, c.rows.tail, (const double*)(c.ws + p.mass), R, c.rows.labels != nullptr};
+  gj.in = RowInputs{stats, dloss, c.rows.tail, (const double*)(c.ws + p.mass), R, c.rows.labels != nullptr, fine != 0};
   DxJob xj{count, H, p.Hp, 0, 1, (size_t)p.rows_cap * p.Hp, (float*)(c.ws + p.acc)};
   // the logits are summed in the scored ones' steps: beside an lse of exacter sums, 2e-6 of z are errors of s that a row has in common (rows whose model
   // is near its teacher or label: up to 6 times the gradients' rounding, 60 x 4096 x 5000; here 2 to 3 % of the time)
@@ -1013,9 +1021,10 @@ long ve_head_loss_workspace(int grads, int want_dx, int x_fp32, int head_fp32, i
 }
 
 // x [R, H] (row pitch ldx), head [V, H] (pitch ldw), each bf16 or fp32. labels (int32 / int64 [R]) or ids int32 [R, K] with logp fp32 [R, K] and
-// tail fp32 [R]. loss fp32 [R], stats fp32 [2, R]: log sum exp of all logits, and of all but the targets.
+// tail fp32 [R]. loss fp32 [R], stats fp32 [2, R]: log sum exp of all logits, and of all but the targets; fine: [4, R], what rounding both to 32 bits left
+// behind them.
 int ve_head_loss(const void* x, int x_fp32, long ldx, const void* head, int head_fp32, long ldw, const void* labels, int label_bytes, const void* ids,
-                 const void* logp, const void* tail, int K, int R, int H, int V, float softcap, void* loss, void* stats, void* ws, long ws_bytes, void* status,
+                 const void* logp, const void* tail, int K, int R, int H, int V, float softcap, void* loss, void* stats, int fine, void* ws, long ws_bytes, void* status,
                  cudaStream_t st) {
   if (R <= 0) return 0;
   if (H <= 0 || V <= 0 || (!labels && (K < 1 || K > kMaxTopk))) return cudaErrorInvalidValue;
@@ -1023,13 +1032,13 @@ int ve_head_loss(const void* x, int x_fp32, long ldx, const void* head, int head
   if ((size_t)ws_bytes < p.bytes) return cudaErrorInvalidValue;
   const HeadCall c{x, x_fp32, ldx, head, head_fp32, ldw, {labels, label_bytes, (const int*)ids, (const float*)logp, (const float*)tail, K, R, V}, H, softcap,
                    (uint8_t*)ws, (int*)status, st};
-  if (p.span == 32) return softcap > 0.f ? head_score<true, 32>(c, p, (float*)loss, (float*)stats) : head_score<false, 32>(c, p, (float*)loss, (float*)stats);
-  return softcap > 0.f ? head_score<true, 128>(c, p, (float*)loss, (float*)stats) : head_score<false, 128>(c, p, (float*)loss, (float*)stats);
+  if (p.span == 32) return softcap > 0.f ? head_score<true, 32>(c, p, (float*)loss, (float*)stats, fine) : head_score<false, 32>(c, p, (float*)loss, (float*)stats, fine);
+  return softcap > 0.f ? head_score<true, 128>(c, p, (float*)loss, (float*)stats, fine) : head_score<false, 128>(c, p, (float*)loss, (float*)stats, fine);
 }
 
 // The gradients for dloss fp32 [R]: dx [R, H] in the states' type and dhead [V, H] in the head's, either may be null.
 int ve_head_loss_grad(const void* x, int x_fp32, long ldx, const void* head, int head_fp32, long ldw, const void* labels, int label_bytes, const void* ids,
-                      const void* logp, const void* tail, int K, int R, int H, int V, float softcap, const void* stats, const void* dloss, void* dx, void* dhead,
+                      const void* logp, const void* tail, int K, int R, int H, int V, float softcap, const void* stats, int fine, const void* dloss, void* dx, void* dhead,
                       void* ws, long ws_bytes, void* status, cudaStream_t st) {
   if (R <= 0 || (!dx && !dhead)) return 0;
   if (H <= 0 || V <= 0 || (!labels && (K < 1 || K > kMaxTopk))) return cudaErrorInvalidValue;
@@ -1038,8 +1047,8 @@ int ve_head_loss_grad(const void* x, int x_fp32, long ldx, const void* head, int
   const HeadCall c{x, x_fp32, ldx, head, head_fp32, ldw, {labels, label_bytes, (const int*)ids, (const float*)logp, (const float*)tail, K, R, V}, H, softcap,
                    (uint8_t*)ws, (int*)status, st};
   const float *s = (const float*)stats, *g = (const float*)dloss;
-  if (p.span == 32) return softcap > 0.f ? head_grad<true, 32>(c, p, s, g, dx, dhead) : head_grad<false, 32>(c, p, s, g, dx, dhead);
-  return softcap > 0.f ? head_grad<true, 128>(c, p, s, g, dx, dhead) : head_grad<false, 128>(c, p, s, g, dx, dhead);
+  if (p.span == 32) return softcap > 0.f ? head_grad<true, 32>(c, p, s, fine, g, dx, dhead) : head_grad<false, 32>(c, p, s, fine, g, dx, dhead);
+  return softcap > 0.f ? head_grad<true, 128>(c, p, s, fine, g, dx, dhead) : head_grad<false, 128>(c, p, s, fine, g, dx, dhead);
 }
 
 }  // extern "C"

@@ -344,9 +344,9 @@ def objective(model, ids, teacher, head=None) -> torch.Tensor:
     if teacher is None:
         labels = torch.cat([ids[1:].long(), torch.full((1,), -100, dtype=torch.int64, device=ids.device)])
         mine, ranks = (labels[model.rows(ids.shape[0])], model.world) if isinstance(model, TunedModelSP) else (labels, 1)
-        return head_cross_entropy_loss(x, head, mine.to(x.device)).sum() * (ranks / max(1, ids.shape[0] - 1))
+        return head_cross_entropy_loss(x, head, mine.to(x.device), fine=True).sum() * (ranks / max(1, ids.shape[0] - 1))
     t_ids, logp, tail = teacher
-    return head_kl_loss(x[: t_ids.shape[0]], head, t_ids.to(torch.int32), logp.float(), tail.float()).mean()
+    return head_kl_loss(x[: t_ids.shape[0]], head, t_ids.to(torch.int32), logp.float(), tail.float(), fine=True).mean()
 
 
 def set_dropout(model, p: float, seed: int, rows: int) -> None:

@@ -55,7 +55,7 @@ def _check(x, head, softcap, others, dloss=None, stats=None):
         raise ValueError(f"softcap {softcap}: zero (none) or a number of at least 1e-30 is wanted")
     if dloss is not None:
         f = (torch.float32,) if x.is_cuda else (torch.float32, torch.float64)
-        others += (("dloss", dloss, f, (rows,)), ("stats", stats, f, (2, rows)))
+        others += (("dloss", dloss, f, (rows,)), ("stats", stats, f, (4 if stats.shape[:1] == (4,) else 2, rows)))
     for name, t, dtypes, shape in others:
         if t.dtype not in dtypes:
             raise TypeError(f"{name} of type {t.dtype}: {' or '.join(str(d) for d in dtypes)} is wanted")
@@ -101,16 +101,16 @@ def _common(x, head, labels, teacher, softcap):
             head.shape[0], softcap)
 
 
-def _forward(x, head, labels, teacher, softcap):
+def _forward(x, head, labels, teacher, softcap, fine):
     x, head = rows_of(x), rows_of(head)
     rows = x.shape[0]
     teacher = tuple(t.contiguous() for t in teacher) if teacher else None
     labels = labels.contiguous() if labels is not None else None
-    out = torch.empty(3, rows, dtype=torch.float32, device=x.device)
+    out = torch.empty(5 if fine else 3, rows, dtype=torch.float32, device=x.device)
     loss, stats = out[0], out[1:]
     if rows:
         ws = _workspace(False, False, x, head, teacher[0].shape[1] if teacher else 1, teacher is not None)
-        launch(x.device, "head_loss", _SIG + "ppplp", *_common(x, head, labels, teacher, softcap), loss.data_ptr(), stats.data_ptr(), ws.data_ptr(),
+        launch(x.device, "head_loss", _SIG + "ppiplp", *_common(x, head, labels, teacher, softcap), loss.data_ptr(), stats.data_ptr(), fine, ws.data_ptr(),
                ws.numel(), status_word(x.device).data_ptr())
     return loss, stats
 
@@ -125,8 +125,8 @@ def _backward(x, head, labels, teacher, stats, dloss, softcap, want_dx, want_dhe
     dhead = (torch.empty if rows else torch.zeros)(head.shape, dtype=head.dtype, device=x.device) if want_dhead else None
     if rows:
         ws = _workspace(True, want_dx, x, head, teacher[0].shape[1] if teacher else 1, teacher is not None)
-        launch(x.device, "head_loss_grad", _SIG + "ppppplp", *_common(x, head, labels, teacher, softcap), stats.data_ptr(), dloss.data_ptr(), ptr(dx),
-               ptr(dhead), ws.data_ptr(), ws.numel(), status_word(x.device).data_ptr())
+        launch(x.device, "head_loss_grad", _SIG + "pipppplp", *_common(x, head, labels, teacher, softcap), stats.data_ptr(), stats.shape[0] == 4,
+               dloss.data_ptr(), ptr(dx), ptr(dhead), ws.data_ptr(), ws.numel(), status_word(x.device).data_ptr())
     return dx, dhead
 
 
@@ -159,6 +159,16 @@ def _sums(z, targets):
     return torch.logsumexp(z, 1), torch.logsumexp(z.masked_fill(targets, -math.inf), 1)
 
 
+def _stats_out(lse, rest, live, fine):
+    out = torch.stack([_spread(lse, live), _spread(rest, live)])
+    return torch.cat([out, torch.zeros_like(out)]) if fine else out                # (sums in the states' own width: nothing behind them)
+
+
+def _stats_in(stats, live, dtype):
+    s = stats.to(dtype)[:, live]
+    return s[:2] + s[2:] if s.shape[0] == 4 else s
+
+
 def _finish_grads(dz, slope, bad, x, head, live, want_dx, want_dhead):
     if slope is not None:
         dz = dz * slope
@@ -174,21 +184,21 @@ def _cpu_labels(z, labels):
     return bad, y, torch.zeros_like(z, dtype=torch.bool).scatter_(1, y, True)
 
 
-def _cpu_ce(x, head, labels, softcap):
+def _cpu_ce(x, head, labels, softcap, fine):
     live = labels >= 0
     z, _ = _capped(_gathered(x, live), head, softcap)
     bad, y, hit = _cpu_labels(z, labels[live])
     lse, rest = _sums(z, hit)
     nll = torch.nn.functional.softplus(rest - z.gather(1, y)[:, 0], threshold=1e9)
     nan = torch.full_like(nll, math.nan)
-    return _spread(torch.where(bad, nan, nll), live), torch.stack([_spread(torch.where(bad, nan, lse), live), _spread(rest, live)])
+    return _spread(torch.where(bad, nan, nll), live), _stats_out(torch.where(bad, nan, lse), rest, live, fine)
 
 
 def _cpu_ce_grad(x, head, labels, stats, dloss, softcap, want_dx, want_dhead):
     live = labels >= 0
     z, slope = _capped(_gathered(x, live), head, softcap)
     bad, y, _ = _cpu_labels(z, labels[live])
-    lse, rest = stats[0][live].to(z.dtype), stats[1][live].to(z.dtype)
+    lse, rest = _stats_in(stats, live, z.dtype)
     dz = torch.exp(z - lse[:, None]).scatter(1, y, -torch.exp(rest - lse)[:, None]) * dloss[live].to(z.dtype)[:, None]
     return _finish_grads(dz, slope, bad, x, head, live, want_dx, want_dhead)
 
@@ -203,7 +213,7 @@ def _cpu_teacher(z, ids, logp, tail):
     return bad, at, torch.exp(logp), logp, tail.to(z.dtype), hit
 
 
-def _cpu_kl(x, head, ids, logp, tail, softcap):
+def _cpu_kl(x, head, ids, logp, tail, softcap, fine):
     live = (ids >= 0).any(1)
     z, _ = _capped(_gathered(x, live), head, softcap)
     bad, at, a, logp, tail, hit = _cpu_teacher(z, ids[live], logp[live], tail[live])
@@ -213,14 +223,14 @@ def _cpu_kl(x, head, ids, logp, tail, softcap):
     kl = torch.where(a == 0, zero, a * (torch.where(whole > a, torch.log(whole), logp) - (z.gather(1, at) - lse[:, None]))).sum(1)
     kl = kl + torch.where(tail == -math.inf, zero, torch.exp(tail) * (tail - (rest - lse).clamp(min=math.log(REST_FLOOR))))
     nan = torch.full_like(kl, math.nan)
-    return _spread(torch.where(bad, nan, kl), live), torch.stack([_spread(torch.where(bad, nan, lse), live), _spread(rest, live)])
+    return _spread(torch.where(bad, nan, kl), live), _stats_out(torch.where(bad, nan, lse), rest, live, fine)
 
 
 def _cpu_kl_grad(x, head, ids, logp, tail, stats, dloss, softcap, want_dx, want_dhead):
     live = (ids >= 0).any(1)
     z, slope = _capped(_gathered(x, live), head, softcap)
     bad, at, a, _, tail, hit = _cpu_teacher(z, ids[live], logp[live], tail[live])
-    lse, rest = stats[0][live].to(z.dtype), stats[1][live].to(z.dtype)
+    lse, rest = _stats_in(stats, live, z.dtype)
     s, t = torch.exp(z - lse[:, None]), torch.exp(tail)
     t = torch.where(rest - lse >= math.log(REST_FLOOR), t, torch.zeros_like(t))
     over = torch.where(t > 0, t * torch.exp(lse - rest), t)
@@ -230,10 +240,12 @@ def _cpu_kl_grad(x, head, ids, logp, tail, stats, dloss, softcap, want_dx, want_
 
 
 # ------------------------------------------------------------------------------------------------ entry points
-def head_cross_entropy(x, head, labels, *, softcap: float = 0.0):
-    """-> (nll [rows], stats [2, rows]): stats are log sum_v exp z_v and the same sum without the label, for the backward pass."""
+def head_cross_entropy(x, head, labels, *, softcap: float = 0.0, fine: bool = False):
+    """-> (nll [rows], stats [2, rows]): stats are log sum_v exp z_v and the same sum without the label, for the backward pass. ``fine``: stats [4, rows],
+    behind both what their rounding to 32 bits left. The backward pass takes either; a sum of 16 to 32 is off by up to 2^-20 without, which a row's
+    gradients have in common: fp32 gradients of few rows, and those of a model near its teacher, are more exact with it."""
     _check(x, head, softcap, _label_args(x, labels))
-    return _forward(x, head, labels, None, softcap) if x.is_cuda else _cpu_ce(x, head, labels, softcap)
+    return _forward(x, head, labels, None, softcap, fine) if x.is_cuda else _cpu_ce(x, head, labels, softcap, fine)
 
 
 def head_cross_entropy_backward(x, head, labels, stats, dloss, *, softcap: float = 0.0, want_dx: bool = True, want_dhead: bool = True):
@@ -246,11 +258,12 @@ def head_cross_entropy_backward(x, head, labels, stats, dloss, *, softcap: float
     return _cpu_ce_grad(x, head, labels, stats, dloss, softcap, want_dx, want_dhead)
 
 
-def head_kl(x, head, ids, logp, tail, *, softcap: float = 0.0):
+def head_kl(x, head, ids, logp, tail, *, softcap: float = 0.0, fine: bool = False):
     """ids int32 [rows, K], logp fp32 [rows, K] and tail fp32 [rows]: the teacher's tokens, their log-probabilities and the log of the mass outside
-    them. -> (kl [rows], stats [2, rows]): stats are log sum_v exp z_v and the same sum without the teacher's tokens."""
+    them. -> (kl [rows], stats [2, rows]): stats are log sum_v exp z_v and the same sum without the teacher's tokens (``fine``: as
+    ``head_cross_entropy``'s)."""
     _check(x, head, softcap, _teacher_args(x, ids, logp, tail))
-    return _forward(x, head, None, (ids, logp, tail), softcap) if x.is_cuda else _cpu_kl(x, head, ids, logp, tail, softcap)
+    return _forward(x, head, None, (ids, logp, tail), softcap, fine) if x.is_cuda else _cpu_kl(x, head, ids, logp, tail, softcap, fine)
 
 
 def head_kl_backward(x, head, ids, logp, tail, stats, dloss, *, softcap: float = 0.0, want_dx: bool = True, want_dhead: bool = True):
@@ -265,9 +278,9 @@ def head_kl_backward(x, head, ids, logp, tail, stats, dloss, *, softcap: float =
 
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, head, softcap, *targets):
+    def forward(ctx, x, head, softcap, fine, *targets):
         refuse_capture(x)
-        loss, stats = (head_cross_entropy if len(targets) == 1 else head_kl)(x, head, *targets, softcap=softcap)
+        loss, stats = (head_cross_entropy if len(targets) == 1 else head_kl)(x, head, *targets, softcap=softcap, fine=fine)
         ctx.save_for_backward(x, head, stats, *targets)
         ctx.softcap = softcap
         return loss
@@ -280,14 +293,14 @@ class _HeadLoss(torch.autograd.Function):
         fn = head_cross_entropy_backward if len(targets) == 1 else head_kl_backward
         dx, dhead = fn(x, head, *targets, stats, dloss.to(stats.dtype), softcap=ctx.softcap, want_dx=ctx.needs_input_grad[0],
                        want_dhead=ctx.needs_input_grad[1])
-        return (dx, dhead, None) + (None,) * len(targets)
+        return (dx, dhead, None, None) + (None,) * len(targets)
 
 
-def head_cross_entropy_loss(x, head, labels, softcap: float = 0.0):
-    """nll [rows], differentiable in ``x`` and ``head``."""
-    return _HeadLoss.apply(x, head, float(softcap), labels)
+def head_cross_entropy_loss(x, head, labels, softcap: float = 0.0, fine: bool = False):
+    """nll [rows], differentiable in ``x`` and ``head``; ``fine`` as in ``head_cross_entropy``."""
+    return _HeadLoss.apply(x, head, float(softcap), fine, labels)
 
 
-def head_kl_loss(x, head, ids, logp, tail, softcap: float = 0.0):
-    """kl [rows], differentiable in ``x`` and ``head``."""
-    return _HeadLoss.apply(x, head, float(softcap), ids, logp, tail)
+def head_kl_loss(x, head, ids, logp, tail, softcap: float = 0.0, fine: bool = False):
+    """kl [rows], differentiable in ``x`` and ``head``; ``fine`` as in ``head_cross_entropy``."""
+    return _HeadLoss.apply(x, head, float(softcap), fine, ids, logp, tail)

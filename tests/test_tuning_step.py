@@ -180,3 +180,35 @@ def test_tuning_step_gpu():
             c, gc = _grads(mc, ids.cuda(), dt, None, 0.3, 9)
             assert torch.allclose(b, c, rtol=1e-5)
             _close(gb, gc, 1e-3)
+
+
+def _capped_objectives(device):
+    """A model whose logits are soft-capped: the tuner's objectives are those of the engine's logits, in fp32 sums over 200 of them."""
+    from volta_engine_b200.runtime.batch import BatchRows
+    from volta_engine_b200.runtime.kv_cache import PagedKVCache
+    model, ids, teacher = _setup(5, logit_softcap=3.0)
+    kv = PagedKVCache(2, 2, 16, 4, 1, 64, "cpu")
+    kv.reserve(0, 41)
+    logits = model.forward(BatchRows.make(ids.tolist(), list(range(40)), [0] * 40, "cpu", G=2, prefill=True), kv)[:, :200].float()
+    assert float(logits.abs().max()) < 3.0
+    m = E.build_from_engine_model(model, (device,)).eval()
+    head, dev = E.scoring_head(m), torch.device(device)
+    t = tuple(v.to(dev) for v in teacher)
+    ce, kl = torch.nn.functional.cross_entropy(logits[:-1], ids[1:]), E.kl_teacher(logits, teacher)
+    with torch.no_grad():
+        # (the engine's layers are bf16: logits off by some 2^-7, losses by less)
+        assert abs(float(E.objective(m, ids.to(dev), None, head)) - float(ce)) < 0.02
+        assert abs(float(E.objective(m, ids.to(dev), t, head)) - float(kl)) < 0.02
+    a, ga = _grads(m, ids.to(dev), t, head)
+    b, gb = _grads(m, ids.to(dev), t, None)
+    assert torch.allclose(a, b, rtol=1e-5)
+    _close(ga, gb, 1e-3)
+
+
+def test_soft_caps_are_part_of_the_objective():
+    _capped_objectives("cpu")
+
+
+@pytest.mark.gpu
+def test_soft_caps_are_part_of_the_objective_gpu():
+    _capped_objectives("cuda:0")

@@ -70,6 +70,10 @@ class TunedNorm(torch.nn.Module):
         return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + self.eps) * (self.w0 + self.delta + self.bias)
 
 
+def soft_capped(logits, cap: float):
+    return cap * torch.tanh(logits / cap) if cap > 0 else logits
+
+
 def _rope(x, pos, theta, rot):
     """x [T, heads, hd], NeoX pairs on the first ``rot`` dims."""
     half = rot // 2
@@ -251,7 +255,7 @@ class TunedModelSP(torch.nn.Module):
 
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
         """-> logits of this rank's rows [T / ranks, vocab]."""
-        return self.states(ids) @ self.head.t()
+        return soft_capped(self.states(ids) @ self.head.t(), self.cfg.logit_softcap)
 
     def sync_grads(self) -> None:
         from ..parallel.sequence_parallel import sum_replicated_grads
@@ -285,7 +289,7 @@ class TunedModel(torch.nn.Module):
         return self.final_norm(h.to(self.devices[-1]))
 
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
-        return self.states(ids) @ self.head.t()
+        return soft_capped(self.states(ids) @ self.head.t(), self.cfg.logit_softcap)
 
 
 def build_from_engine_model(model, devices=("cpu",)) -> TunedModel:
@@ -340,13 +344,13 @@ def objective(model, ids, teacher, head=None) -> torch.Tensor:
     (``scoring_head``): without logits, otherwise (a teacher only) through them. A sequence-parallel model's ranks give parts whose mean that is."""
     if teacher is not None and head is None:
         return kl_teacher(model(ids), teacher)
-    x = model.states(ids)
+    x, cap = model.states(ids), model.cfg.logit_softcap
     if teacher is None:
         labels = torch.cat([ids[1:].long(), torch.full((1,), -100, dtype=torch.int64, device=ids.device)])
         mine, ranks = (labels[model.rows(ids.shape[0])], model.world) if isinstance(model, TunedModelSP) else (labels, 1)
-        return head_cross_entropy_loss(x, head, mine.to(x.device), fine=True).sum() * (ranks / max(1, ids.shape[0] - 1))
+        return head_cross_entropy_loss(x, head, mine.to(x.device), cap, fine=True).sum() * (ranks / max(1, ids.shape[0] - 1))
     t_ids, logp, tail = teacher
-    return head_kl_loss(x[: t_ids.shape[0]], head, t_ids.to(torch.int32), logp.float(), tail.float(), fine=True).mean()
+    return head_kl_loss(x[: t_ids.shape[0]], head, t_ids.to(torch.int32), logp.float(), tail.float(), cap, fine=True).mean()
 
 
 def set_dropout(model, p: float, seed: int, rows: int) -> None:

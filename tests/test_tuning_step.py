@@ -187,18 +187,19 @@ def _capped_objectives(device):
     from volta_engine_b200.runtime.batch import BatchRows
     from volta_engine_b200.runtime.kv_cache import PagedKVCache
     model, ids, teacher = _setup(5, logit_softcap=3.0)
+    model.lm_head.weight.mul_(8)                           # logits that reach the cap
     kv = PagedKVCache(2, 2, 16, 4, 1, 64, "cpu")
     kv.reserve(0, 41)
     logits = model.forward(BatchRows.make(ids.tolist(), list(range(40)), [0] * 40, "cpu", G=2, prefill=True), kv)[:, :200].float()
-    assert float(logits.abs().max()) < 3.0
+    assert 2.9 < float(logits.abs().max()) <= 3.0
     m = E.build_from_engine_model(model, (device,)).eval()
     head, dev = E.scoring_head(m), torch.device(device)
     t = tuple(v.to(dev) for v in teacher)
     ce, kl = torch.nn.functional.cross_entropy(logits[:-1], ids[1:]), E.kl_teacher(logits, teacher)
     with torch.no_grad():
-        # (the engine's layers are bf16: logits off by some 2^-7, losses by less)
-        assert abs(float(E.objective(m, ids.to(dev), None, head)) - float(ce)) < 0.02
-        assert abs(float(E.objective(m, ids.to(dev), t, head)) - float(kl)) < 0.02
+        # (the engine's layers are bf16: logits in front of the cap, 5 to 10 here, off by some 2^-8 of theirs, the means of 40 losses by less)
+        assert abs(float(E.objective(m, ids.to(dev), None, head)) - float(ce)) < 0.04
+        assert abs(float(E.objective(m, ids.to(dev), t, head)) - float(kl)) < 0.04
     a, ga = _grads(m, ids.to(dev), t, head)
     b, gb = _grads(m, ids.to(dev), t, None)
     assert torch.allclose(a, b, rtol=1e-5)

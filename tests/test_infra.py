@@ -92,3 +92,22 @@ def test_every_programmatically_launched_kernel_waits_for_its_predecessor():
             assert "grid_dep_wait" in src[i:j], f"{os.path.basename(path)}: {name} is launched programmatically but never waits"
             seen += 1
     assert seen >= 20
+
+
+def test_status_words_are_the_devices():
+    """A device given without its index is the current one: the word that kernels wrote is the word that is looked at."""
+    from unittest import mock
+    import torch
+    from volta_engine_b200.ops import kernels as K
+    made = []
+
+    def zeros(n, dtype, device):
+        made.append(device)
+        return torch.tensor([0], dtype=dtype)
+    with mock.patch.object(K, "_status", {}), mock.patch.object(torch.cuda, "current_device", lambda: 1), mock.patch.object(K.torch, "zeros", zeros):
+        word = K.status_word(torch.device("cuda", 1))
+        assert K.status_word("cuda") is word and K.status_word("cuda:1") is word and K.status_word(torch.device("cuda")) is word
+        assert K.status_word("cuda:0") is not word and K.status_word("cpu") is not word
+        assert made == [torch.device("cuda", 1), torch.device("cuda", 0), torch.device("cpu")]
+        word[0] = 3
+        assert [K.check_status(d) for d in ("cuda", torch.device("cuda"), "cuda:1", "cuda:0", "cuda:2", "cpu")] == [3, 3, 3, 0, 0, 0]

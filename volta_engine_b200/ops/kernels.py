@@ -41,18 +41,23 @@ def _ws(name, shape, dtype, device, zero=False):
     return t.zero_() if zero else t
 
 
+def _status_device(device) -> torch.device:
+    d = torch.device(device)
+    return torch.device("cuda", torch.cuda.current_device()) if d.type == "cuda" and d.index is None else d      # ("cuda": the current one)
+
+
 def status_word(device) -> torch.Tensor:
     """Per-device int32 word that kernels set when a bounded wait expires (0 = healthy)."""
-    key = str(device)
+    key = _status_device(device)
     t = _status.get(key)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=device)
+        t = torch.zeros(1, dtype=torch.int32, device=key)
         _status[key] = t
     return t
 
 
 def check_status(device) -> int:
-    t = _status.get(str(device))
+    t = _status.get(_status_device(device))
     return int(t.item()) if t is not None else 0
 
 

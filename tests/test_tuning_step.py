@@ -213,3 +213,17 @@ def test_soft_caps_are_part_of_the_objective():
 @pytest.mark.gpu
 def test_soft_caps_are_part_of_the_objective_gpu():
     _capped_objectives("cuda:0")
+
+
+def test_a_teacher_file_called_labels_is_a_teacher(tmp_path, monkeypatch, capsys):
+    from volta_engine_b200.models.factory import save_dense_checkpoint
+    cfg = DenseConfig(n_layers=1, hidden=64, n_q=2, n_kv=1, head_dim=32, ffn=64, vocab=50)
+    save_dense_checkpoint(tmp_path / "src", cfg, seed=5, fmt="bf16", std=0.08)
+    g = torch.Generator().manual_seed(2)
+    seqs = [torch.randint(0, 50, (8,), generator=g, dtype=torch.int32) for _ in range(2)]
+    torch.save(seqs, tmp_path / "seqs.pt")
+    monkeypatch.chdir(tmp_path)
+    args = ["--model", "src", "--inputs", "seqs.pt", "--teacher", "labels", "--out", "out", "--steps", "1", "--batch", "1"]
+    assert E.main(args) == 0 and "held-out cross entropy" in capsys.readouterr().out
+    torch.save([torch.randn(8, 50, generator=g) for _ in seqs], tmp_path / "labels")
+    assert E.main(args) == 0 and "held-out KL" in capsys.readouterr().out

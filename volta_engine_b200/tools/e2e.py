@@ -513,7 +513,8 @@ def main(argv=None) -> int:
     seqs = torch.load(a.inputs, weights_only=True)
     if not (0 <= a.dropout <= 1 and 0 <= a.seed < 1 << 32):
         ap.error("--dropout takes 0 to 1, --seed 0 to 2^32 - 1")
-    if a.teacher == "labels":
+    labels = a.teacher == "labels" and not Path(a.teacher).exists()              # (a file or directory of that name is a teacher)
+    if labels:
         teachers = [None] * len(seqs)
     elif Path(a.teacher).is_dir():
         tmodel, _ = load_model(a.teacher, "cpu", None)
@@ -557,7 +558,7 @@ def main(argv=None) -> int:
         tensors[f"layers.{li}.attn_norm.weight"] = (L.n1.w0 + L.n1.delta).detach().half().cpu()
         tensors[f"layers.{li}.ffn_norm.weight"] = (L.n2.w0 + L.n2.delta).detach().half().cpu()
     write_safetensors(out / "e2e_scales.safetensors", tensors)
-    print(f"held-out {'cross entropy' if a.teacher == 'labels' else 'KL'} {hist['eval'][0][1]:.6f} -> {hist['eval'][-1][1]:.6f}")
+    print(f"held-out {'cross entropy' if labels else 'KL'} {hist['eval'][0][1]:.6f} -> {hist['eval'][-1][1]:.6f}")
     return 0
 
 

@@ -227,3 +227,19 @@ def test_a_teacher_file_called_labels_is_a_teacher(tmp_path, monkeypatch, capsys
     assert E.main(args) == 0 and "held-out cross entropy" in capsys.readouterr().out
     torch.save([torch.randn(8, 50, generator=g) for _ in seqs], tmp_path / "labels")
     assert E.main(args) == 0 and "held-out KL" in capsys.readouterr().out
+
+
+def test_ppl_without_logits_takes_the_teachers_that_it_takes_with_them(tmp_path, capsys):
+    """Ids of 64 bits and log-probabilities of 16 and 64, as other programs write them."""
+    from volta_engine_b200.models.factory import save_dense_checkpoint
+    cfg = DenseConfig(n_layers=1, hidden=64, n_q=2, n_kv=1, head_dim=32, ffn=64, vocab=50)
+    save_dense_checkpoint(tmp_path / "src", cfg, seed=5, fmt="bf16", std=0.08)
+    g = torch.Generator().manual_seed(2)
+    torch.save([torch.randint(0, 50, (24,), generator=g, dtype=torch.int32)], tmp_path / "tok.pt")
+    base = ["--model", str(tmp_path / "src"), "--tokens-file", str(tmp_path / "tok.pt"), "--device", "cpu"]
+    for it, ft in ((torch.int64, torch.float64), (torch.int32, torch.float16)):
+        ids, logp, tail = topk_teacher(2 * torch.randn(24, 50, generator=g), 4)
+        torch.save({"k": 4, "ids": [ids.to(it)], "logp": [logp.to(ft)], "tail": [tail.to(ft)]}, tmp_path / "t.pt")
+        a, b = (_ppl(base + ["--kl-teacher", str(tmp_path / "t.pt")] + more, capsys) for more in ([], ["--no-logits"]))
+        # (what float16 loses of its log-probabilities both read alike; their sums are in its 2^-11 where logits are held)
+        assert abs(a["kl"] - b["kl"]) < (1e-4 if ft == torch.float64 else 2.0 ** -8 * a["kl"])

@@ -140,7 +140,7 @@ def run(engine, seqs, chunk: int = 512, topk: int = 0, teacher: dict | None = No
                 if x is None:
                     kl = kl_topk(lg[: t_ids.shape[0]], t_ids, t_lp, t_tail)
                 else:
-                    kl = head_kl(x[: t_ids.shape[0]], head, t_ids, t_lp, t_tail, softcap=cap)[0]
+                    kl = head_kl(x[: t_ids.shape[0]], head, t_ids.to(torch.int32), t_lp.float(), t_tail.float(), softcap=cap)[0]
                 kl_sum += float(kl.sum())
                 kl_n += kl.numel()
             if out_t is not None:

@@ -566,3 +566,10 @@ def test_fine_statistics_keep_what_sums_lose(topk, vocab):
     xs = x.clone().requires_grad_()
     (L.head_cross_entropy_loss if not topk else L.head_kl_loss)(xs, head, *t, fine=True).backward(dl)
     assert torch.equal(xs.grad, b(x, head, *t, s2, dl, want_dhead=False)[0])
+
+
+def test_sizes_that_tiles_do_not_count_are_refused():
+    for rows, vocab in (((1 << 24) - 255, 2), (2, 1 << 24)):
+        x, head = torch.zeros(1, 8).expand(rows, 8), torch.zeros(1, 8).expand(vocab, 8)
+        with pytest.raises(ValueError, match="below 2"):
+            L.head_cross_entropy(x, head, torch.zeros(1, dtype=torch.int64).expand(rows))

@@ -11,10 +11,12 @@ K most likely tokens and the mass of the rest (what ``volta_ppl --topk-out`` wri
 
 Rows that do not count: a negative label, or a teacher row whose ids are all negative (single negative ids are padding). Their loss, statistics and
 gradients are zero and their states are not read. An id listed twice is one token whose teacher's mass is the sum. A label or id at or behind
-``vocab`` makes the row's loss NaN (and with it the gradients it takes part in): the ids stay on the device, nothing waits to look at them.
+``vocab`` makes the row's loss NaN (and with it the gradients it takes part in): the ids stay on the device, nothing waits to look at them. NaN among a
+row's logits or its teacher's numbers is its loss.
 
 GPU tensors use csrc/cuda/head_loss.cu: the explicit forward / backward pairs launch on the current stream of the tensors' device, take their
-workspace from the caching allocator and may be captured into a CUDA graph. CPU tensors run the same arithmetic in PyTorch (fp64 stays fp64).
+workspace from the caching allocator and may be captured into a CUDA graph. The same call gives the same bits; between calls of few and of many rows the last
+bits of a row's loss may differ (sums of exponentials by blocks of 32 tokens, or of 128). CPU tensors run the same arithmetic in PyTorch (fp64 stays fp64).
 ``head_cross_entropy_loss`` and ``head_kl_loss`` are the pairs as one differentiable call.
 """
 from __future__ import annotations
@@ -42,8 +44,8 @@ def _check(x, head, softcap, others, dloss=None, stats=None):
     rows, vocab, device = x.shape[0], head.shape[0], x.device
     if vocab < 1 or x.shape[1] < 1:
         raise ValueError(f"a head of {tuple(head.shape)} has no logits")
-    if rows >= 1 << 24 or vocab >= 1 << 24:
-        raise ValueError("rows and vocabulary have to stay below 2^24")
+    if rows > (1 << 24) - 256 or vocab >= 1 << 24:            # (rows are padded to whole tiles of 256)
+        raise ValueError("rows have to stay below 2^24 - 255, the vocabulary below 2^24")
     allowed = _DTYPES if x.is_cuda else _DTYPES + (torch.float64,)
     if x.dtype not in allowed:
         raise TypeError(f"states of type {x.dtype}: bf16 and fp32 are supported")

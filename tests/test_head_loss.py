@@ -420,9 +420,9 @@ def beside_rounding(got, want):
                                                             (300, 264, 20100, 16, 0.0)])
 def test_bf16_gradients_are_off_by_their_rounding(rows, hidden, vocab, topk, softcap):
     """Rows of dx and dhead (those of nobody's label too) in 47 to 682 blocks of 64 columns, in ranges of the vocabulary, in two pieces of it, with a cap:
-    what stands in front of the last rounding adds less than a tenth to it. dz comes in two slabs, 2^-18 of a value, where the result's rounding is 2^-9
-    of its own, and a common part of three times the spread makes 2^-18 of dz about 2^-16 of dx; the logits' share is below 2^-13 of s, an
-    eighth of the rounding even beside that part: sqrt(1 + 1/64). Near a teacher (noise 0.1) a row's dz is a difference of two nearly equal shares, in some
+    what stands in front of the last rounding adds less than a tenth to it. dz comes in two slabs, 2^-16 of a value, where the result's rounding is 2^-8
+    of its own, and a common part of three times the spread makes 2^-16 of dz about 2^-14 of dx; the logits' share is below 2^-14 of s, 2^-12 beside
+    that part, an eighth of the rounding (2^-9 as a root mean square): sqrt(1 + 1/64). Near a teacher (noise 0.1) a row's dz is a difference of two nearly equal shares, in some
     rows to the logits' own error: the middle row is looked at."""
     a = near(rows, hidden, vocab, topk, 0.1, 3.0, "cuda")
     got, want = run(*a, softcap), P.wanted(*a, softcap)

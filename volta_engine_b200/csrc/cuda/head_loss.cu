@@ -13,7 +13,7 @@
 // out of the sums so that log(1 + exp(..)) and log(rho) do not come from the difference of two nearly equal numbers. The gradient computes the
 // logits again, a piece of the vocabulary at a time, writes dz of that piece in bf16 slabs (rows x piece: the only array of that kind) and
 // multiplies it with the head's rows and with the states. dz beside fp32 operands is three bf16 slabs (fp32's 24 bits), beside bf16 operands two
-// (2^-18 of a value, and gradients are rounded to 2^-9 of theirs). One slab alone would be 2^-9 off as the gradients are, but of every addend: a row of dz
+// (2^-16 of a value, and gradients are rounded to 2^-8 of theirs). One slab alone would be 2^-8 off as the gradients are, but of every addend: a row of dz
 // sums to zero, so what the head's rows have in common leaves dx except for that rounding, and near a teacher the addends are far above their sum
 // (errors of 2 to 6 times the gradients' own rounding; rows of dhead 1.3 to 2.9 times it).
 // Sums run in a fixed order: the same call gives the same bits.
